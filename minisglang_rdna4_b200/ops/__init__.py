@@ -20,6 +20,12 @@ def _cuda():
     return cuda
 
 
+def _ref_fp4():
+    from . import ref_fp4
+
+    return ref_fp4
+
+
 # ---------------------------------------------------------------------------- elementwise
 def embedding(ids, weight, vocab_start: int = 0, vocab_len: Optional[int] = None):
     if weight.is_cuda:
@@ -146,6 +152,125 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, seq_lens, scale: flo
                                        quant=quant)
     return ref.paged_attention(q, k_cache, v_cache, block_table, cu_q, seq_lens, scale, causal, window,
                                mask, k_scale, v_scale, mask_window, chunk, softcap, gate, bias, sink, talk)
+
+
+# ---------------------------------------------------------------------------- K/V pool of 4 bits
+def store_kv_fp4(k, v, cache, out_loc, k_scale=None, v_scale=None, weights=None) -> None:
+    """Quantises rows ``k``, ``v [T, Hk, D]`` (bf16 or fp16, any row stride) and writes them to the token slots ``out_loc [T]``
+    (int32) of a pool of 4 bits: ``cache [pages, Hk, page / 16, 18 D]`` bytes (D 64, 128 or 256).
+
+    A value is an e2m1 code times an e4m3 scale of its 16 channels times the head's ``k_scale`` / ``v_scale [Hk]`` (fp32,
+    positive; None: 1). Blocks whose magnitude passes ``2688 scale`` saturate; a NaN makes its block NaN. ``weights [pages, Hk,
+    page]`` (fp32): the slots' attention weights start at zero. Slots outside the pool are skipped; of a slot that is named
+    twice any of the rows' blocks may stay."""
+    from . import kv_fp4 as F4
+
+    _, pages, hk, page, dim = F4.pool_shape(cache)
+    F4.check_here(cache, k, v, out_loc, k_scale, v_scale, weights)
+    F4.check_ints("out_loc", out_loc, None)
+    F4.check_rows("k", k, out_loc.numel(), hk, dim)
+    F4.check_rows("v", v, out_loc.numel(), hk, dim)
+    if k.dtype != v.dtype:
+        raise TypeError(f"k is {k.dtype} and v is {v.dtype}")
+    F4.check_heads("k_scale", k_scale, hk)
+    F4.check_heads("v_scale", v_scale, hk)
+    if weights is not None:
+        F4.check_weights(weights, cache, pages, hk, page)
+    (F4 if cache.is_cuda else _ref_fp4()).store_kv_fp4(k, v, cache, out_loc, k_scale, v_scale, weights)
+
+
+def load_kv_fp4(cache, slots, k_scale=None, v_scale=None, dtype: torch.dtype = torch.bfloat16):
+    """Keys and values ``[T, Hk, D]`` of the token slots ``slots [T]`` (int32) in ``dtype`` (bf16 or fp16, rounded once). With
+    layers in front of the pool's shape, ``[layers, T, Hk, D]``. Slots outside the pool give zeros."""
+    from . import kv_fp4 as F4
+
+    hk = F4.pool_shape(cache, True)[2]
+    F4.check_here(cache, slots, k_scale, v_scale)
+    F4.check_ints("slots", slots, None)
+    F4.check_heads("k_scale", k_scale, hk)
+    F4.check_heads("v_scale", v_scale, hk)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"load_kv_fp4 gives bf16 or fp16, not {dtype}")
+    return (F4 if cache.is_cuda else _ref_fp4()).load_kv_fp4(cache, slots, k_scale, v_scale, dtype)
+
+
+def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, k_scale=None, v_scale=None, window: int = 0,
+                        max_q: int = 0, max_kv: int = 0, weights=None, plan=None, workspace=None):
+    """Causal attention over a pool of 4 bits (``store_kv_fp4``): decode steps, prompts behind a prefix, rows that look back.
+
+    ``q [T, Hq, D]`` (bf16 or fp16); request b has the rows ``cu_q[b]:cu_q[b + 1]`` (int32), the last positions of its
+    ``seq_lens[b]`` tokens, whose pages are ``block_table[b]`` (int32). ``window`` > 0: a row sees that many positions, its own
+    included. A row that sees nothing gives zeros. ``max_q`` (rows of the longest request; 0: read from the device) may be
+    larger than what the step has; ``max_kv`` likewise.
+
+    ``weights [pages, Hk, page]`` (fp32): the softmax weights that the rows give a token, summed over the rows and the query
+    heads of its key head, are added to the token's. (A page that several requests of the step share has them added in any
+    order.) ``plan``: ``prefill_plan_fp4``; it may be used by a step without ``weights``. ``workspace``: fp32, for parts of split
+    requests; one that is too small is replaced for the call."""
+    from . import kv_fp4 as F4
+
+    _, pages, hk, page, dim = F4.pool_shape(cache)
+    F4.check_here(cache, q, block_table, cu_q, seq_lens, k_scale, v_scale, weights)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"queries of bf16 or fp16, not {q.dtype}")
+    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % hk or q.shape[1] == 0:
+        raise ValueError(f"q is [T, a multiple of {hk}, {dim}], not {tuple(q.shape)}")
+    F4.check_ints("seq_lens", seq_lens, None)
+    F4.check_ints("cu_q", cu_q, seq_lens.numel() + 1)
+    F4.check_ints("block_table", block_table, seq_lens.numel(), None)
+    F4.check_heads("k_scale", k_scale, hk)
+    F4.check_heads("v_scale", v_scale, hk)
+    if window < 0 or max_q < 0 or max_kv < 0:
+        raise ValueError("window, max_q and max_kv are not negative")
+    if weights is not None:
+        F4.check_weights(weights, cache, pages, hk, page)
+        if plan is not None:
+            raise ValueError("a step that adds to attention weights takes no prefill plan")
+    if cache.is_cuda:
+        return F4.paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, max_kv, weights,
+                                      plan, workspace)
+    return _ref_fp4().paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, weights)
+
+
+def prefill_plan_fp4(q, cache, cu_q, seq_lens, window: int = 0):
+    """Tables of a prompt step for ``paged_attention_fp4``, for all layers of the step; ``cu_q`` and ``seq_lens`` are the lengths
+    on the host (numpy). ``None`` where the step does not take the form for prompts (CPU, few rows for the keys in sight,
+    shapes that it does not have)."""
+    from . import kv_fp4 as F4
+
+    F4.pool_shape(cache)
+    return F4.prefill_plan_fp4(q, cache, cu_q, seq_lens, window) if cache.is_cuda else None
+
+
+def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, recent: int, sinks: int = 0, max_kv: int = 0):
+    """Cuts requests down to ``budget`` tokens per key head by their accumulated attention weights.
+
+    ``cache [pages, Hk, page / 16, 18 D]``, ``weights [pages, Hk, page]``, or both with layers in front. A request of more than
+    ``budget`` tokens (``seq_lens [B]``, pages ``block_table [B, .]``) keeps, in every layer and key head on its own, its first
+    ``sinks``, its last ``recent``, and of the others those with the largest weights (of equal ones the earlier; a NaN is
+    larger than any number); a shorter one keeps all. What stays is copied in its order, rows and weights, to the pages
+    ``new_table [B, at least budget / page]``, which must not be among the pages of any request here; slots behind it and the old
+    pages stay as they are. ``max_kv``: an upper bound of ``seq_lens`` (0: what the table holds).
+
+    Returns ``(kept [(layers,) B, Hk, budget] int32: token indices in order, -1 behind them, new lengths [B] int32)``. Later steps
+    go on behind the new lengths, at the positions that their tokens have in the text."""
+    from . import kv_fp4 as F4
+
+    _, pages, hk, page, _ = F4.pool_shape(cache, True)
+    F4.check_here(cache, weights, block_table, seq_lens, new_table)
+    F4.check_weights(weights, cache, pages, hk, page)
+    F4.check_ints("seq_lens", seq_lens, None)
+    F4.check_ints("block_table", block_table, seq_lens.numel(), None)
+    F4.check_ints("new_table", new_table, seq_lens.numel(), None)
+    if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError(f"a budget of {budget} with {sinks} first and {recent} last tokens")
+    if new_table.shape[1] * page < budget or block_table.shape[1] < 1:
+        raise ValueError(f"new pages for {new_table.shape[1] * page} tokens, a budget of {budget}")
+    if max_kv < 0:
+        raise ValueError("max_kv is not negative")
+    if cache.is_cuda:
+        return F4.evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv)
+    return _ref_fp4().evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks)
 
 
 # ---------------------------------------------------------------------------- GEMMs

@@ -1,0 +1,141 @@
+"""Python side of the paged K/V pool of 4 bits: checks of arguments, and the kernels of ``csrc/kv_fp4.cu`` and
+``csrc/attention_fp4.cu``. The checks hold on the CPU path too (``ops.ref_fp4``)."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from . import cuda as K
+from ._lib import c_f, c_i, c_ll, c_p, check, lib
+
+_lib.bind("msgl_store_fp4", c_i, [c_p, c_p, c_ll, c_ll] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
+_lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
+_lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 8 + [c_p])
+_lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_i] + [c_p] * 5 + [c_i] * 7 + [c_f, c_i, c_p])
+
+TILE = 16                       # tokens of a tile
+WIDTHS = (64, 128, 256)
+_ROWS = (torch.bfloat16, torch.float16)
+
+
+def tile_bytes(dim: int) -> int:
+    """Bytes of 16 tokens of one head: codes of keys and values (8 D each) and their scales (D each)."""
+    return 18 * dim
+
+
+def pool_shape(cache: torch.Tensor, layered: bool = False) -> Tuple[int, int, int, int, int]:
+    """``(layers, pages, heads, page size, D)`` of ``[pages, heads, page / 16, 18 D]`` bytes (``layered``: with or without
+    layers in front)."""
+    if cache.dtype != torch.uint8 or cache.dim() not in ((4, 5) if layered else (4,)):
+        raise ValueError("a 4-bit K/V pool is uint8 [pages, heads, page / 16, 18 D]" + (", layers in front" if layered else ""))
+    layers = cache.shape[0] if cache.dim() == 5 else 1
+    pages, hk, tiles, width = cache.shape[-4:]
+    dim = width // 18
+    if dim not in WIDTHS or width % 18 or tiles < 1 or hk < 1 or pages < 1:
+        raise ValueError(f"a 4-bit K/V pool has heads of 64, 128 or 256 channels (tiles of 18 D bytes), not tiles of {width} bytes")
+    one = cache[0] if cache.dim() == 5 else cache
+    if not one.is_contiguous() or (cache.dim() == 5 and cache.stride(0) % 16) or cache.data_ptr() % 16:
+        raise ValueError("the layers of a 4-bit K/V pool are contiguous, on 16-byte boundaries")
+    return layers, pages, hk, tiles * TILE, dim
+
+
+def check_here(*tensors: Optional[torch.Tensor]) -> None:
+    """All on one device, on a GPU the current one: the kernels go to its current stream."""
+    first = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != first:
+            raise ValueError(f"tensors on {first} and {t.device}")
+    if first.type == "cuda" and first.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on {first}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def check_ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> None:
+    if t.dtype != torch.int32 or t.dim() != len(shape) or any(s is not None and s != x for s, x in zip(shape, t.shape)):
+        raise ValueError(f"{name} is int32 of shape {tuple('any' if s is None else s for s in shape)}, not {t.dtype} {tuple(t.shape)}")
+
+
+def check_heads(name: str, t: Optional[torch.Tensor], hk: int) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.shape != (hk,) or not t.is_contiguous()):
+        raise ValueError(f"{name} is fp32 [{hk}], one factor per key / value head")
+
+
+def check_weights(weights: torch.Tensor, cache: torch.Tensor, pages: int, hk: int, page: int) -> None:
+    want = (cache.shape[0],) * (cache.dim() == 5) + (pages, hk, page)
+    one = weights[0] if weights.dim() == 4 else weights
+    if weights.dtype != torch.float32 or tuple(weights.shape) != want or not one.is_contiguous():
+        raise ValueError(f"attention weights are contiguous fp32 {want}, not {weights.dtype} {tuple(weights.shape)}")
+
+
+def check_rows(name: str, x: torch.Tensor, rows: int, hk: int, dim: int) -> None:
+    if x.dtype not in _ROWS:
+        raise TypeError(f"{name}: rows of bf16 or fp16, not {x.dtype}")
+    if x.dim() not in (2, 3) or x.shape[0] != rows or x.numel() != rows * hk * dim:
+        raise ValueError(f"{name} is [{rows}, {hk}, {dim}], not {tuple(x.shape)}")
+
+
+def _row_view(x: torch.Tensor, hk: int, dim: int) -> torch.Tensor:
+    """``[rows, hk * dim]`` whose rows the kernel reads where they lie if they may (16-byte steps), else a copy."""
+    if x.dim() == 3:
+        x = x.flatten(1) if x.stride(1) != dim or x.stride(2) != 1 else x.as_strided((x.shape[0], hk * dim), (x.stride(0), 1))
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def store_kv_fp4(k, v, cache, out_loc, k_scale=None, v_scale=None, weights=None):
+    _, pages, hk, page, dim = pool_shape(cache)
+    t = out_loc.numel()
+    k, v = _row_view(k, hk, dim), _row_view(v, hk, dim)
+    out_loc = out_loc.contiguous()
+    check(lib().msgl_store_fp4(
+        k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), cache.data_ptr(), out_loc.data_ptr(), K._p(k_scale), K._p(v_scale),
+        K._p(weights), t, hk, dim, page, pages, K._dt(k), K._stream()), "store_kv_fp4")
+    K._count("store_kv_fp4", "store_fp4_kernel")
+
+
+def load_kv_fp4(cache, slots, k_scale, v_scale, dtype):
+    layers, pages, hk, page, dim = pool_shape(cache, True)
+    slots = slots.contiguous()
+    lead = (layers,) if cache.dim() == 5 else ()
+    k, v = (torch.empty(*lead, slots.numel(), hk, dim, dtype=dtype, device=cache.device) for _ in (0, 1))
+    check(lib().msgl_load_fp4(cache.data_ptr(), cache.stride(0) if lead else 0, layers, slots.data_ptr(), K._p(k_scale),
+                              K._p(v_scale), k.data_ptr(), v.data_ptr(), slots.numel(), hk, dim, page, pages, K._dt(k),
+                              K._stream()), "load_kv_fp4")
+    K._count("load_kv_fp4", "load_fp4_kernel")
+    return k, v
+
+
+def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv):
+    layers, pages, hk, page, dim = pool_shape(cache, True)
+    lead = (layers,) if cache.dim() == 5 else ()
+    b = seq_lens.numel()
+    block_table, seq_lens, new_table = block_table.contiguous(), seq_lens.contiguous(), new_table.contiguous()
+    kept = torch.empty(*lead, b, hk, budget, dtype=torch.int32, device=cache.device)
+    lens = torch.empty(b, dtype=torch.int32, device=cache.device)
+    check(lib().msgl_evict_fp4(
+        cache.data_ptr(), cache.stride(0) if lead else 0, weights.data_ptr(), weights.stride(0) if lead else 0, layers,
+        block_table.data_ptr(), block_table.shape[1], new_table.data_ptr(), new_table.shape[1], seq_lens.data_ptr(),
+        kept.data_ptr(), lens.data_ptr(), b, hk, dim, page, pages, budget, recent, sinks, K._stream()), "evict_kv_fp4")
+    K._count("evict_kv_fp4", "evict_select_kernel + evict_move_kernel", 2)
+    return kept, lens
+
+
+def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, max_kv, weights, plan,
+                        workspace):
+    _, pages, hk, page, dim = pool_shape(cache)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_like(q)
+    block_table, cu_q, seq_lens = block_table.contiguous(), cu_q.contiguous(), seq_lens.contiguous()
+    check(lib().msgl_attention_fp4(
+        q.data_ptr(), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(),
+        seq_lens.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights), seq_lens.numel(), q.shape[1], hk, dim, page, pages, window,
+        scale, K._dt(q), K._stream()), "paged_attention_fp4")
+    K._count("paged_attention_fp4", "fp4_attention_simple_kernel")
+    return out
+
+
+def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
+    return None

@@ -1,0 +1,377 @@
+"""Kernels of the paged K/V pool of 4 bits against loops in 64 bits (``plain_kv_fp4``)."""
+import math
+
+import pytest
+import torch
+
+import plain_kv_fp4 as plain
+from minisglang_rdna4_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def make(pages, hk, page, dim, seed=0, powers=True):
+    """A pool that the store filled with random rows, and the factors of its heads."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    cache = torch.zeros(pages, hk, page // 16, 18 * dim, dtype=torch.uint8, device="cuda")
+    if powers:
+        ks, vs = (2.0 ** torch.randint(lo, lo + 3, (hk,), generator=g, device="cuda") for lo in (-6, -8))
+    else:
+        ks, vs = (0.02 + 0.01 * torch.rand(hk, generator=g, device="cuda") for _ in range(2))
+    k, v = (torch.randn(pages * page, hk, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    k[..., 5::31] *= 5
+    ops.store_kv_fp4(k, v, cache, torch.arange(pages * page, dtype=torch.int32, device="cuda"), ks, vs)
+    return cache, ks, vs, k, v
+
+
+def tables(lens, page, spare=2, seed=0, width=None):
+    """Pages in a random order; unused entries name the last page."""
+    need = [-(-n // page) for n in lens]
+    total = sum(need) + spare
+    order = torch.randperm(total, generator=torch.Generator().manual_seed(seed)).tolist()
+    width = width or max(need + [1])
+    rows, at = [], 0
+    for n in need:
+        rows.append(order[at:at + n] + [order[-1]] * (width - n))
+        at += n
+    return ints(rows), total
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hk,page", [(1, 16), (3, 48), (8, 64)])
+@pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16"])
+def test_store_and_load(dim, hk, page, dtype):
+    torch.manual_seed(dim + hk)
+    pages, rows = 5, 2 * page + 5
+    cache = torch.full((pages, hk, page // 16, 18 * dim), 0x11, dtype=torch.uint8, device="cuda")
+    before = plain.values(cache)
+    ks, vs = 2.0 ** torch.randint(-6, -2, (hk,), device="cuda"), 2.0 ** torch.randint(-9, -5, (hk,), device="cuda")
+    # rows of a projection: keys and values lie in wider rows
+    wide = torch.randn(rows, 2 * hk * dim + 24, device="cuda").to(dtype)
+    k, v = wide[:, 8:8 + hk * dim], wide[:, 8 + hk * dim:8 + 2 * hk * dim]
+    loc = torch.randperm(pages * page, device="cuda")[:rows].int()
+    loc[3], loc[7] = -1, pages * page
+    weights = torch.ones(pages, hk, page, device="cuda")
+    ops.store_kv_fp4(k, v, cache, loc, ks, vs, weights)
+    inside = (loc >= 0) & (loc < pages * page)
+    at = loc[inside].long().cpu()
+    got = plain.values(cache, ks, vs)
+    for x, y, old, head in zip(got, (k, v), before, (ks, vs)):
+        want = (old * head.cpu().double()[:, None, None]).transpose(1, 2).flatten(0, 1)
+        want[at] = plain.rounded(y.reshape(rows, hk, dim)[inside], head)
+        assert torch.equal(x.transpose(1, 2).flatten(0, 1), want)
+    assert torch.equal(weights.transpose(1, 2).flatten(0, 1).cpu()[at], torch.zeros(len(at), hk))
+    assert int(weights.sum()) == (pages * page - len(at)) * hk
+    back = ops.load_kv_fp4(cache, loc, ks, vs, dtype)
+    for x, y in zip(back, got):
+        want = torch.zeros(rows, hk, dim, dtype=torch.float64)
+        want[inside.cpu()] = y.transpose(1, 2).flatten(0, 1)[at]
+        assert torch.equal(x.cpu().double(), want.to(dtype).double())
+    # rows that do not lie on 16 bytes, and a copy's
+    odd = torch.randn(rows, hk * dim + 3, device="cuda").to(dtype)[:, 3:]
+    ops.store_kv_fp4(odd, odd, cache, loc, ks, vs)
+    first = cache.clone()
+    ops.store_kv_fp4(odd.contiguous().view(rows, hk, dim), odd.contiguous().view(rows, hk, dim), cache, loc, ks, vs)
+    assert torch.equal(first, cache)
+
+
+def test_store_of_special_rows():
+    # (2 alone in its block: 2 / 6 lies between the scales 0.3125 and 0.34375, nearer to the second, 6 times which is held)
+    cache = torch.full((1, 1, 1, 18 * 64), 0x55, dtype=torch.uint8, device="cuda")
+    k = torch.zeros(4, 1, 64, device="cuda")
+    k[1, 0, :3] = torch.tensor([1e30, -1e30, 1.0])
+    k[2, 0, 20], k[2, 0, 40], k[3, 0] = math.nan, 2.0, 1e-30
+    k = k.bfloat16()
+    ops.store_kv_fp4(k, k, cache, ints([0, 1, 2, 3]))
+    for x in plain.values(cache):
+        x = x[0, 0]
+        assert (x[0] == 0).all() and (x[3] == 0).all() and x[1, :3].tolist() == [2688.0, -2688.0, 0.0]
+        assert x[2, 16:32].isnan().all() and x[2, 40] == 6 * 0.34375 and not x[2, 32:].isnan().any()
+    k[0, 0, 0] = math.inf
+    ops.store_kv_fp4(k[:1], k[:1], cache, ints([0]))
+    assert plain.values(cache)[0][0, 0, 0, 0] == 2688.0
+
+
+def attend(lens, news, hq, hk, dim, dtype=torch.bfloat16, page=16, window=0, weighed=False, seed=0, powers=True, scale=None, **kw):
+    table, pages = tables(lens, page, seed=seed)
+    cache, ks, vs, _, _ = make(pages, hk, page, dim, seed, powers)
+    g = torch.Generator("cuda").manual_seed(seed + 1)
+    cu = ints([0] + torch.tensor(news).cumsum(0).tolist())
+    q = torch.randn(sum(news), hq, dim, generator=g, device="cuda").to(dtype)
+    weights = torch.rand(pages, hk, page, generator=g, device="cuda") if weighed else None
+    before = weights.clone() if weighed else None
+    scale = scale or dim ** -0.5
+    lens = ints(lens)
+    out = ops.paged_attention_fp4(q, cache, table, cu, lens, scale, k_scale=ks, v_scale=vs, window=window, weights=weights,
+                                  **{"max_q": max(news), "max_kv": int(lens.max()), **kw})
+    want, tol, w, w_tol = plain.attention(q, *plain.values(cache, ks, vs), table, cu, lens, scale, window)
+    assert torch.isfinite(out).all()
+    assert ((out.cpu().double() - want).abs() <= tol).all(), float(((out.cpu().double() - want).abs() / tol).max())
+    if weighed:
+        expect, room = before.cpu().double(), torch.zeros(before.shape, dtype=torch.float64)
+        for b, n in enumerate(lens.tolist()):
+            i = torch.arange(n)
+            at = (table[b].cpu().long()[i // page], slice(None), i % page)
+            expect[at] += w[b].T
+            room[at] += w_tol[b].T
+        room = room + expect * 2.0 ** -22                     # sums over the heads and with what was there
+        off = (weights.cpu().double() - expect).abs()
+        assert (off <= room).all(), float((off / room).max())
+        assert torch.equal(weights.cpu()[room == 0], before.cpu()[room == 0])
+    return out
+
+
+DECODE = {
+    "one": [1], "tile": [16], "over": [17], "edges": [15, 16, 17, 31, 32, 33, 63, 64, 65], "none": [0, 5, 0], "alone": [700],
+    "ragged": [90, 3500, 64, 1, 1200, 65, 2500, 0, 333], "many": [(37 * i) % 300 + 1 for i in range(200)], "long": [20011],
+}
+
+
+@pytest.mark.parametrize("lens", DECODE.values(), ids=DECODE.keys())
+@pytest.mark.parametrize("weighed", [False, True], ids=["", "weighed"])
+def test_decode(lens, weighed):
+    attend(lens, [1] * len(lens), 8, 2, 128, weighed=weighed)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (2, 2), (5, 1), (14, 2), (32, 4), (16, 1), (24, 8), (40, 2)])
+@pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16"])
+def test_decode_heads(dim, hq, hk, dtype):
+    attend([333, 50, 1], [1, 1, 1], hq, hk, dim, dtype, page=32, weighed=hq % 2 == 0, powers=False)
+
+
+@pytest.mark.parametrize("window", [1, 15, 16, 100, 5000])
+def test_windows(window):
+    attend([1, 200, 17, 1000], [1] * 4, 8, 2, 64, window=window, weighed=True, page=64)
+    attend([1, 200, 17, 1000], [1, 30, 17, 9], 8, 2, 128, window=window, weighed=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hq,hk", [(4, 4), (7, 1), (8, 2), (16, 1)])
+@pytest.mark.parametrize("weighed", [False, True], ids=["", "weighed"])
+def test_rows(dim, hq, hk, weighed):
+    """Requests that bring 0, 1 or many rows, up to all of their tokens."""
+    attend([30, 100, 513, 40, 77], [30, 0, 5, 1, 70], hq, hk, dim, weighed=weighed, powers=False)
+
+
+def test_more_rows_than_tokens():
+    """Rows in front of the text see nothing."""
+    attend([3, 0, 20], [5, 2, 20], 4, 2, 64, weighed=True)
+
+
+def test_bounds_may_be_loose_or_read_from_the_device():
+    for kw in (dict(max_q=9, max_kv=4096), dict(max_q=0, max_kv=0)):
+        attend([70, 200], [1, 4], 8, 2, 128, weighed=True, **kw)
+    attend([70, 200], [1, 1], 8, 2, 128, weighed=True, max_q=0, max_kv=1 << 20)
+
+
+def test_large_scores():
+    """Scores of some hundreds: one token takes all."""
+    attend([300, 1000], [1, 3], 8, 2, 128, scale=6.0)
+
+
+def test_what_lies_behind_a_request_does_not_matter():
+    lens, page = [21, 90], 16
+    table, pages = tables(lens, page)
+    cache, ks, vs, _, _ = make(pages, 2, page, 128)
+    q = torch.randn(2, 8, 128, device="cuda").bfloat16()
+    run = lambda: ops.paged_attention_fp4(q, cache, table, ints([0, 1, 2]), ints(lens), 0.1, k_scale=ks, v_scale=vs, max_q=1,  # noqa: E731
+                                          max_kv=90)
+    first = run()
+    bad = torch.full((1, 2, 128), math.nan, device="cuda").bfloat16()
+    for i in range(21, 32):
+        ops.store_kv_fp4(bad, bad, cache, ints([int(table[0, 1]) * page + i % page]), ks, vs)
+    for i in range(90, 96):
+        ops.store_kv_fp4(bad, bad, cache, ints([int(table[1, 5]) * page + i % page]), ks, vs)
+    assert torch.equal(first, run())
+    # a NaN that is seen shows
+    ops.store_kv_fp4(bad, bad, cache, ints([int(table[0, 1]) * page + 20 % page]), ks, vs)
+    assert run()[0].isnan().all() and torch.equal(run()[1], first[1])
+
+
+def test_same_results_every_time():
+    kw = dict(lens=[3000, 17, 900, 0, 20000], news=[1] * 5, hq=8, hk=2, dim=128)
+    assert torch.equal(attend(**kw, weighed=True), attend(**kw, weighed=True))
+
+
+def test_a_table_of_any_stride_and_queries_of_any_stride():
+    lens, page = [40, 60], 16
+    table, pages = tables(lens, page)
+    cache, ks, vs, _, _ = make(pages, 2, page, 64)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    run = lambda q, t: ops.paged_attention_fp4(q, cache, t, ints([0, 1, 2]), ints(lens), 0.1, k_scale=ks, v_scale=vs)  # noqa: E731
+    want = run(q, table)
+    wide = torch.zeros(2, 11, dtype=torch.int32, device="cuda")
+    wide[:, 3:7] = table
+    assert torch.equal(run(torch.stack([q, q], 2).flatten(1, 2)[:, ::2], wide[:, 3:7]), want)
+    assert torch.equal(run(q, table.t().contiguous().t()), want)
+
+
+def test_pool_beyond_32_bits():
+    page, hk, dim = 64, 8, 128
+    pages = (1 << 32) // (hk * 4 * 18 * dim) + 40
+    cache = torch.zeros(pages, hk, page // 16, 18 * dim, dtype=torch.uint8, device="cuda")
+    n = 150
+    k, v = (torch.randn(n, hk, dim, device="cuda").bfloat16() for _ in range(2))
+    table = ints([[pages - 1, 3, pages - 7]])
+    loc = torch.cat([torch.arange(page, device="cuda") + p * page for p in table[0].tolist()])[:n].int()
+    weights = torch.zeros(pages, hk, page, device="cuda")
+    ops.store_kv_fp4(k, v, cache, loc)
+    q = torch.randn(1, 16, dim, device="cuda").bfloat16()
+    out = ops.paged_attention_fp4(q, cache, table, ints([0, 1]), ints([n]), 0.1, max_q=1, max_kv=n, weights=weights)
+    small = cache[table[0].long()]
+    want, tol, w, _ = plain.attention(q, *plain.values(small), ints([[0, 1, 2]]), ints([0, 1]), ints([n]), 0.1)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+    got = weights[table[0].long()].transpose(0, 1).flatten(1)[:, :n].cpu().double()
+    assert (got - w[0]).abs().max() < 1e-5
+    back = ops.load_kv_fp4(cache, loc)
+    assert all(torch.equal(x.cpu().double(), plain.rounded(y, None)) for x, y in zip(back, (k, v)))
+    kept, _ = ops.evict_kv_fp4(cache, weights, table, ints([n]), ints([[pages - 3]]), 50, 5)
+    rows = kept[0, 0].long()
+    slots = (torch.arange(50, device="cuda") + (pages - 3) * page).int()
+    assert all(torch.equal(x[:, 0], y[rows, 0]) for x, y in zip(ops.load_kv_fp4(cache, slots), back))
+
+
+# ------------------------------------------------------------------------------------------ eviction
+EVICT = [([50, 21, 5, 0, 64, 22], 21, 6, 2), ([100, 3000, 900], 64, 64, 0), ([100, 3000, 900], 64, 0, 64), ([70, 2000], 33, 0, 0),
+         ([9000, 8193, 12000], 2048, 100, 4), ([40], 1, 0, 0), ([60000], 1000, 10, 1)]
+
+
+@pytest.mark.parametrize("lens,budget,recent,sinks", EVICT, ids=[str(e[0][0]) + "_to_" + str(e[1]) for e in EVICT])
+@pytest.mark.parametrize("dim,page,layers", [(64, 16, 0), (128, 32, 2), (256, 16, 1)])
+def test_evict(lens, budget, recent, sinks, dim, page, layers):
+    hk = 2
+    slim = -(-budget // page)
+    table, pages = tables(lens, page, spare=len(lens) * slim + 1)
+    new = torch.tensor([p for p in range(pages) if p not in set(table.flatten().tolist())][:len(lens) * slim],
+                       dtype=torch.int32, device="cuda").view(len(lens), slim)
+    g = torch.Generator("cuda").manual_seed(1)
+    cache = torch.randint(0, 256, (max(layers, 1), pages, hk, page // 16, 18 * dim), generator=g, device="cuda", dtype=torch.uint8)
+    weights = torch.rand(max(layers, 1), pages, hk, page, generator=g, device="cuda")
+    weights = torch.round(weights ** 4 * 256)                # many equal ones
+    weights[0, table[0, 0], 0, 3], weights[0, table[0, 0], 1, 9] = math.nan, math.inf
+    weights[0, table[0, 0], 1, 5], weights[0, table[0, 0], 1, 6] = -0.0, -3.0
+    if not layers:
+        cache, weights = cache[0], weights[0]
+    old, old_w = cache.clone(), weights.clone()
+    kept, now = ops.evict_kv_fp4(cache, weights, table, ints(lens), new, budget, recent, sinks,
+                                 **({"max_kv": max(lens)} if dim == 128 else {}))
+    assert now.tolist() == [min(n, budget) for n in lens]
+    from minisglang_rdna4_b200.ops import ref_fp4
+
+    for a, w, a0, w0, kept in zip(*((x if layers else x[None]) for x in (cache, weights, old, old_w, kept))):
+        want, want_w = a0.clone(), w0.clone()
+        stay, _ = ref_fp4.evict_kv_fp4(want, want_w, table, ints(lens), new, budget, recent, sinks)
+        if max(lens) <= 9000:
+            for b, n in enumerate(lens):
+                i = torch.arange(n)
+                for h in range(hk):
+                    mine = w0[table[b].long()[i.cuda() // page], h, i.cuda() % page].tolist()
+                    s = plain.chosen(mine, n, budget, recent, sinks)
+                    assert kept[b, h].tolist() == s + [-1] * (budget - len(s))
+        assert torch.equal(kept, stay)
+        assert torch.equal(a, want) and torch.equal(w.nan_to_num(-7.0), want_w.nan_to_num(-7.0))
+
+
+def test_a_conversation_is_stored_weighed_and_cut():
+    """Store, weighed attention, eviction, new tokens, attention again, in a captured graph and eagerly."""
+    page, hk, hq, dim, lens, budget = 16, 2, 8, 128, [700, 90, 1500], 128
+    slim = budget // page + 1
+    torch.manual_seed(5)
+    pages = 44 + 6 + 94 + 3 * slim              # of the requests, and those that they are cut down into
+    ks, vs = torch.full((hk,), 1 / 64, device="cuda"), torch.full((hk,), 1 / 128, device="cuda")
+    order = torch.randperm(pages).int().cuda()
+    table = torch.zeros(3, 94, dtype=torch.int32, device="cuda")
+    table[0, :44], table[1, :6], table[2] = order[:44], order[44:50], order[50:144]
+    new = order[144:].view(3, slim)
+    cache = torch.zeros(pages, hk, 1, 18 * dim, dtype=torch.uint8, device="cuda")
+    weights = torch.full((pages, hk, page), 9.0, device="cuda")
+    total = sum(lens)
+    k, v = (torch.randn(total + 3, hk, dim, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(total + 3, hq, dim, device="cuda").bfloat16()
+    loc = torch.cat([(table[b].long()[i // page] * page + i % page) for b, n in enumerate(lens)
+                     for i in [torch.arange(n, device="cuda")]]).int()
+    cu, n = ints([0, 700, 790, 2290]), ints(lens)
+
+    def turn():
+        ops.store_kv_fp4(k[:total], v[:total], cache, loc, ks, vs, weights)
+        first = ops.paged_attention_fp4(q[:total], cache, table, cu, n, 0.1, k_scale=ks, v_scale=vs, max_q=1500, max_kv=1500,
+                                        weights=weights)
+        kept, now = ops.evict_kv_fp4(cache, weights, table, n, new, budget, 20, 4)
+        at = torch.gather(new, 1, (now // page)[:, None].long())[:, 0] * page + now % page
+        ops.store_kv_fp4(k[total:], v[total:], cache, at, ks, vs, weights)
+        last = ops.paged_attention_fp4(q[total:], cache, new, steps, now + 1, 0.1, k_scale=ks, v_scale=vs, max_q=1, max_kv=budget + 1, weights=weights)
+        return first, kept, now, last, weights.clone()
+
+    steps = ints([0, 1, 2, 3])
+    eager = [x.clone() for x in turn()]
+    kk, vv = plain.rounded(k, ks), plain.rounded(v, vs)
+    for b in range(3):
+        for h in range(hq):
+            at = eager[1][b, h // 4].cpu().long()
+            at = torch.cat([at[at >= 0] + int(cu[b]), torch.tensor([total + b])])
+            w = torch.softmax(q[total + b, h].cpu().double() @ kk[at, h // 4].T * 0.1, -1)
+            assert (eager[3][b, h].cpu().double() - w @ vv[at, h // 4]).abs().max() < 2.0 ** -7
+    assert torch.isfinite(eager[4]).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        turn()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = turn()
+    cache.zero_()
+    weights.fill_(1.0)
+    graph.replay()
+    weights_then = captured[4].clone()
+    graph.replay()
+    assert all(torch.equal(x, y) for x, y in zip(captured[:4], eager[:4]))
+    for b, m in enumerate(eager[2].tolist()):            # slots behind the rows keep what was there: 9 before, 1 now
+        mine = [w[new[b].long()].transpose(0, 1).flatten(1) for w in (captured[4], eager[4])]
+        assert torch.equal(mine[0][:, :m + 1], mine[1][:, :m + 1])
+        assert (mine[0][:, m + 1:] == 1.0).all() and (mine[1][:, m + 1:] == 9.0).all()
+    assert torch.equal(weights_then, captured[4])
+
+
+def test_two_streams_at_once():
+    lens = [5000, 300, 9000]
+    table, pages = tables(lens, 16)
+    cache, ks, vs, _, _ = make(pages, 2, 16, 128)
+    qs = [torch.randn(3, 8, 128, device="cuda").bfloat16() for _ in range(2)]
+    cu, n = ints([0, 1, 2, 3]), ints(lens)
+    run = lambda q: ops.paged_attention_fp4(q, cache, table, cu, n, 0.1, k_scale=ks, v_scale=vs, max_q=1, max_kv=9000)  # noqa: E731
+    want = [run(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(qs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
+
+
+def test_refusals():
+    cache, ks, vs, k, v = make(4, 2, 16, 64)
+    loc = ints([1, 2])
+    with pytest.raises(ValueError):
+        ops.store_kv_fp4(k[:2], v[:2], cache, loc.cpu(), ks, vs)
+    with pytest.raises(ValueError):
+        ops.store_kv_fp4(k[:2].cpu(), v[:2], cache, loc, ks, vs)
+    with pytest.raises(ValueError):
+        ops.load_kv_fp4(cache, loc, ks.cpu())
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    with pytest.raises(ValueError):
+        ops.paged_attention_fp4(q, cache, ints([[0], [1]]), ints([0, 1, 2]), ints([5, 6]).cpu(), 1.0)
+    assert ops.load_kv_fp4(cache, ints([]), ks, vs)[0].shape == (0, 2, 64)
+    none = ops.paged_attention_fp4(q[:0], cache, ints([[0], [1]]), ints([0, 0, 0]), ints([5, 6]), 1.0)
+    assert none.shape == (0, 4, 64)
+    ops.store_kv_fp4(k[:0], v[:0], cache, ints([]), ks, vs)
