@@ -1,108 +1,736 @@
-// Attention over the paged K/V pool of 4 bits (kv_fp4.cuh).
+// Causal attention over the paged K/V pool of 4 bits (kv_fp4.cuh).
+//
+// A unit is a tile of rows of one request and key head, a row being a (query position, head of the group) pair, with all 16-token
+// tiles that its request's rows see. The tiles of all units in a line are dealt evenly to the warps of the GPU; a warp
+// fetches its tiles into a ring of its own (bulk copies of 18 D bytes) and keeps the softmax of the unit it is in. Units that a
+// warp has whole are written at once, parts of others go to the workspace and a second kernel joins them.
+//
+// Both products take the cache as their first operand (rows: 16 tokens, or 16 channels), so a row tile is 8 queries wide and
+// no product is spent on more rows than a group of 8 heads has: S^T = K Q^T, O^T = V^T P^T. Codes go e2m1 -> f16 (one
+// conversion for two) and are multiplied by their scale, which is exact (2 + 4 significant bits). Queries are scaled to
+// powers of two around 2^10 and taken as f16: exact for bf16 and fp16 values down to 2^-24 of a row's largest. Sums, running
+// maximum and sum of the softmax are fp32. Probabilities go into the second product as f16 (11 bits) after a factor of 2^7,
+// so that they are normal numbers down to 2^-21 of the largest; the maximum moves only when a score passes it by 2^8, which
+// the factor leaves room for (2^15).
 #include "kv_fp4.cuh"
+#include "ptx.cuh"
 
 using namespace msgl;
 using namespace msgl::fp4;
+using namespace msgl::ptx;
 
 namespace {
+
+constexpr int kWarps = 4;            // of a CTA
+constexpr int kMost = 1024;          // requests of a launch
+constexpr int kFewTiles = 4;         // a warp gets at least so many tiles
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kUp = 7.f, kSlack = 8.f;   // log2 of the probabilities' factor; by how much a score may pass the maximum
+
+__device__ int g_fp4_status = 0;
 
 struct Fp4Args {
   const void* q;
   void* out;
   const uint8_t* pool;
   const int32_t* table;
+  long long table_stride;
   const int32_t* cu_q;
   const int32_t* lens;
   const float* k_head;
   const float* v_head;
+  float* lse;               // [rows, hq], log2; null without weights
   float* weights;
-  int width, B, hq, hk, page_size, pages, window;
+  float* parts;             // [2 * workers][rows of a tile][D + 2]
+  long long* line;          // [B + 2]: first tile of every request in the line, total; workers
+  int width, B, hq, hk, group, page_size, pages, window, row_tile, workers;
   float scale;
+  int* status;
 };
 
-// A CTA for each (request, key head); rows and the heads that share the keys one after another. Softmax statistics first, then
-// the probabilities again and the sum of the values.
-template <typename T, int D> __global__ void __launch_bounds__(256) fp4_attention_simple_kernel(const Fp4Args a) {
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// four bytes of two codes each -> four pairs of f16
+__device__ __forceinline__ void widen(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t widen_e4m3(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// token of a tile in row g + 8 r of the keys' operand
+__device__ __forceinline__ int token_of(int g, int r) { return 4 * (g >> 1) + 2 * r + (g & 1); }
+
+// ---- the line of tiles -----------------------------------------------------------------
+struct Request {
+  int q0, q_len, n;         // first row, rows, tokens
+  int tile0, tiles;         // tiles that its rows see
+  int row_tiles;
+  __device__ __forceinline__ void load(const Fp4Args& a, int b) {
+    q0 = a.cu_q[b];
+    q_len = a.cu_q[b + 1] - q0;
+    n = min(max(a.lens[b], 0), a.width * a.page_size);
+    const int lo = a.window > 0 ? max(0, n - q_len - a.window + 1) : 0;
+    tile0 = lo / kTile;
+    tiles = q_len > 0 && n > lo ? (n + kTile - 1) / kTile - tile0 : 0;
+    row_tiles = (max(q_len, 0) * a.group + a.row_tile - 1) / a.row_tile;
+  }
+  __device__ __forceinline__ long long cost(const Fp4Args& a, bool whole_rows) const {
+    return (long long)tiles * a.hk * (whole_rows ? 1 : row_tiles);
+  }
+};
+
+// First tile of every request in `line` (kMost + 1 entries), the total in line[B].
+__device__ __forceinline__ void lay_line(const Fp4Args& a, long long* line, bool whole_rows) {
+  __shared__ long long sums[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32);
+  const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    Request r;
+    r.load(a, b);
+    line[b] = mine;
+    mine += r.cost(a, whole_rows);
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+  for (int b = b0; b < b1; ++b) line[b] += before;
+  if (threadIdx.x == kWarps * 32 - 1) line[a.B] = before + mine;
+  __syncthreads();
+}
+
+// Worker w of W has tiles [begin(w), begin(w + 1)).
+struct Deal {
+  long long base;
+  int workers, extra;
+  __device__ __forceinline__ Deal(long long total, int most) {
+    workers = (int)max(1ll, min((long long)most, total / kFewTiles));
+    base = total / workers;
+    extra = (int)(total - base * workers);
+  }
+  __device__ __forceinline__ long long begin(int w) const { return w * base + min(w, extra); }
+  __device__ __forceinline__ int owner(long long at) const {
+    const long long big = (base + 1) * extra;
+    return (int)(at < big ? at / (base + 1) : extra + (at - big) / max(base, 1ll));
+  }
+};
+
+// A place in the line.
+struct Walk {
+  int b, unit, tile;        // unit: head * row tiles + row tile
+  Request r;
+  __device__ __forceinline__ void seek(const Fp4Args& a, const long long* line, long long at) {
+    int lo = 0, hi = a.B - 1;                   // the last request that starts at or before `at` has it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (line[mid] <= at) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    r.load(a, b);
+    const long long o = at - line[b];
+    unit = (int)(o / max(r.tiles, 1));
+    tile = (int)(o - (long long)unit * r.tiles);
+  }
+  // true where another unit begins
+  __device__ __forceinline__ bool next(const Fp4Args& a, const long long* line, bool whole_rows) {
+    if (++tile < r.tiles) return false;
+    tile = 0;
+    if (++unit < a.hk * (whole_rows ? 1 : r.row_tiles)) return true;
+    unit = 0;
+    do ++b; while (b < a.B - 1 && line[b] == line[b + 1]);
+    r.load(a, min(b, a.B - 1));
+    return true;
+  }
+  __device__ __forceinline__ int page(const Fp4Args& a) const {
+    const int col = min((r.tile0 + tile) * kTile / a.page_size, a.width - 1);
+    const int page = a.table[(long long)b * a.table_stride + col];
+    (void)MSGL_OOB(page, a.pages);
+    return min(max(page, 0), a.pages - 1);
+  }
+  template <int D> __device__ __forceinline__ long long address(const Fp4Args& a, int page, int head) const {
+    const int per = a.page_size / kTile;
+    return (((long long)page * a.hk + head) * per + (r.tile0 + tile) % per) * Tile<D>::bytes;
+  }
+};
+
+// ---- queries ---------------------------------------------------------------------------
+// Lane 4 g + j takes channels j D / 4 .. of row g as the second operand of S^T, scaled by a power of two; returns what the
+// row's scores have to be multiplied by.
+template <typename T, int D>
+__device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, int head, int row, int lane, uint32_t (&qf)[D / 8]) {
+  const bool there = row < r.q_len * a.group;
+  const int pos = there ? row / a.group : 0;
+  const T* src = reinterpret_cast<const T*>(a.q) + ((long long)(r.q0 + pos) * a.hq + head * a.group + (there ? row - pos * a.group : 0)) * D
+                 + (lane & 3) * (D / 4);
+  float top = 0.f;
+  Vec8<T> raw[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    if (there) raw[i] = *reinterpret_cast<const Vec8<T>*>(src + 8 * i);
+    else
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[i].v[e] = Pack2<T>::make(0.f, 0.f);
+    float x[8];
+    unpack8(raw[i], x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int ex = (int)(__float_as_uint(top) >> 23);            // 0: zeros; 255: infinite
+  const int up = top > 0.f && ex < 255 ? min(max(137 - ex, -126), 126) : 0;
+  const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    float x[8];
+    unpack8(raw[i], x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qf[4 * i + e] = f16x2(x[2 * e] * f, x[2 * e + 1] * f);
+  }
+  return __uint_as_float((uint32_t)(127 - up) << 23);
+}
+
+template <int D> struct Raw {          // a lane's share of a tile
+  uint4 k[D / 64], v[D / 64];
+  uint32_t ks[D / 128 > 0 ? D / 128 : 1], vs[D / 128 > 0 ? D / 128 : 1];
+};
+
+template <int D> __device__ __forceinline__ void load_keys(const uint8_t* tile, int lane, Raw<D>& x) {
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) x.k[i] = *reinterpret_cast<const uint4*>(tile + 512 * i + 16 * lane);
+  if (D == 64) x.ks[0] = *reinterpret_cast<const uint16_t*>(tile + Tile<D>::k_sf + 2 * lane);
+  else
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i) x.ks[i] = *reinterpret_cast<const uint32_t*>(tile + Tile<D>::k_sf + lane * (D / 32) + 4 * i);
+}
+template <int D> __device__ __forceinline__ void load_values(const uint8_t* tile, int lane, Raw<D>& x) {
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) x.v[i] = *reinterpret_cast<const uint4*>(tile + Tile<D>::v + 512 * i + 16 * lane);
+  const int g = lane >> 2, j = lane & 3;
+#pragma unroll
+  for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
+    const int block = D == 64 ? g >> 1 : D == 128 ? g : 2 * g + i;
+    x.vs[i] = *reinterpret_cast<const uint32_t*>(tile + Tile<D>::v_sf + (block * 4 + j) * 4);
+  }
+}
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// Keys of row r, block of 32 bits w (8 channels): D / 32 words of each row.
+template <int D> __device__ __forceinline__ uint32_t key_word(const Raw<D>& x, int r, int w) {
+  const int at = r * (D / 32) + w;
+  return word(x.k[at / 4], at % 4);
+}
+// scale of row r, block i (of D / 64), in both halves
+template <int D> __device__ __forceinline__ uint32_t key_scale(const Raw<D>& x, int r, int i) {
+  const int at = r * (D / 64) + i;                                  // byte
+  const uint32_t two = widen_e4m3(x.ks[at / 4] >> (at % 4 / 2 * 16));
+  return __byte_perm(two, two, at % 2 ? 0x3232 : 0x1010);
+}
+
+// S^T of the tile for NB blocks of 8 rows
+template <int D, int NB> __device__ __forceinline__ void scores(const Raw<D>& x, const uint32_t (&qf)[NB][D / 8], float (&s)[NB][4]) {
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {                                // blocks of 16 channels: 2 words, 4 products
+    const uint32_t s0 = key_scale<D>(x, 0, i), s1 = key_scale<D>(x, 1, i);
+#pragma unroll
+    for (int w = 2 * i; w < 2 * i + 2; ++w) {
+      uint32_t h0[4], h1[4];
+      widen(key_word<D>(x, 0, w), h0);
+      widen(key_word<D>(x, 1, w), h1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t a0 = times(h0[2 * c], s0), a1 = times(h1[2 * c], s1), a2 = times(h0[2 * c + 1], s0), a3 = times(h1[2 * c + 1], s1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma(s[nb], a0, a1, a2, a3, qf[nb][4 * w + 2 * c], qf[nb][4 * w + 2 * c + 1]);
+      }
+    }
+  }
+}
+
+template <int D, int NB> struct Shape {
+  static constexpr int stages = D == 64 ? 6 : D == 128 ? 4 : 3;
+  static constexpr int ring = kWarps * stages * Tile<D>::bytes;
+  static constexpr int ctas = D == 256 ? (NB == 1 ? 3 : 2) : NB == 1 ? 4 : NB == 2 ? 3 : 2;
+  static constexpr int smem = ring + kWarps * stages * 8 + 16 + (kMost + 2) * 8;
+};
+
+template <typename T, int D, int NB>
+__global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention_kernel(const Fp4Args a) {
+  constexpr int STAGES = Shape<D, NB>::stages, BYTES = Tile<D>::bytes;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint8_t* ring = smem + warp * STAGES * BYTES;
+  const uint32_t bar = smem_u32(smem + Shape<D, NB>::ring) + warp * STAGES * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8);
+  long long* line = reinterpret_cast<long long*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8 + 16);
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(bar + 8 * s, 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
   pdl_enter();
-  __shared__ float qs[D], ps[256], scratch[32];
-  const int b = blockIdx.x / a.hk, h = blockIdx.x % a.hk, G = a.hq / a.hk;
-  const int q0 = a.cu_q[b], q_len = a.cu_q[b + 1] - q0;
-  const int n = min(a.lens[b], a.width * a.page_size);
-  const float kh = a.k_head != nullptr ? a.k_head[h] : 1.f, vh = a.v_head != nullptr ? a.v_head[h] : 1.f;
-  auto tile_of = [&](int i) {
-    const int page = min(max(a.table[(long long)b * a.width + i / a.page_size], 0), a.pages - 1);
-    return a.pool + tile_at<D>(page, i % a.page_size, h, a.hk, a.page_size);
+  lay_line(a, line, false);
+  const Deal deal(line[a.B], a.workers);
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b <= a.B; b += kWarps * 32) a.line[b] = line[b];
+  }
+  // neighbours in the line lie on different SMs: a short line is spread over all of them
+  const int worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= deal.workers) return;
+  long long at = deal.begin(worker);
+  const long long end = deal.begin(worker + 1);
+  if (at >= end) return;
+
+  Walk get, put;                 // what is computed; what is fetched
+  get.seek(a, line, at);
+  put = get;
+  long long ahead = at;
+  int page = put.page(a);
+  auto fetch = [&](int stage) {  // the tile at `ahead`; then the page of the next one is asked for
+    if (lane == 0) {
+      mbar_expect_tx(bar + 8 * stage, BYTES);
+      bulk_load(smem_u32(ring + stage * BYTES), a.pool + put.address<D>(a, page, put.unit / put.r.row_tiles), BYTES, bar + 8 * stage);
+    }
+    if (++ahead < end) {
+      put.next(a, line, false);
+      page = put.page(a);
+    }
   };
-  for (int r = 0; r < q_len * G; ++r) {
-    const long long row = q0 + r / G;
-    const int head = h * G + r % G, pos = n - q_len + r / G;
-    const int hi = min(n, pos + 1), lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += 256) qs[d] = to_float(reinterpret_cast<const T*>(a.q)[(row * a.hq + head) * D + d]) * a.scale * kh;
-    __syncthreads();
-    auto score = [&](int i) {
-      const uint8_t* tile = tile_of(i);
-      const int t = i % kTile;
-      float s = 0.f;
-      for (int blk = 0; blk < D / 16; ++blk) {
-        float part = 0.f;
-        for (int d = 0; d < 16; d += 2) {
-          const float2 x = decode2(tile[k_byte<D>(t, blk * 16 + d)]);
-          part += qs[blk * 16 + d] * x.x + qs[blk * 16 + d + 1] * x.y;
+  for (int s = 0; s < STAGES && ahead < end; ++s) fetch(s);
+
+  const int g = lane >> 2, j = lane & 3;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  while (at < end) {
+    // ---- one unit, or this warp's part of it
+    const int first = get.tile, head = get.unit / get.r.row_tiles, row0 = (get.unit - head * get.r.row_tiles) * a.row_tile;
+    const int count = (int)min(end - at, (long long)(get.r.tiles - first));
+    const Request r = get.r;
+    const int rows = min(a.row_tile, r.q_len * a.group - row0);
+    uint32_t qf[NB][D / 8];
+    float cA[NB], cB[NB];        // factors of the scores of rows 2 j and 2 j + 1
+    const float kh = a.scale * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float back = load_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, qf[nb]);
+      cA[nb] = kh * __shfl_sync(0xffffffffu, back, 8 * j);
+      cB[nb] = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
+    }
+    float o[NB][D / 16][4], m[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+      m[nb][0] = m[nb][1] = -INFINITY;
+      l[nb][0] = l[nb][1] = 0.f;
+    }
+    // tokens that the first and the last row see: [lo, hi) all rows, outside of them some do not
+    const int pos0 = r.n - r.q_len + row0 / a.group, pos1 = r.n - r.q_len + (row0 + rows - 1) / a.group;
+    const int hi_all = pos0 + 1, lo_all = a.window > 0 ? pos1 - a.window + 1 : 0;
+
+    for (int t = 0; t < count; ++t) {
+      if (ok) ok = mbar_wait(bar + 8 * stage, phase, abort_flag, a.status, 401);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      Raw<D> x;
+      load_keys<D>(ring + stage * BYTES, lane, x);
+      load_values<D>(ring + stage * BYTES, lane, x);
+      __syncwarp();
+      if (ahead < end) fetch(stage);
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+
+      const int tok0 = (r.tile0 + first + t) * kTile;
+      if (tok0 > pos1) continue;     // other rows of the request see it
+      float s[NB][4];
+      scores<D, NB>(x, qf, s);
+      const bool ragged = tok0 + kTile > hi_all || tok0 < lo_all;
+      bool move = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        s[nb][0] *= cA[nb]; s[nb][1] *= cB[nb]; s[nb][2] *= cA[nb]; s[nb][3] *= cB[nb];
+        if (ragged) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = tok0 + token_of(g, i >> 1), pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + (i & 1)) / a.group;
+            if (tok > min(pos, r.n - 1) || (a.window > 0 && tok <= pos - a.window)) s[nb][i] = -INFINITY;
+          }
         }
-        s += part * e4m3_to_float(tile[k_sf_byte<D>(t, blk)]);
+        move |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kSlack || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kSlack;
       }
-      return s;
-    };
-    float m = -INFINITY;
-    for (int i = lo + threadIdx.x; i < hi; i += 256) m = fmaxf(m, score(i));
-    m = block_max(m, scratch);
-    float l = 0.f;
-    for (int i = lo + threadIdx.x; i < hi; i += 256) l += expf(score(i) - m);
-    l = block_sum(l, scratch);
-    float o = 0.f;
-    for (int i0 = lo; i0 < hi; i0 += 256) {
-      const int i = i0 + threadIdx.x;
-      const float p = i < hi ? expf(score(i) - m) / l : 0.f;
-      __syncthreads();
-      ps[threadIdx.x] = p;
-      if (i < hi && a.weights != nullptr) {
-        const int page = min(max(a.table[(long long)b * a.width + i / a.page_size], 0), a.pages - 1);
-        atomicAdd(a.weights + ((long long)page * a.hk + h) * a.page_size + i % a.page_size, p);
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(s[nb][c], s[nb][2 + c]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(top, m[nb][c]);
+            const float f = m[nb][c] == top ? 1.f : exp2_fast(m[nb][c] - top);
+            m[nb][c] = top;
+            l[nb][c] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) { o[nb][i][c] *= f; o[nb][i][2 + c] *= f; }
+          }
+        }
       }
-      __syncthreads();
-      if (threadIdx.x < D) {
-        const int d = threadIdx.x;
-        for (int k = 0; k < min(256, hi - i0); ++k) {
-          const uint8_t* tile = tile_of(i0 + k);
-          const int t = (i0 + k) % kTile;
-          const float2 x = decode2(tile[v_byte<D>(t, d & ~1)]);
-          o += ps[k] * (d & 1 ? x.y : x.x) * e4m3_to_float(tile[v_sf_byte<D>(t, d / 16)]);
+      uint32_t p0[NB], p1[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float mA = (m[nb][0] == -INFINITY ? 0.f : m[nb][0]) - kUp, mB = (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) - kUp;
+        const float e0 = exp2_fast(s[nb][0] - mA), e1 = exp2_fast(s[nb][1] - mB), e2 = exp2_fast(s[nb][2] - mA),
+                    e3 = exp2_fast(s[nb][3] - mB);
+        l[nb][0] += e0 + e2;
+        l[nb][1] += e1 + e3;
+        p0[nb] = transpose8(f16x2(e0, e1));
+        p1[nb] = transpose8(f16x2(e2, e3));
+      }
+      // values of tokens that no row sees may be anything; a NaN that only some rows see must not reach the others
+      uint32_t nan_mask = 0;       // bit 4 i + e: token 4 j + e has no number in block i of the lane's channels
+      if (ragged) {
+#pragma unroll
+        for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t byte = x.vs[i] >> (8 * e) & 0x7F;
+            if (byte == 0x7F) {
+              nan_mask |= 1u << (4 * i + e);
+              x.vs[i] &= ~(0xFFu << (8 * e));
+            }
+          }
+      }
+#pragma unroll
+      for (int w = 0; w < D / 64; ++w) {                  // words of 8 channels of the lane: 4 products
+        const int i = D == 256 ? w / 2 : 0;
+        const uint32_t s01 = widen_e4m3(x.vs[i]), s23 = widen_e4m3(x.vs[i] >> 16);
+        // words of tokens e = 0 .. 3: D / 64 words each
+        uint32_t tw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x.v[k / 4], k % 4); }
+        uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
+        widen((tw[0] & 0x0F0F0F0Fu) | ((tw[1] << 4) & 0xF0F0F0F0u), lo01);
+        widen(((tw[0] >> 4) & 0x0F0F0F0Fu) | (tw[1] & 0xF0F0F0F0u), hi01);
+        widen((tw[2] & 0x0F0F0F0Fu) | ((tw[3] << 4) & 0xF0F0F0F0u), lo23);
+        widen(((tw[2] >> 4) & 0x0F0F0F0Fu) | (tw[3] & 0xF0F0F0F0u), hi23);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a0 = times(lo01[k], s01), a1 = times(hi01[k], s01), a2 = times(lo23[k], s23), a3 = times(hi23[k], s23);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma(o[nb][4 * w + k], a0, a1, a2, a3, p0[nb], p1[nb]);
+        }
+      }
+      if (ragged && __any_sync(0xffffffffu, nan_mask != 0)) {
+        for (int jj = 0; jj < 4; ++jj) {
+          const uint32_t bits = __shfl_sync(0xffffffffu, nan_mask, 4 * g + jj);
+          for (int e = 0; e < 4; ++e) {
+            const int tok = tok0 + 4 * jj + e;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + c) / a.group;
+                const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                  if (seen && (bits >> ((D == 256 ? i / 8 * 4 : 0) + e) & 1)) o[nb][i][c] = o[nb][i][2 + c] = NAN;
+              }
+          }
         }
       }
     }
-    if (threadIdx.x < D)
-      reinterpret_cast<T*>(a.out)[(row * a.hq + head) * D + threadIdx.x] = from_float<T>(o * vh);
+    if (!ok) break;
+    at += count;
+
+    // ---- rows 2 j and 2 j + 1 of every block: channels g D / 8 .. (D / 8 of them)
+    const bool whole = first == 0 && count == r.tiles;
+    const float vh = a.v_head != nullptr ? a.v_head[head] : 1.f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
+        const int row = nb * 8 + 2 * j + c;
+        if (row >= rows) continue;
+        if (whole) {
+          const float f = l[nb][c] > 0.f || l[nb][c] != l[nb][c] ? vh / l[nb][c] : 0.f;
+          const int qi = (row0 + row) / a.group;
+          const long long to = (long long)(r.q0 + qi) * a.hq + head * a.group + (row0 + row - qi * a.group);
+          T* dst = reinterpret_cast<T*>(a.out) + to * D + g * (D / 8);
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { y[2 * e] = o[nb][4 * i + e][c] * f; y[2 * e + 1] = o[nb][4 * i + e][2 + c] * f; }
+            store8(dst + 8 * i, y);
+          }
+          if (a.lse != nullptr && g == 0) a.lse[to] = (m[nb][c] == -INFINITY ? 0.f : m[nb][c]) - kUp + log2f(l[nb][c]);
+        } else {
+          float* part = a.parts + ((long long)(2 * worker + (first == 0 ? 1 : 0)) * a.row_tile + row) * (D + 4);
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { y[2 * e] = o[nb][4 * i + e][c]; y[2 * e + 1] = o[nb][4 * i + e][2 + c]; }
+            store8(part + g * (D / 8) + 8 * i, y);
+          }
+          if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[nb][c], l[nb][c]);
+        }
+      }
+    }
+    if (at < end) { get.tile += count - 1; get.next(a, line, false); }
   }
+  if (!ok) {     // copies may be in flight: they land before the shared memory goes
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+}
+
+// A warp for each (row, query head) whose unit several workers share, or that sees nothing: the parts joined.
+template <typename T, int D> __global__ void __launch_bounds__(256) fp4_join_kernel(const Fp4Args a, int total_rows) {
+  pdl_enter();
+  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (id >= (long long)total_rows * a.hq) return;
+  const int row = (int)(id / a.hq), qh = (int)(id % a.hq);
+  if (row < a.cu_q[0] || row >= a.cu_q[a.B]) return;      // of another launch, or of no request
+  int lo = 0, hi = a.B - 1;                               // the last request that starts at or before the row
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
+  }
+  Request r;
+  r.load(a, lo);
+  T* dst = reinterpret_cast<T*>(a.out) + id * D + lane * (D / 32);
+  constexpr int E = D / 32;
+  float y[E] = {};
+  if (r.tiles > 0) {
+    const Deal deal(a.line[a.B], a.workers);
+    const int head = qh / a.group, in_unit = (row - r.q0) * a.group + qh % a.group;
+    const int rt = in_unit / a.row_tile, in_tile = in_unit - rt * a.row_tile;
+    const long long u0 = a.line[lo] + ((long long)head * r.row_tiles + rt) * r.tiles;
+    const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
+    if (w0 == w1) return;                                // written by its worker
+    float m = -INFINITY, l = 0.f;
+    for (int w = w0; w <= w1; ++w) {
+      const float* part = a.parts + ((long long)(2 * w + (w == w0 ? 1 : 0)) * a.row_tile + in_tile) * (D + 4);
+      const float2 ml = *reinterpret_cast<const float2*>(part + D);
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = part[lane * E + e];
+      const float top = fmaxf(m, ml.x);
+      const float f0 = m == top ? 1.f : exp2_fast(m - top), f1 = ml.x == top ? 1.f : exp2_fast(ml.x - top);
+      m = top;
+      l = l * f0 + ml.y * f1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + x[e] * f1;
+    }
+    const float f = l > 0.f || l != l ? (a.v_head != nullptr ? a.v_head[head] : 1.f) / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] *= f;
+    if (a.lse != nullptr && lane == 0) a.lse[id] = (m == -INFINITY ? 0.f : m) - kUp + log2f(l);
+  }
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<typename Pack2<T>::type*>(dst + e) = Pack2<T>::make(y[e], y[e + 1]);
+}
+
+// What the rows give every token: the keys once more, with the rows' final maxima and sums. The warps deal out the tiles of
+// all (request, key head) pairs; a tile goes through all rows of its pair.
+template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 3 : 4) fp4_weights_kernel(const Fp4Args a) {
+  __shared__ long long line[kMost + 2];
+  pdl_enter();
+  lay_line(a, line, true);
+  Deal deal(line[a.B], gridDim.x * kWarps);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const int worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= deal.workers) return;
+  long long at = deal.begin(worker);
+  const long long end = deal.begin(worker + 1);
+  if (at >= end) return;
+  Walk get;
+  get.seek(a, line, at);
+  uint32_t qf[1][D / 8];
+  float cA = 0.f, cB = 0.f, eA = 0.f, eB = 0.f;
+  bool fresh = true;
+  while (at < end) {
+    const Request& r = get.r;
+    const int head = get.unit, page = get.page(a), tok0 = (r.tile0 + get.tile) * kTile;
+    Raw<D> x;
+    load_keys<D>(a.pool + get.address<D>(a, page, head), lane, x);
+    const int rows = r.q_len * a.group;
+    const float kh = a.scale * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
+    float sum0 = 0.f, sum1 = 0.f;
+    for (int row0 = 0; row0 < rows; row0 += 8) {
+      const int posA = r.n - r.q_len + (row0 + 2 * j) / a.group, posB = r.n - r.q_len + (row0 + 2 * j + 1) / a.group;
+      if (fresh || rows > 8) {
+        const float back = load_query<T, D>(a, r, head, row0 + g, lane, qf[0]);
+        cA = kh * __shfl_sync(0xffffffffu, back, 8 * j);
+        cB = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
+        auto lse = [&](int row) {
+          if (row >= rows) return INFINITY;                // weight 0
+          const int qi = row / a.group;
+          return a.lse[(long long)(r.q0 + qi) * a.hq + head * a.group + row - qi * a.group];
+        };
+        eA = lse(row0 + 2 * j);
+        eB = lse(row0 + 2 * j + 1);
+      }
+      float s[1][4];
+      scores<D, 1>(x, qf, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = tok0 + token_of(g, i >> 1), pos = i & 1 ? posB : posA;
+        const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
+        const float p = seen && (i & 1 ? eB : eA) != INFINITY ? exp2_fast(s[0][i] * (i & 1 ? cB : cA) - (i & 1 ? eB : eA)) : 0.f;
+        if (i < 2) sum0 += p; else sum1 += p;
+      }
+    }
+    fresh = false;
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      sum0 += __shfl_xor_sync(0xffffffffu, sum0, d);
+      sum1 += __shfl_xor_sync(0xffffffffu, sum1, d);
+    }
+    if (j < 2) {      // lane 0 of the four has row g's token, lane 1 row g + 8's
+      const int t = token_of(g, j);
+      if (tok0 + t < r.n)
+        atomicAdd(a.weights + ((long long)page * a.hk + head) * a.page_size + tok0 % a.page_size + t, j ? sum1 : sum0);
+    }
+    if (++at < end) fresh = get.next(a, line, true);
+  }
+}
+
+template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows, int sms, cudaStream_t stream) {
+  using S = Shape<D, NB>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(fp4_attention_kernel<T, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+    if (e != cudaSuccess) { msgl_set_error("paged_attention_fp4 shared memory", e); return MSGL_CUDA_ERROR; }
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  msgl_launch(fp4_attention_kernel<T, D, NB>, dim3(a.workers / kWarps), dim3(kWarps * 32), S::smem, stream, a);
+  MSGL_CHECK_LAUNCH("paged_attention_fp4");
+  msgl_launch(fp4_join_kernel<T, D>, dim3((unsigned)(((long long)total_rows * a.hq + 7) / 8)), dim3(256), 0, stream, a, total_rows);
+  MSGL_CHECK_LAUNCH("paged_attention_fp4 join");
+  if (a.weights != nullptr) {
+    msgl_launch(fp4_weights_kernel<T, D>, dim3(sms * (D == 256 ? 3 : 4)), dim3(kWarps * 32), 0, stream, a);
+    MSGL_CHECK_LAUNCH("paged_attention_fp4 weights");
+  }
+  return MSGL_OK;
+}
+
+int row_blocks(int d, int rows) { return rows <= 8 ? 1 : rows <= 16 || d == 256 ? 2 : 4; }
+
+int device_sms() {
+  static int sms[64] = {};
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && sms[dev]) return sms[dev];
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 0 && dev < 64) sms[dev] = n;
+  return n;
+}
+
+int worker_count(int d, int nb) {
+  const int ctas = d == 256 ? (nb == 1 ? 3 : 2) : nb == 1 ? 4 : nb == 2 ? 3 : 2;
+  return device_sms() * ctas * kWarps;
 }
 
 }  // namespace
 
-MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, const void* table, int width, const void* cu_q,
-                                const void* lens, const void* k_head, const void* v_head, void* weights, int B, int hq, int hk, int d,
-                                int page_size, int pages, int window, float scale, int dtype, cudaStream_t stream) {
-  if (B <= 0) return MSGL_OK;
-  if (hk <= 0 || hq % hk || (d != 64 && d != 128 && d != 256) || page_size <= 0 || page_size % kTile || (uintptr_t)pool % 16 ||
-      (uintptr_t)q % 16 || (uintptr_t)out % 16 || width <= 0 || (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
+// fp32 words of the workspace: the parts, the line (64 bits each), the rows' sums with weights.
+MSGL_API long long msgl_attention_fp4_workspace(int total_rows, int B, int hq, int hk, int d, int max_q, int weighed) {
+  if (hk <= 0) return 0;
+  const int nb = row_blocks(d, max_q * (hq / hk));
+  const long long parts = 2ll * worker_count(d, nb) * nb * 8 * (d + 4);
+  return parts + 2ll * ((B < kMost ? B : kMost) + 2) + (weighed ? (long long)total_rows * hq : 0);
+}
+
+MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, const void* table, long long table_stride, int width,
+                                const void* cu_q, const void* lens, const void* k_head, const void* v_head, void* weights,
+                                void* workspace, int total_rows, int B, int hq, int hk, int d, int page_size, int pages, int max_q,
+                                int window, float scale, int dtype, cudaStream_t stream) {
+  if (B <= 0 || total_rows <= 0) return MSGL_OK;
+  if (hk <= 0 || hq <= 0 || hq % hk || (d != 64 && d != 128 && d != 256) || page_size <= 0 || page_size % kTile ||
+      (uintptr_t)pool % 16 || (uintptr_t)q % 16 || (uintptr_t)out % 16 || (uintptr_t)workspace % 16 || width <= 0 || max_q <= 0 ||
+      (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
     msgl_set_error_text("paged_attention_fp4: heads of 64, 128 or 256 channels, pages of whole tiles of 16 tokens, 16-bit queries");
     return MSGL_BAD_ARG;
   }
-  Fp4Args a{q, out, (const uint8_t*)pool, (const int32_t*)table, (const int32_t*)cu_q, (const int32_t*)lens, (const float*)k_head,
-            (const float*)v_head, (float*)weights, width, B, hq, hk, page_size, pages, window, scale};
-#define ATT(T, D) msgl_launch(fp4_attention_simple_kernel<T, D>, dim3(B * hk), dim3(256), 0, stream, a)
-  if (dtype == MSGL_BF16) { if (d == 64) ATT(__nv_bfloat16, 64); else if (d == 128) ATT(__nv_bfloat16, 128); else ATT(__nv_bfloat16, 256); }
-  else { if (d == 64) ATT(__half, 64); else if (d == 128) ATT(__half, 128); else ATT(__half, 256); }
-#undef ATT
-  MSGL_CHECK_LAUNCH("paged_attention_fp4");
+  const int nb = row_blocks(d, max_q * (hq / hk)), workers = worker_count(d, nb);
+  int* status = nullptr;
+  cudaGetSymbolAddress((void**)&status, g_fp4_status);
+  float* ws = (float*)workspace;
+  const long long parts = 2ll * workers * nb * 8 * (d + 4);
+  for (int b0 = 0; b0 < B; b0 += kMost) {
+    Fp4Args a{};
+    a.B = B - b0 < kMost ? B - b0 : kMost;
+    a.q = q; a.out = out; a.pool = (const uint8_t*)pool;
+    a.table = (const int32_t*)table + b0 * table_stride; a.table_stride = table_stride; a.width = width;
+    a.cu_q = (const int32_t*)cu_q + b0; a.lens = (const int32_t*)lens + b0;
+    a.k_head = (const float*)k_head; a.v_head = (const float*)v_head; a.weights = (float*)weights;
+    a.parts = ws; a.line = (long long*)(ws + parts);
+    a.lse = weights != nullptr ? ws + parts + 2ll * ((B < kMost ? B : kMost) + 2) : nullptr;
+    a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.pages = pages; a.window = window;
+    a.row_tile = 8 * nb; a.workers = workers; a.scale = scale; a.status = status;
+    int rc = MSGL_BAD_ARG;
+    const int sms = device_sms();
+#define RUN(T, D, N) rc = launch<T, D, N>(a, total_rows, sms, stream)
+#define WIDTHS(T)                                                                                                          \
+  if (d == 64) { if (nb == 1) RUN(T, 64, 1); else if (nb == 2) RUN(T, 64, 2); else RUN(T, 64, 4); }                         \
+  else if (d == 128) { if (nb == 1) RUN(T, 128, 1); else if (nb == 2) RUN(T, 128, 2); else RUN(T, 128, 4); }                \
+  else { if (nb == 1) RUN(T, 256, 1); else RUN(T, 256, 2); }
+    if (dtype == MSGL_BF16) { WIDTHS(__nv_bfloat16) } else { WIDTHS(__half) }
+#undef WIDTHS
+#undef RUN
+    if (rc != MSGL_OK) return rc;
+  }
   return MSGL_OK;
+}
+
+MSGL_API int msgl_attention_fp4_status(int reset) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_fp4_status, sizeof(int));
+  if (reset && v != 0) {
+    const int z = 0;
+    cudaMemcpyToSymbol(g_fp4_status, &z, sizeof(int));
+  }
+  return v;
 }

@@ -13,7 +13,9 @@ from ._lib import c_f, c_i, c_ll, c_p, check, lib
 _lib.bind("msgl_store_fp4", c_i, [c_p, c_p, c_ll, c_ll] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 8 + [c_p])
-_lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_i] + [c_p] * 5 + [c_i] * 7 + [c_f, c_i, c_p])
+_lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 6 + [c_i] * 9 + [c_f, c_i, c_p])
+_lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 7)
+_lib.bind("msgl_attention_fp4_status", c_i, [c_i])
 
 TILE = 16                       # tokens of a tile
 WIDTHS = (64, 128, 256)
@@ -128,13 +130,26 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
-    block_table, cu_q, seq_lens = block_table.contiguous(), cu_q.contiguous(), seq_lens.contiguous()
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    cu_q, seq_lens = cu_q.contiguous(), seq_lens.contiguous()
+    t, b, hq = q.shape[0], seq_lens.numel(), q.shape[1]
+    if max_q == 0 and t and b:
+        max_q = int((cu_q[1:] - cu_q[:-1]).max())
+    need = int(lib().msgl_attention_fp4_workspace(t, b, hq, hk, dim, max_q, weights is not None))
+    if workspace is None or workspace.numel() < need or workspace.data_ptr() % 16:
+        workspace = torch.empty(need, dtype=torch.float32, device=q.device)
     check(lib().msgl_attention_fp4(
-        q.data_ptr(), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(),
-        seq_lens.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights), seq_lens.numel(), q.shape[1], hk, dim, page, pages, window,
-        scale, K._dt(q), K._stream()), "paged_attention_fp4")
-    K._count("paged_attention_fp4", "fp4_attention_simple_kernel")
+        q.data_ptr(), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        cu_q.data_ptr(), seq_lens.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights), workspace.data_ptr(), t, b, hq, hk, dim,
+        page, pages, max_q, window, scale, K._dt(q), K._stream()), "paged_attention_fp4")
+    K._count("paged_attention_fp4", "fp4_attention_kernel", 2 + (weights is not None))
     return out
+
+
+def attention_fp4_status(reset=True) -> int:
+    """Nonzero: a wait in the kernel ran out."""
+    return int(lib().msgl_attention_fp4_status(int(reset)))
 
 
 def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
