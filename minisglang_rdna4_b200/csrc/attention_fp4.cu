@@ -43,7 +43,7 @@ struct Fp4Args {
   float* weights;
   float* parts;             // [2 * workers][rows of a tile][D + 2]
   long long* line;          // [B + 2]: first tile of every request in the line, total; workers
-  int width, B, hq, hk, group, page_size, pages, window, row_tile, workers;
+  int width, B, hq, hk, group, page_size, per, pages, window, row_tile, workers;   // per: tiles of a page
   float scale;
   int* status;
 };
@@ -54,7 +54,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -148,11 +148,17 @@ struct Deal {
   }
 };
 
-// A place in the line.
+// A place in the line: a row tile (rt) of a key head of request b, and a tile of 16 tokens: sub of the page in column col of
+// the block table. Steps take no divisions.
 struct Walk {
-  int b, unit, tile;        // unit: head * row tiles + row tile
+  int b, head, rt, tile, col, sub;
   Request r;
-  __device__ __forceinline__ void seek(const Fp4Args& a, const long long* line, long long at) {
+  __device__ __forceinline__ void start_unit(const Fp4Args& a) {
+    tile = 0;
+    col = r.tile0 / a.per;
+    sub = r.tile0 - col * a.per;
+  }
+  __device__ __forceinline__ void seek(const Fp4Args& a, const long long* line, long long at, bool whole_rows) {
     int lo = 0, hi = a.B - 1;                   // the last request that starts at or before `at` has it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -161,28 +167,38 @@ struct Walk {
     b = lo;
     r.load(a, b);
     const long long o = at - line[b];
-    unit = (int)(o / max(r.tiles, 1));
+    const int unit = (int)(o / max(r.tiles, 1)), row_tiles = whole_rows ? 1 : max(r.row_tiles, 1);
     tile = (int)(o - (long long)unit * r.tiles);
+    head = unit / row_tiles;
+    rt = unit - head * row_tiles;
+    col = (r.tile0 + tile) / a.per;
+    sub = r.tile0 + tile - col * a.per;
+  }
+  // on to the next unit that has tiles
+  __device__ __forceinline__ void next_unit(const Fp4Args& a, const long long* line, bool whole_rows) {
+    if (!whole_rows && ++rt < r.row_tiles) { start_unit(a); return; }
+    rt = 0;
+    if (++head == a.hk) {
+      head = 0;
+      do ++b; while (b < a.B - 1 && line[b] == line[b + 1]);
+      r.load(a, min(b, a.B - 1));
+    }
+    start_unit(a);
   }
   // true where another unit begins
   __device__ __forceinline__ bool next(const Fp4Args& a, const long long* line, bool whole_rows) {
+    if (++sub == a.per) { sub = 0; ++col; }
     if (++tile < r.tiles) return false;
-    tile = 0;
-    if (++unit < a.hk * (whole_rows ? 1 : r.row_tiles)) return true;
-    unit = 0;
-    do ++b; while (b < a.B - 1 && line[b] == line[b + 1]);
-    r.load(a, min(b, a.B - 1));
+    next_unit(a, line, whole_rows);
     return true;
   }
   __device__ __forceinline__ int page(const Fp4Args& a) const {
-    const int col = min((r.tile0 + tile) * kTile / a.page_size, a.width - 1);
     const int page = a.table[(long long)b * a.table_stride + col];
     (void)MSGL_OOB(page, a.pages);
     return min(max(page, 0), a.pages - 1);
   }
-  template <int D> __device__ __forceinline__ long long address(const Fp4Args& a, int page, int head) const {
-    const int per = a.page_size / kTile;
-    return (((long long)page * a.hk + head) * per + (r.tile0 + tile) % per) * Tile<D>::bytes;
+  template <int D> __device__ __forceinline__ const uint8_t* address(const Fp4Args& a, int page) const {
+    return a.pool + (long long)((page * a.hk + head) * a.per + sub) * Tile<D>::bytes;
   }
 };
 
@@ -212,7 +228,7 @@ __device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, 
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int ex = (int)(__float_as_uint(top) >> 23);            // 0: zeros; 255: infinite
   const int up = top > 0.f && ex < 255 ? min(max(137 - ex, -126), 126) : 0;
-  const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+  const float f = copysignf(__uint_as_float((uint32_t)(127 + up) << 23), a.scale);     // a negative scale: on the query
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     float x[8];
@@ -282,10 +298,13 @@ template <int D, int NB> __device__ __forceinline__ void scores(const Raw<D>& x,
   }
 }
 
+// CTAs on an SM: what the registers allow without spilling the loop's values
+__host__ __device__ constexpr int ctas_of(int d, int nb) { return d == 256 ? (nb == 1 ? 3 : 2) : nb == 1 ? (d == 64 ? 5 : 4) : nb == 2 ? 3 : 2; }
+
 template <int D, int NB> struct Shape {
-  static constexpr int stages = D == 64 ? 6 : D == 128 ? 4 : 3;
-  static constexpr int ring = kWarps * stages * Tile<D>::bytes;
-  static constexpr int ctas = D == 256 ? (NB == 1 ? 3 : 2) : NB == 1 ? 4 : NB == 2 ? 3 : 2;
+  static constexpr int stages = D == 64 ? 4 : 2;         // of two tiles
+  static constexpr int ring = kWarps * stages * 2 * Tile<D>::bytes;
+  static constexpr int ctas = ctas_of(D, NB);
   static constexpr int smem = ring + kWarps * stages * 8 + 16 + (kMost + 2) * 8;
 };
 
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
   constexpr int STAGES = Shape<D, NB>::stages, BYTES = Tile<D>::bytes;
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint8_t* ring = smem + warp * STAGES * BYTES;
+  uint8_t* ring = smem + warp * STAGES * 2 * BYTES;
   const uint32_t bar = smem_u32(smem + Shape<D, NB>::ring) + warp * STAGES * 8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8);
   long long* line = reinterpret_cast<long long*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8 + 16);
@@ -312,170 +331,199 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
   // neighbours in the line lie on different SMs: a short line is spread over all of them
   const int worker = warp * gridDim.x + blockIdx.x;
   if (worker >= deal.workers) return;
-  long long at = deal.begin(worker);
-  const long long end = deal.begin(worker + 1);
-  if (at >= end) return;
+  const long long at = deal.begin(worker);
+  const int total = (int)(deal.begin(worker + 1) - at);     // tiles
+  if (total <= 0) return;
 
-  Walk get, put;                 // what is computed; what is fetched
-  get.seek(a, line, at);
-  put = get;
-  long long ahead = at;
-  int page = put.page(a);
-  auto fetch = [&](int stage) {  // the tile at `ahead`; then the page of the next one is asked for
-    if (lane == 0) {
-      mbar_expect_tx(bar + 8 * stage, BYTES);
-      bulk_load(smem_u32(ring + stage * BYTES), a.pool + put.address<D>(a, page, put.unit / put.r.row_tiles), BYTES, bar + 8 * stage);
+  // Tiles come in pairs, a stage for each. Lane i finds the places of pairs i, 32 + i, ... and fetches them: no step along the
+  // line for each tile.
+  const int pairs = (total + 1) / 2;
+  const uint8_t *mine0 = nullptr, *mine1 = nullptr;
+  int fetched = 0;
+  auto fetch = [&](int stage) {
+    if (fetched % 32 == 0) {
+      Walk w;
+      w.seek(a, line, at + min(2 * (fetched + lane), total - 1), false);
+      mine0 = w.address<D>(a, w.page(a));
+      w.seek(a, line, at + min(2 * (fetched + lane) + 1, total - 1), false);
+      mine1 = w.address<D>(a, w.page(a));
     }
-    if (++ahead < end) {
-      put.next(a, line, false);
-      page = put.page(a);
+    if (lane == fetched % 32) {
+      const bool both = 2 * fetched + 1 < total;
+      const uint32_t full = bar + 8 * stage, to = smem_u32(ring + stage * 2 * BYTES);
+      mbar_expect_tx(full, both ? 2 * BYTES : BYTES);
+      bulk_load(to, mine0, BYTES, full);
+      if (both) bulk_load(to + BYTES, mine1, BYTES, full);
     }
+    ++fetched;
   };
-  for (int s = 0; s < STAGES && ahead < end; ++s) fetch(s);
+  for (int s = 0; s < STAGES && s < pairs; ++s) fetch(s);
+  Walk get;
+  get.seek(a, line, at, false);
 
   const int g = lane >> 2, j = lane & 3;
-  int stage = 0;
+  int done = 0, stage = 0;       // done: tiles; stage: of the next one
   uint32_t phase = 0;
   bool ok = true;
-  while (at < end) {
+  while (done < total) {
     // ---- one unit, or this warp's part of it
-    const int first = get.tile, head = get.unit / get.r.row_tiles, row0 = (get.unit - head * get.r.row_tiles) * a.row_tile;
-    const int count = (int)min(end - at, (long long)(get.r.tiles - first));
+    const int first = get.tile, head = get.head, row0 = get.rt * a.row_tile;
+    const int count = min(total - done, get.r.tiles - first);
     const Request r = get.r;
     const int rows = min(a.row_tile, r.q_len * a.group - row0);
     uint32_t qf[NB][D / 8];
-    float cA[NB], cB[NB];        // factors of the scores of rows 2 j and 2 j + 1
-    const float kh = a.scale * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
+    float c[NB][2];              // factors of the scores of rows 2 j and 2 j + 1, above 0
+    const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const float back = load_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, qf[nb]);
-      cA[nb] = kh * __shfl_sync(0xffffffffu, back, 8 * j);
-      cB[nb] = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
+      c[nb][0] = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j), 1e-37f);
+      c[nb][1] = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j + 4), 1e-37f);
     }
-    float o[NB][D / 16][4], m[NB][2], l[NB][2];
+    // m: running maxima; base: what is taken from a score in the exponent
+    float o[NB][D / 16][4], m[NB][2], base[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
       m[nb][0] = m[nb][1] = -INFINITY;
+      base[nb][0] = base[nb][1] = -kUp;
       l[nb][0] = l[nb][1] = 0.f;
     }
-    // tokens that the first and the last row see: [lo, hi) all rows, outside of them some do not
+    // tokens [lo_all, hi_all) are seen by all rows
     const int pos0 = r.n - r.q_len + row0 / a.group, pos1 = r.n - r.q_len + (row0 + rows - 1) / a.group;
     const int hi_all = pos0 + 1, lo_all = a.window > 0 ? pos1 - a.window + 1 : 0;
 
-    for (int t = 0; t < count; ++t) {
-      if (ok) ok = mbar_wait(bar + 8 * stage, phase, abort_flag, a.status, 401);
-      ok = __all_sync(0xffffffffu, ok);
+    for (int t = 0; t < count;) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, phase, abort_flag, a.status, 401));
       if (!ok) break;
-      Raw<D> x;
-      load_keys<D>(ring + stage * BYTES, lane, x);
-      load_values<D>(ring + stage * BYTES, lane, x);
-      __syncwarp();
-      if (ahead < end) fetch(stage);
-      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-
-      const int tok0 = (r.tile0 + first + t) * kTile;
-      if (tok0 > pos1) continue;     // other rows of the request see it
-      float s[NB][4];
-      scores<D, NB>(x, qf, s);
-      const bool ragged = tok0 + kTile > hi_all || tok0 < lo_all;
-      bool move = false;
+      const uint8_t* tile = ring + stage * 2 * BYTES;
+      // of the stage's tiles one may be another unit's: `from` .. `to` are the tokens of this one, tok0 is the stage's first
+      const int u0 = done & 1, from = u0 * kTile, to = min(2, u0 + count - t) * kTile;
+      const int tok0 = (r.tile0 + first + t - u0) * kTile;
+      if (tok0 + from <= pos1) {                               // else rows behind these see it
+        float s[2][NB][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        s[nb][0] *= cA[nb]; s[nb][1] *= cB[nb]; s[nb][2] *= cA[nb]; s[nb][3] *= cB[nb];
-        if (ragged) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok = tok0 + token_of(g, i >> 1), pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + (i & 1)) / a.group;
-            if (tok > min(pos, r.n - 1) || (a.window > 0 && tok <= pos - a.window)) s[nb][i] = -INFINITY;
-          }
+        for (int u = 0; u < 2; ++u) {
+          Raw<D> x;
+          load_keys<D>(tile + u * BYTES, lane, x);
+          scores<D, NB>(x, qf, s[u]);
         }
-        move |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kSlack || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kSlack;
-      }
-      if (__any_sync(0xffffffffu, move)) {
+        const bool ragged = tok0 + 2 * kTile > hi_all || tok0 < lo_all || to - from < 2 * kTile;
+        bool move = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
+          if (ragged) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(s[nb][c], s[nb][2 + c]);
+            for (int k = 0; k < 2; ++k) {
+              const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + k) / a.group;
+              const int hi = min(min(pos + 1, r.n) - tok0, to), lo = max(a.window > 0 ? pos - a.window + 1 - tok0 : 0, from);
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            top = fmaxf(top, m[nb][c]);
-            const float f = m[nb][c] == top ? 1.f : exp2_fast(m[nb][c] - top);
-            m[nb][c] = top;
-            l[nb][c] *= f;
+              for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) { o[nb][i][c] *= f; o[nb][i][2 + c] *= f; }
-          }
-        }
-      }
-      uint32_t p0[NB], p1[NB];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float mA = (m[nb][0] == -INFINITY ? 0.f : m[nb][0]) - kUp, mB = (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) - kUp;
-        const float e0 = exp2_fast(s[nb][0] - mA), e1 = exp2_fast(s[nb][1] - mB), e2 = exp2_fast(s[nb][2] - mA),
-                    e3 = exp2_fast(s[nb][3] - mB);
-        l[nb][0] += e0 + e2;
-        l[nb][1] += e1 + e3;
-        p0[nb] = transpose8(f16x2(e0, e1));
-        p1[nb] = transpose8(f16x2(e2, e3));
-      }
-      // values of tokens that no row sees may be anything; a NaN that only some rows see must not reach the others
-      uint32_t nan_mask = 0;       // bit 4 i + e: token 4 j + e has no number in block i of the lane's channels
-      if (ragged) {
-#pragma unroll
-        for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t byte = x.vs[i] >> (8 * e) & 0x7F;
-            if (byte == 0x7F) {
-              nan_mask |= 1u << (4 * i + e);
-              x.vs[i] &= ~(0xFFu << (8 * e));
+                for (int h = 0; h < 2; ++h) {
+                  const int tok = u * kTile + token_of(g, h);
+                  if (tok >= hi || tok < lo) s[u][nb][2 * h + k] = -INFINITY;
+                }
             }
           }
-      }
 #pragma unroll
-      for (int w = 0; w < D / 64; ++w) {                  // words of 8 channels of the lane: 4 products
-        const int i = D == 256 ? w / 2 : 0;
-        const uint32_t s01 = widen_e4m3(x.vs[i]), s23 = widen_e4m3(x.vs[i] >> 16);
-        // words of tokens e = 0 .. 3: D / 64 words each
-        uint32_t tw[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x.v[k / 4], k % 4); }
-        uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
-        widen((tw[0] & 0x0F0F0F0Fu) | ((tw[1] << 4) & 0xF0F0F0F0u), lo01);
-        widen(((tw[0] >> 4) & 0x0F0F0F0Fu) | (tw[1] & 0xF0F0F0F0u), hi01);
-        widen((tw[2] & 0x0F0F0F0Fu) | ((tw[3] << 4) & 0xF0F0F0F0u), lo23);
-        widen(((tw[2] >> 4) & 0x0F0F0F0Fu) | (tw[3] & 0xF0F0F0F0u), hi23);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t a0 = times(lo01[k], s01), a1 = times(hi01[k], s01), a2 = times(lo23[k], s23), a3 = times(hi23[k], s23);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma(o[nb][4 * w + k], a0, a1, a2, a3, p0[nb], p1[nb]);
+          for (int k = 0; k < 2; ++k)
+            move |= fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) * c[nb][k] > m[nb][k] + kSlack;
         }
-      }
-      if (ragged && __any_sync(0xffffffffu, nan_mask != 0)) {
-        for (int jj = 0; jj < 4; ++jj) {
-          const uint32_t bits = __shfl_sync(0xffffffffu, nan_mask, 4 * g + jj);
-          for (int e = 0; e < 4; ++e) {
-            const int tok = tok0 + 4 * jj + e;
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+          for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + c) / a.group;
-                const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
+            for (int k = 0; k < 2; ++k) {
+              float top = fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) * c[nb][k];
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                  if (seen && (bits >> ((D == 256 ? i / 8 * 4 : 0) + e) & 1)) o[nb][i][c] = o[nb][i][2 + c] = NAN;
-              }
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              top = fmaxf(top, m[nb][k]);
+              const float f = m[nb][k] == top ? 1.f : exp2_fast(m[nb][k] - top);
+              m[nb][k] = top;
+              base[nb][k] = (top == -INFINITY ? 0.f : top) - kUp;
+              l[nb][k] *= f;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) { o[nb][i][k] *= f; o[nb][i][2 + k] *= f; }
+            }
           }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t p0[NB], p1[NB];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const float e0 = exp2_fast(fmaf(s[u][nb][0], c[nb][0], -base[nb][0])), e1 = exp2_fast(fmaf(s[u][nb][1], c[nb][1], -base[nb][1])),
+                        e2 = exp2_fast(fmaf(s[u][nb][2], c[nb][0], -base[nb][0])), e3 = exp2_fast(fmaf(s[u][nb][3], c[nb][1], -base[nb][1]));
+            l[nb][0] += e0 + e2;
+            l[nb][1] += e1 + e3;
+            p0[nb] = transpose8(f16x2(e0, e1));
+            p1[nb] = transpose8(f16x2(e2, e3));
+          }
+          Raw<D> x;
+          load_values<D>(tile + u * BYTES, lane, x);
+          // values of tokens that no row sees may be anything; a NaN that only some rows see must not reach the others
+          uint32_t nan_mask = 0;       // bit 4 i + e: token 4 j + e has no number in block i of the lane's channels
+          if (ragged) {
+#pragma unroll
+            for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((x.vs[i] >> (8 * e) & 0x7F) == 0x7F) {
+                  nan_mask |= 1u << (4 * i + e);
+                  x.vs[i] &= ~(0xFFu << (8 * e));
+                }
+          }
+#pragma unroll
+          for (int w = 0; w < D / 64; ++w) {                  // words of 8 channels of the lane: 4 products
+            const int i = D == 256 ? w / 2 : 0;
+            const uint32_t s01 = widen_e4m3(x.vs[i]), s23 = widen_e4m3(x.vs[i] >> 16);
+            uint32_t tw[4];                                    // of tokens 4 j .. 4 j + 3
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x.v[k / 4], k % 4); }
+            uint32_t lo01[4], hi01[4], lo23[4], hi23[4];       // pairs of tokens of the even and of the odd channels
+            widen((tw[0] & 0x0F0F0F0Fu) | ((tw[1] << 4) & 0xF0F0F0F0u), lo01);
+            widen(((tw[0] >> 4) & 0x0F0F0F0Fu) | (tw[1] & 0xF0F0F0F0u), hi01);
+            widen((tw[2] & 0x0F0F0F0Fu) | ((tw[3] << 4) & 0xF0F0F0F0u), lo23);
+            widen(((tw[2] >> 4) & 0x0F0F0F0Fu) | (tw[3] & 0xF0F0F0F0u), hi23);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a0 = times(lo01[k], s01), a1 = times(hi01[k], s01), a2 = times(lo23[k], s23), a3 = times(hi23[k], s23);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma(o[nb][4 * w + k], a0, a1, a2, a3, p0[nb], p1[nb]);
+            }
+          }
+          if (ragged && __any_sync(0xffffffffu, nan_mask != 0)) {
+            for (int jj = 0; jj < 4; ++jj) {
+              const uint32_t bits = __shfl_sync(0xffffffffu, nan_mask, 4 * g + jj);
+              for (int e = 0; e < 4; ++e) {
+                const int tok = u * kTile + 4 * jj + e;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + c) / a.group;
+                    const bool seen = tok < min(min(pos + 1, r.n) - tok0, to) && tok >= from &&
+                                      !(a.window > 0 && tok0 + tok <= pos - a.window);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                      if (seen && (bits >> ((D == 256 ? i / 8 * 4 : 0) + e) & 1)) o[nb][i][c] = o[nb][i][2 + c] = NAN;
+                  }
+              }
+            }
+          }
+        }
+      }
+      t += (to - from) / kTile;
+      done += (to - from) / kTile;
+      if (to == 2 * kTile) {
+        __syncwarp();
+        if (fetched < pairs) fetch(stage);
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
     }
     if (!ok) break;
-    at += count;
 
     // ---- rows 2 j and 2 j + 1 of every block: channels g D / 8 .. (D / 8 of them)
     const bool whole = first == 0 && count == r.tiles;
@@ -514,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
         }
       }
     }
-    if (at < end) { get.tile += count - 1; get.next(a, line, false); }
+    if (done < total) get.next_unit(a, line, false);
   }
   if (!ok) {     // copies may be in flight: they land before the shared memory goes
     const uint64_t t0 = globaltimer_ns();
@@ -522,52 +570,83 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
   }
 }
 
-// A warp for each (row, query head) whose unit several workers share, or that sees nothing: the parts joined.
-template <typename T, int D> __global__ void __launch_bounds__(256) fp4_join_kernel(const Fp4Args a, int total_rows) {
+// Rows of units that several workers share, or that see nothing: the parts joined. SPREAD warps of a CTA take the parts of one
+// (row, query head) in turn.
+template <typename T, int D, int SPREAD> __global__ void __launch_bounds__(256) fp4_join_kernel(const Fp4Args a, int total_rows) {
+  constexpr int E = D / 32, AHEAD = 4;
+  __shared__ float sum[8][D + 2];
   pdl_enter();
-  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (id >= (long long)total_rows * a.hq) return;
-  const int row = (int)(id / a.hq), qh = (int)(id % a.hq);
-  if (row < a.cu_q[0] || row >= a.cu_q[a.B]) return;      // of another launch, or of no request
-  int lo = 0, hi = a.B - 1;                               // the last request that starts at or before the row
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
-  }
-  Request r;
-  r.load(a, lo);
-  T* dst = reinterpret_cast<T*>(a.out) + id * D + lane * (D / 32);
-  constexpr int E = D / 32;
-  float y[E] = {};
-  if (r.tiles > 0) {
-    const Deal deal(a.line[a.B], a.workers);
-    const int head = qh / a.group, in_unit = (row - r.q0) * a.group + qh % a.group;
-    const int rt = in_unit / a.row_tile, in_tile = in_unit - rt * a.row_tile;
-    const long long u0 = a.line[lo] + ((long long)head * r.row_tiles + rt) * r.tiles;
-    const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
-    if (w0 == w1) return;                                // written by its worker
-    float m = -INFINITY, l = 0.f;
-    for (int w = w0; w <= w1; ++w) {
-      const float* part = a.parts + ((long long)(2 * w + (w == w0 ? 1 : 0)) * a.row_tile + in_tile) * (D + 4);
-      const float2 ml = *reinterpret_cast<const float2*>(part + D);
-      float x[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = part[lane * E + e];
-      const float top = fmaxf(m, ml.x);
-      const float f0 = m == top ? 1.f : exp2_fast(m - top), f1 = ml.x == top ? 1.f : exp2_fast(ml.x - top);
-      m = top;
-      l = l * f0 + ml.y * f1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + x[e] * f1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long id = (long long)blockIdx.x * (8 / SPREAD) + warp / SPREAD;
+  const int row = (int)(id / a.hq), qh = (int)(id - (long long)row * a.hq), mine = warp % SPREAD;
+  // of another launch, or of no request; the CTA's rows may differ in it
+  bool there = id < (long long)total_rows * a.hq && row >= a.cu_q[0] && row < a.cu_q[a.B], empty = false;
+  float m = -INFINITY, l = 0.f, y[E] = {};
+  int head = 0;
+  if (there) {
+    int lo = 0, hi = a.B - 1;                             // the last request that starts at or before the row
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
     }
-    const float f = l > 0.f || l != l ? (a.v_head != nullptr ? a.v_head[head] : 1.f) / l : 0.f;
+    Request r;
+    r.load(a, lo);
+    empty = r.tiles == 0;
+    if (!empty) {
+      const Deal deal(a.line[a.B], a.workers);
+      head = qh / a.group;
+      const int in_unit = (row - r.q0) * a.group + qh - head * a.group;
+      const int rt = in_unit / a.row_tile, in_tile = in_unit - rt * a.row_tile;
+      const long long u0 = a.line[lo] + ((long long)head * r.row_tiles + rt) * r.tiles;
+      const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
+      there = w0 != w1;                                   // else written by its worker
+      for (int wb = w0 + mine; there && wb <= w1; wb += AHEAD * SPREAD) {
+        float2 ml[AHEAD];
+        float x[AHEAD][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] *= f;
-    if (a.lse != nullptr && lane == 0) a.lse[id] = (m == -INFINITY ? 0.f : m) - kUp + log2f(l);
+        for (int i = 0; i < AHEAD; ++i) {
+          const int w = wb + i * SPREAD;
+          ml[i] = make_float2(-INFINITY, 0.f);
+          const float* part = a.parts + ((long long)(2 * w + (w == w0 ? 1 : 0)) * a.row_tile + in_tile) * (D + 4);
+          if (w <= w1) ml[i] = *reinterpret_cast<const float2*>(part + D);
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[i][e] = w <= w1 ? part[lane * E + e] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const float top = fmaxf(m, ml[i].x);
+          const float f0 = m == top ? 1.f : exp2_fast(m - top), f1 = ml[i].x == top ? 1.f : exp2_fast(ml[i].x - top);
+          m = top;
+          l = l * f0 + ml[i].y * f1;
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + x[i][e] * f1;
+        }
+      }
+    }
   }
+  if (SPREAD > 1) {
+    if (mine != 0) {
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<typename Pack2<T>::type*>(dst + e) = Pack2<T>::make(y[e], y[e + 1]);
+      for (int e = 0; e < E; ++e) sum[warp][lane * E + e] = y[e];
+      if (lane == 0) { sum[warp][D] = m; sum[warp][D + 1] = l; }
+    }
+    __syncthreads();
+    if (mine != 0) return;
+    for (int k = 1; k < SPREAD; ++k) {
+      const float* o = sum[warp + k];
+      const float top = fmaxf(m, o[D]), f0 = m == top ? 1.f : exp2_fast(m - top), f1 = o[D] == top ? 1.f : exp2_fast(o[D] - top);
+      m = top;
+      l = l * f0 + o[D + 1] * f1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + o[lane * E + e] * f1;
+    }
+  }
+  if (!there) return;
+  const float f = l > 0.f || l != l ? (a.v_head != nullptr ? a.v_head[head] : 1.f) / l : 0.f;
+  if (a.lse != nullptr && lane == 0 && !empty) a.lse[id] = (m == -INFINITY ? 0.f : m) - kUp + log2f(l);
+  T* dst = reinterpret_cast<T*>(a.out) + id * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<typename Pack2<T>::type*>(dst + e) = Pack2<T>::make(y[e] * f, y[e + 1] * f);
 }
 
 // What the rows give every token: the keys once more, with the rows' final maxima and sums. The warps deal out the tiles of
@@ -584,17 +663,17 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32, D ==
   const long long end = deal.begin(worker + 1);
   if (at >= end) return;
   Walk get;
-  get.seek(a, line, at);
+  get.seek(a, line, at, true);
   uint32_t qf[1][D / 8];
   float cA = 0.f, cB = 0.f, eA = 0.f, eB = 0.f;
   bool fresh = true;
   while (at < end) {
     const Request& r = get.r;
-    const int head = get.unit, page = get.page(a), tok0 = (r.tile0 + get.tile) * kTile;
+    const int head = get.head, page = get.page(a), tok0 = (r.tile0 + get.tile) * kTile;
     Raw<D> x;
-    load_keys<D>(a.pool + get.address<D>(a, page, head), lane, x);
+    load_keys<D>(get.address<D>(a, page), lane, x);
     const int rows = r.q_len * a.group;
-    const float kh = a.scale * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
+    const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
     float sum0 = 0.f, sum1 = 0.f;
     for (int row0 = 0; row0 < rows; row0 += 8) {
       const int posA = r.n - r.q_len + (row0 + 2 * j) / a.group, posB = r.n - r.q_len + (row0 + 2 * j + 1) / a.group;
@@ -635,6 +714,77 @@ template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32, D ==
   }
 }
 
+// Rows that a prompt step sees, in 16 bits, for the tensor-core kernel of prompts (attention_tc.cu): keys [Hk][t_cap][128] and
+// values transposed [Hk][128][t_cap], zeros where a request has no token and behind the 64 channels of narrow heads; the heads'
+// factors go to scores and output there. A warp has a tile and a head: values leave 16 tokens of a channel at a time (32
+// bytes), as the lanes hold them. Bound: the 512 bytes written for a token and head.
+template <typename T, int D> __global__ void __launch_bounds__(256)
+fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const int* __restrict__ blk_req, const int* __restrict__ req_info,
+                  long long t_cap, int tiles) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, id = blockIdx.x * 8 + (threadIdx.x >> 5), g = lane >> 2, j = lane & 3;
+  if (id >= tiles) return;
+  const int h = blockIdx.y, t0 = id * kTile, req = blk_req[t0 >> 7];
+  const int tok0 = t0 - req_info[3 * req] + req_info[3 * req + 2], n = req_info[3 * req + 1];
+  Raw<D> x = {};
+  if (tok0 < n) {
+    int page = a.table[(long long)req * a.table_stride + min(tok0 / a.page_size, a.width - 1)];
+    (void)MSGL_OOB(page, a.pages);
+    page = min(max(page, 0), a.pages - 1);
+    const uint8_t* tile = a.pool + ((long long)(page * a.hk + h) * a.per + tok0 / kTile % a.per) * Tile<D>::bytes;
+    load_keys<D>(tile, lane, x);
+    load_values<D>(tile, lane, x);
+  }
+  auto to_t = [](uint32_t f16) {
+    if (sizeof(T) == 2 && __is_same(T, __half)) return f16;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&f16));
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&b);
+  };
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int t = token_of(g, r);
+    const bool there = tok0 + t < n;
+    T* row = kc + ((long long)h * t_cap + t0 + t) * 128;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      uint32_t k[4];
+      widen(key_word<D>(x, r, w), k);
+      const uint32_t s = key_scale<D>(x, r, w / 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = there ? to_t(times(k[i], s)) : 0u;
+      *reinterpret_cast<uint4*>(row + j * (D / 4) + 8 * w) = make_uint4(k[0], k[1], k[2], k[3]);
+    }
+    if (D == 64)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) *reinterpret_cast<uint4*>(row + 64 + j * 16 + 8 * w) = make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)                  // what lies behind the request may be anything
+    if (tok0 + 4 * j + e >= n) x.vs[0] &= ~(0xFFu << (8 * e));
+  const uint32_t s01 = widen_e4m3(x.vs[0]), s23 = widen_e4m3(x.vs[0] >> 16);
+#pragma unroll
+  for (int w = 0; w < D / 64; ++w) {
+    uint32_t tw[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x.v[k / 4], k % 4); }
+    uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
+    widen((tw[0] & 0x0F0F0F0Fu) | ((tw[1] << 4) & 0xF0F0F0F0u), lo01);
+    widen(((tw[0] >> 4) & 0x0F0F0F0Fu) | (tw[1] & 0xF0F0F0F0u), hi01);
+    widen((tw[2] & 0x0F0F0F0Fu) | ((tw[3] << 4) & 0xF0F0F0F0u), lo23);
+    widen(((tw[2] >> 4) & 0x0F0F0F0Fu) | (tw[3] & 0xF0F0F0F0u), hi23);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      T* to = vt + ((long long)h * 128 + g * (D / 8) + 8 * w + 2 * k) * t_cap + t0 + 4 * j;
+      *reinterpret_cast<uint2*>(to) = make_uint2(to_t(times(lo01[k], s01)), to_t(times(lo23[k], s23)));
+      *reinterpret_cast<uint2*>(to + t_cap) = make_uint2(to_t(times(hi01[k], s01)), to_t(times(hi23[k], s23)));
+    }
+  }
+  if (D == 64)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint2*>(vt + ((long long)h * 128 + 64 + g * 8 + i) * t_cap + t0 + 4 * j) = make_uint2(0, 0);
+}
+
 template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows, int sms, cudaStream_t stream) {
   using S = Shape<D, NB>;
   static bool ready[64] = {};
@@ -647,7 +797,11 @@ template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows
   }
   msgl_launch(fp4_attention_kernel<T, D, NB>, dim3(a.workers / kWarps), dim3(kWarps * 32), S::smem, stream, a);
   MSGL_CHECK_LAUNCH("paged_attention_fp4");
-  msgl_launch(fp4_join_kernel<T, D>, dim3((unsigned)(((long long)total_rows * a.hq + 7) / 8)), dim3(256), 0, stream, a, total_rows);
+  // a row's parts are some workers / (requests * key heads * row tiles): up to four for a warp
+  const long long rows = (long long)total_rows * a.hq, each = (long long)a.workers * a.row_tile / (rows > 0 ? rows : 1);
+  if (each < 8) msgl_launch(fp4_join_kernel<T, D, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a, total_rows);
+  else if (each < 16) msgl_launch(fp4_join_kernel<T, D, 2>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, total_rows);
+  else msgl_launch(fp4_join_kernel<T, D, 8>, dim3((unsigned)rows), dim3(256), 0, stream, a, total_rows);
   MSGL_CHECK_LAUNCH("paged_attention_fp4 join");
   if (a.weights != nullptr) {
     msgl_launch(fp4_weights_kernel<T, D>, dim3(sms * (D == 256 ? 3 : 4)), dim3(kWarps * 32), 0, stream, a);
@@ -669,8 +823,7 @@ int device_sms() {
 }
 
 int worker_count(int d, int nb) {
-  const int ctas = d == 256 ? (nb == 1 ? 3 : 2) : nb == 1 ? 4 : nb == 2 ? 3 : 2;
-  return device_sms() * ctas * kWarps;
+  return device_sms() * ctas_of(d, nb) * kWarps;
 }
 
 }  // namespace
@@ -708,7 +861,7 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
     a.k_head = (const float*)k_head; a.v_head = (const float*)v_head; a.weights = (float*)weights;
     a.parts = ws; a.line = (long long*)(ws + parts);
     a.lse = weights != nullptr ? ws + parts + 2ll * ((B < kMost ? B : kMost) + 2) : nullptr;
-    a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.pages = pages; a.window = window;
+    a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages; a.window = window;
     a.row_tile = 8 * nb; a.workers = workers; a.scale = scale; a.status = status;
     int rc = MSGL_BAD_ARG;
     const int sms = device_sms();
@@ -722,6 +875,28 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
 #undef RUN
     if (rc != MSGL_OK) return rc;
   }
+  return MSGL_OK;
+}
+
+MSGL_API int msgl_gather_fp4(const void* pool, const void* table, long long table_stride, int width, void* kc, void* vt, const void* blk_req,
+                             const void* req_info, long long t_cap, int t_pad, int hk, int d, int page_size, int pages, int dtype,
+                             cudaStream_t stream) {
+  if (t_pad <= 0) return MSGL_OK;
+  if (hk <= 0 || (d != 64 && d != 128) || page_size <= 0 || page_size % kTile || (uintptr_t)pool % 16 || t_pad % 128 || t_pad > t_cap ||
+      width <= 0 || (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
+    msgl_set_error_text("gather of a 4-bit pool: heads of 64 or 128 channels, blocks of 128 rows");
+    return MSGL_BAD_ARG;
+  }
+  Fp4Args a{};
+  a.pool = (const uint8_t*)pool; a.table = (const int32_t*)table; a.table_stride = table_stride; a.width = width;
+  a.hk = hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages;
+  const int tiles = t_pad / kTile;
+  const dim3 grid((tiles + 7) / 8, hk);
+#define GATHER(T, D) msgl_launch(fp4_gather_kernel<T, D>, grid, dim3(256), 0, stream, a, (T*)kc, (T*)vt, (const int*)blk_req, (const int*)req_info, t_cap, tiles)
+  if (dtype == MSGL_BF16) { if (d == 64) GATHER(__nv_bfloat16, 64); else GATHER(__nv_bfloat16, 128); }
+  else { if (d == 64) GATHER(__half, 64); else GATHER(__half, 128); }
+#undef GATHER
+  MSGL_CHECK_LAUNCH("gather of a 4-bit pool");
   return MSGL_OK;
 }
 

@@ -1153,7 +1153,7 @@ MSGL_API int msgl_attn_prefill_tc(const void* q, long long q_row_stride, void* o
     return MSGL_BAD_ARG;
   }
   const bool ext = d != kD || window > 0 || chunk > 0 || softcap > 0.f || gate != nullptr;
-  if ((ext || pos_form) && (dtype != MSGL_BF16 || kv_fp8)) {
+  if ((ext || pos_form) && (dtype != MSGL_BF16 || kv_fp8 == 1)) {
     msgl_set_error_text("prefill attention: reaches, soft caps, gates, rows of 64 and unpaired query heads need bf16");
     return MSGL_BAD_ARG;
   }
@@ -1201,7 +1201,8 @@ MSGL_API int msgl_attn_prefill_tc(const void* q, long long q_row_stride, void* o
   msgl_launch(kv_gather_kernel<T, F8, ROW>, dim3(ggrid), dim3(256), 0, stream, k_pool, v_pool, (T*)kc, (T*)vt, (const int*)blk_req,          \
                                                      (const int*)req_info, (const int*)block_table, bt_stride, hk, \
                                                      page_size, t_cap, v_rows)
-  if (d == 64) GATHER(__nv_bfloat16, false, 64);
+  if (kv_fp8 == 2) {}
+  else if (d == 64) GATHER(__nv_bfloat16, false, 64);
   else if (dtype == MSGL_BF16) { if (kv_fp8) GATHER(__nv_bfloat16, true, 128); else GATHER(__nv_bfloat16, false, 128); }
   else { if (kv_fp8) GATHER(__half, true, 128); else GATHER(__half, false, 128); }
 #undef GATHER

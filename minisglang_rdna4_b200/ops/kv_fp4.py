@@ -4,6 +4,7 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -15,6 +16,7 @@ _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll
 _lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 8 + [c_p])
 _lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 6 + [c_i] * 9 + [c_f, c_i, c_p])
 _lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 7)
+_lib.bind("msgl_gather_fp4", c_i, [c_p, c_p, c_ll, c_i] + [c_p] * 4 + [c_ll] + [c_i] * 6 + [c_p])
 _lib.bind("msgl_attention_fp4_status", c_i, [c_i])
 
 TILE = 16                       # tokens of a tile
@@ -132,6 +134,8 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v
     out = torch.empty_like(q)
     if block_table.stride(1) != 1:
         block_table = block_table.contiguous()
+    if plan is not None:
+        return _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window)
     cu_q, seq_lens = cu_q.contiguous(), seq_lens.contiguous()
     t, b, hq = q.shape[0], seq_lens.numel(), q.shape[1]
     if max_q == 0 and t and b:
@@ -152,5 +156,47 @@ def attention_fp4_status(reset=True) -> int:
     return int(lib().msgl_attention_fp4_status(int(reset)))
 
 
+class PromptPlan(K.PrefillPlan):
+    """The tables, and the window that they are for."""
+
+    __slots__ = ("window", "group", "dim")
+
+
 def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
-    return None
+    """The tcgen05 form of prompts: heads of 128 channels in pairs that share a key head, any types of 16 bits; for bf16 also of
+    64 channels, unpaired heads and windows."""
+    hk, dim = cache.shape[1], cache.shape[3] // 18
+    group = q.shape[1] // hk
+    if dim == 256 or (q.dtype != torch.bfloat16 and (dim != 128 or group % 2 or window > 0)):
+        return None
+    cu_q, seq_lens = (np.minimum(np.asarray(x, dtype=np.int64), 1 << 30) for x in (cu_q, seq_lens))
+    b = seq_lens.size
+    if b == 0 or (np.diff(cu_q) > seq_lens).any():            # rows in front of their text
+        return None
+    if not K.tc_prefill_pays(int(cu_q[b]), K.PrefillPlan.rows_in_reach(cu_q, seq_lens, window)):
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a prefill plan is made of lengths on the host, outside of a graph's capture")
+    plan = PromptPlan(cu_q, seq_lens, q.device, window, tile=256 if group % 2 else 128)
+    plan.window, plan.group, plan.dim = window, group, dim
+    return plan
+
+
+def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window):
+    _, pages, hk, page, dim = pool_shape(cache)
+    if not isinstance(plan, PromptPlan) or (plan.window, plan.group, plan.dim) != (window, q.shape[1] // hk, dim):
+        raise ValueError("the prefill plan was made for another window or other heads")
+    if scale <= 0:
+        raise ValueError("the form for prompts takes a scale above 0")
+    kc, vt, cap = K._tc_scratch(q.device, q.dtype, hk, plan.t_pad)
+    base = plan.tables.data_ptr()
+    blk, req = base + 4 * plan.off_blk, base + 4 * plan.off_req
+    check(lib().msgl_gather_fp4(cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], kc.data_ptr(),
+                                vt.data_ptr(), blk, req, cap, plan.t_pad, hk, dim, page, pages, K._dt(q), K._stream()), "gather_fp4")
+    check(lib().msgl_attn_prefill_tc(
+        q.data_ptr(), q.stride(0), out.data_ptr(), None, None, kc.data_ptr(), vt.data_ptr(), cap, plan.t_pad, base, plan.n_items, blk,
+        req, block_table.data_ptr(), block_table.stride(0), K._p(k_scale), K._p(v_scale), q.shape[0], q.shape[1], hk, dim, page, 2,
+        float(scale), int(window), 0, 0.0, None, 0, None, 0, 0, None, 0, int(plan.tile == 256), K._dt(q), K._stream()),
+        "attn_prefill_tc")
+    K._count("paged_attention_fp4 (prompts)", "fp4_gather_kernel + attn_prefill_tc_kernel", 2)
+    return out

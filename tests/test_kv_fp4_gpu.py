@@ -160,6 +160,52 @@ def test_rows(dim, hq, hk, weighed):
     attend([30, 100, 513, 40, 77], [30, 0, 5, 1, 70], hq, hk, dim, weighed=weighed, powers=False)
 
 
+PROMPTS = [(8, 2, 128, torch.bfloat16, 0), (8, 2, 128, torch.float16, 0), (7, 1, 128, torch.bfloat16, 0), (6, 6, 64, torch.bfloat16, 0),
+           (8, 4, 64, torch.bfloat16, 0), (8, 2, 128, torch.bfloat16, 100), (5, 1, 64, torch.bfloat16, 300)]
+
+
+@pytest.mark.parametrize("hq,hk,dim,dtype,window", PROMPTS, ids=["-".join(map(str, p)) for p in PROMPTS])
+def test_prompts(hq, hk, dim, dtype, window):
+    """With a plan: the tensor-core form. Its probabilities go into the second product in q's type."""
+    lens, news, page = [300, 129, 128, 700, 5], [300, 128, 5, 200, 5], 32
+    table, pages = tables(lens, page)
+    cache, ks, vs, _, _ = make(pages, hk, page, dim, powers=False)
+    # what lies behind the requests and in no page may be anything
+    cache[int(table[4, -1])] = 0x7F
+    cu = ints([0] + torch.tensor(news).cumsum(0).tolist())
+    q = torch.randn(sum(news), hq, dim, device="cuda").to(dtype)
+    plan = ops.prefill_plan_fp4(q, cache, cu.cpu().numpy(), ints(lens).cpu().numpy(), window)
+    assert plan is not None
+    out = ops.paged_attention_fp4(q, cache, table, cu, ints(lens), 0.1, k_scale=ks, v_scale=vs, window=window, max_q=300, max_kv=700,
+                                  plan=plan)
+    values = plain.values(cache, ks, vs)
+    want, tol, _, _ = plain.attention(q, *values, table, cu, ints(lens), 0.1, window)
+    if dtype == torch.bfloat16:
+        # 8 bits in place of 11 for the probabilities: the sum of weighted magnitudes times 2^-8 more. That sum is the attention
+        # over the magnitudes of the values
+        size = torch.zeros_like(want)
+        weight = lambda v: plain.attention(q, values[0], v, table, cu, ints(lens), 0.1, window)[0]  # noqa: E731
+        size = weight(values[1].abs())
+        tol = tol + size * 2.0 ** -8
+    assert torch.isfinite(out).all()
+    assert ((out.cpu().double() - want).abs() <= tol).all(), float(((out.cpu().double() - want).abs() / tol).max())
+    with pytest.raises(ValueError):
+        ops.paged_attention_fp4(q, cache, table, cu, ints(lens), 0.1, window=window + 1, max_q=300, plan=plan)
+
+
+def test_steps_that_take_no_prompt_form():
+    cache = torch.zeros(4, 2, 1, 18 * 128, dtype=torch.uint8, device="cuda")
+    n = lambda *x: torch.tensor(x, dtype=torch.int32).numpy()  # noqa: E731
+    q = torch.zeros(200, 4, 128, device="cuda", dtype=torch.bfloat16)
+    assert ops.prefill_plan_fp4(q, cache, n(0, 200), n(200)) is not None
+    assert ops.prefill_plan_fp4(q, cache, n(0, 200), n(100)) is None              # more rows than tokens
+    assert ops.prefill_plan_fp4(q[:20], cache, n(0, 20), n(50000)) is None        # few rows for the keys
+    assert ops.prefill_plan_fp4(q[:0], cache, n(0), n()) is None
+    assert ops.prefill_plan_fp4(q.half(), cache, n(0, 200), n(200), 64) is None
+    wide = torch.zeros(4, 2, 1, 18 * 256, dtype=torch.uint8, device="cuda")
+    assert ops.prefill_plan_fp4(torch.zeros(200, 4, 256, device="cuda").half(), wide, n(0, 200), n(200)) is None
+
+
 def test_more_rows_than_tokens():
     """Rows in front of the text see nothing."""
     attend([3, 0, 20], [5, 2, 20], 4, 2, 64, weighed=True)
