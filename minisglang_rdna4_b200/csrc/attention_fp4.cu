@@ -649,68 +649,214 @@ template <typename T, int D, int SPREAD> __global__ void __launch_bounds__(256) 
   for (int e = 0; e < E; e += 2) *reinterpret_cast<typename Pack2<T>::type*>(dst + e) = Pack2<T>::make(y[e] * f, y[e + 1] * f);
 }
 
-// What the rows give every token: the keys once more, with the rows' final maxima and sums. The warps deal out the tiles of
-// all (request, key head) pairs; a tile goes through all rows of its pair.
-template <typename T, int D> __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 3 : 4) fp4_weights_kernel(const Fp4Args a) {
-  __shared__ long long line[kMost + 2];
+// What the rows give every token: the keys once more, with the rows' final maxima and sums. A tile's keys go through all rows of
+// their (request, key head) pair, so a token's sum is taken by one lane in one order. MANY false: up to 8 rows, in registers;
+// warps deal out the tiles of all pairs. MANY: CTAs do; the pair's queries lie in shared memory, kChunk blocks of 8 rows at
+// a time, and the warps take the CTA's tiles in turn. A warp has four tiles' keys under way.
+template <int D, bool MANY> struct WeightsShape {
+  static constexpr int stages = 4, key_bytes = 9 * D;                  // codes and scales
+  static constexpr int chunk = !MANY ? 0 : D == 256 ? 4 : 8;           // blocks of 8 rows
+  static constexpr int ctas = D == 256 ? 2 : 4;
+  static constexpr int ring = kWarps * stages * key_bytes, bars = ring, slots = bars + kWarps * stages * 8;
+  static constexpr int flag = slots + kWarps * stages * 4, line = flag + 16, queries = line + (kMost + 2) * 8;
+  static constexpr int rows = queries + chunk * 16 * D, smem = rows + chunk * 8 * 8;
+};
+
+// keys of a tile as the first operand
+template <int D> __device__ __forceinline__ void key_operand(const Raw<D>& x, uint32_t (&k)[D / 16][4]) {
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const uint32_t s0 = key_scale<D>(x, 0, i), s1 = key_scale<D>(x, 1, i);
+#pragma unroll
+    for (int w = 2 * i; w < 2 * i + 2; ++w) {
+      uint32_t h0[4], h1[4];
+      widen(key_word<D>(x, 0, w), h0);
+      widen(key_word<D>(x, 1, w), h1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        k[2 * w + c][0] = times(h0[2 * c], s0);
+        k[2 * w + c][1] = times(h1[2 * c], s1);
+        k[2 * w + c][2] = times(h0[2 * c + 1], s0);
+        k[2 * w + c][3] = times(h1[2 * c + 1], s1);
+      }
+    }
+  }
+}
+
+template <typename T, int D, bool MANY>
+__global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_weights_kernel(const Fp4Args a) {
+  using S = WeightsShape<D, MANY>;
+  constexpr int STAGES = S::stages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  uint8_t* ring = smem + warp * STAGES * S::key_bytes;
+  const uint32_t bar = smem_u32(smem + S::bars) + warp * STAGES * 8;
+  int* slots = reinterpret_cast<int*>(smem + S::slots) + warp * STAGES;        // of the pool: the stages' tiles
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::flag);
+  long long* line = reinterpret_cast<long long*>(smem + S::line);
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(bar + 8 * s, 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
   pdl_enter();
   lay_line(a, line, true);
-  Deal deal(line[a.B], gridDim.x * kWarps);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-  const int worker = warp * gridDim.x + blockIdx.x;
+  const Deal deal(line[a.B], MANY ? gridDim.x : gridDim.x * kWarps);
+  const int worker = MANY ? blockIdx.x : warp * gridDim.x + blockIdx.x;
   if (worker >= deal.workers) return;
   long long at = deal.begin(worker);
   const long long end = deal.begin(worker + 1);
   if (at >= end) return;
-  Walk get;
-  get.seek(a, line, at, true);
-  uint32_t qf[1][D / 8];
-  float cA = 0.f, cB = 0.f, eA = 0.f, eB = 0.f;
-  bool fresh = true;
-  while (at < end) {
-    const Request& r = get.r;
-    const int head = get.head, page = get.page(a), tok0 = (r.tile0 + get.tile) * kTile;
-    Raw<D> x;
-    load_keys<D>(get.address<D>(a, page), lane, x);
-    const int rows = r.q_len * a.group;
-    const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
-    float sum0 = 0.f, sum1 = 0.f;
-    for (int row0 = 0; row0 < rows; row0 += 8) {
-      const int posA = r.n - r.q_len + (row0 + 2 * j) / a.group, posB = r.n - r.q_len + (row0 + 2 * j + 1) / a.group;
-      if (fresh || rows > 8) {
-        const float back = load_query<T, D>(a, r, head, row0 + g, lane, qf[0]);
-        cA = kh * __shfl_sync(0xffffffffu, back, 8 * j);
-        cB = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
-        auto lse = [&](int row) {
-          if (row >= rows) return INFINITY;                // weight 0
-          const int qi = row / a.group;
-          return a.lse[(long long)(r.q0 + qi) * a.hq + head * a.group + row - qi * a.group];
-        };
-        eA = lse(row0 + 2 * j);
-        eB = lse(row0 + 2 * j + 1);
-      }
-      float s[1][4];
-      scores<D, 1>(x, qf, s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = tok0 + token_of(g, i >> 1), pos = i & 1 ? posB : posA;
-        const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
-        const float p = seen && (i & 1 ? eB : eA) != INFINITY ? exp2_fast(s[0][i] * (i & 1 ? cB : cA) - (i & 1 ? eB : eA)) : 0.f;
-        if (i < 2) sum0 += p; else sum1 += p;
-      }
+
+  // tiles first, first + step, ... of the line, `count` of them
+  long long first = at;
+  const int step = MANY ? kWarps : 1;
+  int count = 0, fetched = 0, done = 0, uses = 0, mine = 0;        // uses: stages used up before this run of tiles
+  auto fetch = [&]() {
+    if (fetched % 32 == 0) {
+      Walk w;
+      w.seek(a, line, first + (long long)min(fetched + lane, count - 1) * step, true);
+      mine = (w.page(a) * a.hk + w.head) * a.per + w.sub;
     }
-    fresh = false;
+    if (lane == fetched % 32) {
+      const int s = (uses + fetched) % STAGES;
+      const uint8_t* tile = a.pool + (long long)mine * Tile<D>::bytes;
+      const uint32_t to = smem_u32(ring + s * S::key_bytes);
+      slots[s] = mine;
+      mbar_expect_tx(bar + 8 * s, S::key_bytes);
+      bulk_load(to, tile, 8 * D, bar + 8 * s);
+      bulk_load(to + 8 * D, tile + Tile<D>::k_sf, D, bar + 8 * s);
+    }
+    ++fetched;
+  };
+  uint32_t k[D / 16][4];
+  int slot = 0;
+  bool ok = true;
+  auto next_keys = [&]() {          // waits for the next tile, takes its keys and lets another one in
+    const int s = (uses + done) % STAGES;
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(bar + 8 * s, (uses + done) / STAGES & 1, abort_flag, a.status, 402));
+    if (!ok) return;
+    Raw<D> x;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) x.k[i] = *reinterpret_cast<const uint4*>(ring + s * S::key_bytes + 512 * i + 16 * lane);
+    const uint8_t* sf = ring + s * S::key_bytes + 8 * D + lane * (D / 32);
+    if (D == 64) x.ks[0] = *reinterpret_cast<const uint16_t*>(sf);
+    else
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) x.ks[i] = *reinterpret_cast<const uint32_t*>(sf + 4 * i);
+    slot = slots[s];
+    key_operand<D>(x, k);
+    __syncwarp();
+    ++done;
+    if (fetched < count) fetch();
+    __syncwarp();
+  };
+  // weights that the two rows 2 j, 2 j + 1 of a block give tokens of rows g and g + 8
+  auto given = [&](const Request& r, int row0, int tok0, const float (&s)[4], float cA, float cB, float eA, float eB, float& s0, float& s1) {
+    const int posA = r.n - r.q_len + (row0 + 2 * j) / a.group, posB = r.n - r.q_len + (row0 + 2 * j + 1) / a.group;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = tok0 + token_of(g, i >> 1), pos = i & 1 ? posB : posA;
+      const float c = i & 1 ? cB : cA, e = i & 1 ? eB : eA;
+      const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
+      const float p = seen && e != INFINITY ? exp2_fast(s[i] * c - e) : 0.f;
+      if (i < 2) s0 += p; else s1 += p;
+    }
+  };
+  auto give = [&](const Request& r, int tok0, float s0, float s1) {
 #pragma unroll
     for (int d = 1; d < 4; d <<= 1) {
-      sum0 += __shfl_xor_sync(0xffffffffu, sum0, d);
-      sum1 += __shfl_xor_sync(0xffffffffu, sum1, d);
+      s0 += __shfl_xor_sync(0xffffffffu, s0, d);
+      s1 += __shfl_xor_sync(0xffffffffu, s1, d);
     }
-    if (j < 2) {      // lane 0 of the four has row g's token, lane 1 row g + 8's
-      const int t = token_of(g, j);
-      if (tok0 + t < r.n)
-        atomicAdd(a.weights + ((long long)page * a.hk + head) * a.page_size + tok0 % a.page_size + t, j ? sum1 : sum0);
+    const int t = token_of(g, j & 1);      // lane 0 of the four has row g's token, lane 1 row g + 8's
+    if (j < 2 && tok0 + t < r.n) atomicAdd(a.weights + (long long)slot * kTile + t, j ? s1 : s0);
+  };
+  auto lse_of = [&](const Request& r, int head, int row) {
+    if (row >= r.q_len * a.group) return INFINITY;         // weight 0
+    const int qi = row / a.group;
+    return a.lse[(long long)(r.q0 + qi) * a.hq + head * a.group + row - qi * a.group];
+  };
+  Walk get;
+  get.seek(a, line, at, true);
+  if constexpr (!MANY) {
+    count = (int)(end - at);
+    for (int s = 0; s < min(STAGES, count); ++s) fetch();
+    __syncwarp();
+    uint32_t qf[D / 8];
+    float cA = 0.f, cB = 0.f, eA = 0.f, eB = 0.f;
+    bool fresh = true;
+    while (done < count) {
+      if (fresh) {
+        const float back = load_query<T, D>(a, get.r, get.head, g, lane, qf);
+        const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[get.head] : 1.f);
+        cA = kh * __shfl_sync(0xffffffffu, back, 8 * j);
+        cB = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
+        eA = lse_of(get.r, get.head, 2 * j);
+        eB = lse_of(get.r, get.head, 2 * j + 1);
+      }
+      next_keys();
+      if (!ok) break;
+      float s[4] = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
+      const int tok0 = (get.r.tile0 + get.tile) * kTile;
+      float s0 = 0.f, s1 = 0.f;
+      given(get.r, 0, tok0, s, cA, cB, eA, eB, s0, s1);
+      give(get.r, tok0, s0, s1);
+      if (done < count) fresh = get.next(a, line, true);
     }
-    if (++at < end) fresh = get.next(a, line, true);
+  } else {
+    uint4* queries = reinterpret_cast<uint4*>(smem + S::queries);      // [block][D / 32 pieces of 16 bytes][lane]
+    float2* rowc = reinterpret_cast<float2*>(smem + S::rows);          // factor and log of the sum of a row
+    while (at < end) {
+      const Request r = get.r;
+      const int head = get.head, seg = (int)min(end - at, (long long)(r.tiles - get.tile)), rows = r.q_len * a.group;
+      const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
+      for (int row0 = 0; row0 < rows; row0 += 8 * S::chunk) {
+        __syncthreads();                                               // the last chunk has been used
+        const int blocks = min(S::chunk, (rows - row0 + 7) / 8);
+        for (int nb = warp; nb < blocks; nb += kWarps) {
+          uint32_t qf[D / 8];
+          const float back = load_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, qf);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) queries[(nb * (D / 32) + i) * 32 + lane] = make_uint4(qf[4 * i], qf[4 * i + 1], qf[4 * i + 2], qf[4 * i + 3]);
+          if (j == 0) rowc[nb * 8 + g] = make_float2(kh * back, lse_of(r, head, row0 + nb * 8 + g));
+        }
+        __syncthreads();
+        uses += count;                                                 // (of the run before: all of its tiles were taken)
+        first = at + warp;
+        count = seg > warp ? (seg - warp + kWarps - 1) / kWarps : 0;
+        fetched = done = 0;
+        if (ok)
+          for (int s = 0; s < min(STAGES, count); ++s) fetch();
+        __syncwarp();
+        while (done < count && ok) {
+          const int tok0 = (r.tile0 + get.tile + warp + done * kWarps) * kTile;
+          next_keys();
+          if (!ok) break;
+          float s0 = 0.f, s1 = 0.f;
+          for (int nb = 0; nb < blocks; ++nb) {
+            float s[4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              const uint4 q = queries[(nb * (D / 32) + i) * 32 + lane];
+              mma(s, k[2 * i][0], k[2 * i][1], k[2 * i][2], k[2 * i][3], q.x, q.y);
+              mma(s, k[2 * i + 1][0], k[2 * i + 1][1], k[2 * i + 1][2], k[2 * i + 1][3], q.z, q.w);
+            }
+            const float4 c = *reinterpret_cast<const float4*>(rowc + nb * 8 + 2 * j);
+            given(r, row0 + nb * 8, tok0, s, c.x, c.z, c.y, c.w, s0, s1);
+          }
+          give(r, tok0, s0, s1);
+        }
+      }
+      at += seg;
+      if (at < end) get.next_unit(a, line, true);
+    }
+  }
+  if (!ok) {     // copies may be in flight: they land before the shared memory goes
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
 }
 
@@ -787,7 +933,7 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
 
 template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows, int sms, cudaStream_t stream) {
   using S = Shape<D, NB>;
-  static bool ready[64] = {};
+  static bool ready[64] = {}, weights_ready[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
@@ -804,7 +950,13 @@ template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows
   else msgl_launch(fp4_join_kernel<T, D, 8>, dim3((unsigned)rows), dim3(256), 0, stream, a, total_rows);
   MSGL_CHECK_LAUNCH("paged_attention_fp4 join");
   if (a.weights != nullptr) {
-    msgl_launch(fp4_weights_kernel<T, D>, dim3(sms * (D == 256 ? 3 : 4)), dim3(kWarps * 32), 0, stream, a);
+    using W = WeightsShape<D, (NB > 1)>;
+    if (dev < 0 || dev >= 64 || !weights_ready[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(fp4_weights_kernel<T, D, (NB > 1)>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::smem);
+      if (e != cudaSuccess) { msgl_set_error("paged_attention_fp4 weights shared memory", e); return MSGL_CUDA_ERROR; }
+      if (dev >= 0 && dev < 64) weights_ready[dev] = true;
+    }
+    msgl_launch(fp4_weights_kernel<T, D, (NB > 1)>, dim3(sms * W::ctas), dim3(kWarps * 32), W::smem, stream, a);
     MSGL_CHECK_LAUNCH("paged_attention_fp4 weights");
   }
   return MSGL_OK;

@@ -16,98 +16,149 @@ struct RowArgs {
   const float* k_head;      // [hk] or null: 1
   const float* v_head;
   float* weights;           // store: attention weights of the slots that are written start at 0, or null
-  int rows, hk, page_size, layers;
+  int rows, hk, per;        // per: tiles of a page
+  uint32_t per_magic;       // 2^32 / per, rounded up: i / per = (i * per_magic) >> 32 while i * per < 2^32
   long long slots;
 };
 
-// A thread has one block of 16 channels of a key or value: 32 bytes in, 8 bytes and a scale out. Bound: DRAM; neighbouring
-// threads read neighbouring blocks of one row.
-template <typename T, int D> __global__ void __launch_bounds__(256) store_fp4_kernel(const RowArgs a) {
-  pdl_enter();
-  constexpr int NB = D / 16;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int b = (int)(id % NB);
-  const long long rest = id / NB;
-  const int h = (int)(rest % a.hk);
-  const long long row = rest / a.hk;
-  if (row >= a.rows) return;
-  const bool val = blockIdx.y != 0;
-  const long long loc = a.loc[row];
-  (void)MSGL_OOB(loc, a.slots);
-  if (loc < 0 || loc >= a.slots) return;
-  const T* src = reinterpret_cast<const T*>(val ? a.v : a.k) + row * (val ? a.ldv : a.ldk) + h * D + b * 16;
-  float x[16];
-  {
-    float lo[8], hi[8];
-    load8(src, lo);
-    load8(src + 8, hi);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { x[i] = lo[i]; x[8 + i] = hi[i]; }
+// A thread has 8 channels of a key or value (a 16-byte access; D / 4 threads for a row and head, the key's first) in U rows that
+// follow each other, so that their loads are under way at once: four where the rows fill the GPU twice all the same, else one.
+// B200, us, store + load of 8192 rows, 8 heads of 128: one row 31.7, four 23.6; 64 rows: 6.2, four 8.9.
+template <int D, int U> struct Place {
+  int h, c, row0;           // c: channels 8 c .. 8 c + 7
+  int code_at, sf_at;       // the channels' part of where they lie in a tile
+  bool val;
+  __device__ __forceinline__ Place(const RowArgs& a) {
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, items = (D / 4) * a.hk;
+    const uint32_t row = id / items, item = id - row * items;
+    row0 = (int)row * U;
+    c = (int)(item % (D / 8));
+    val = item / (D / 8) & 1;
+    h = (int)(item / (D / 4));
+    code_at = val ? v_channel<D>(8 * c) : k_channel<D>(8 * c);
+    sf_at = val ? v_sf_byte<D>(0, c / 2) : k_sf_block<D>(c / 2);
   }
-  const float* heads = val ? a.v_head : a.k_head;
-  uint8_t sf;
-  const uint2 code = quantise16(x, heads != nullptr ? heads[h] : 1.f, sf);
-  const long long page = loc / a.page_size;
-  const int off = (int)(loc - page * a.page_size), t = off % kTile;
-  uint8_t* tile = a.pool + tile_at<D>(page, off, h, a.hk, a.page_size);
-  if (!val) {
-    *reinterpret_cast<uint2*>(tile + k_byte<D>(t, b * 16)) = code;
-    tile[k_sf_byte<D>(t, b)] = sf;
-    if (b == 0 && a.weights != nullptr) a.weights[(page * a.hk + h) * a.page_size + off] = 0.f;
-  } else {
-    if (D == 64) {
-      *reinterpret_cast<uint32_t*>(tile + v_byte<D>(t, b * 16)) = code.x;
-      *reinterpret_cast<uint32_t*>(tile + v_byte<D>(t, b * 16 + 8)) = code.y;
-    } else {
-      *reinterpret_cast<uint2*>(tile + v_byte<D>(t, b * 16)) = code;
+};
+// Tile of a slot, the slot's place in an [pages, hk, page] array, and its token in the tile.
+template <int D> __device__ __forceinline__ uint8_t* tile_of(const RowArgs& a, int loc, int h, int& t, long long& at) {
+  const int tile = loc / kTile, page = a.per == 1 ? tile : (int)__umulhi((uint32_t)tile, a.per_magic);
+  t = loc % kTile;
+  const long long first = ((long long)page * a.hk + h) * a.per + (tile - page * a.per);
+  at = first * kTile + t;
+  return a.pool + first * Tile<D>::bytes;
+}
+
+template <typename T> __device__ __forceinline__ float magnitude(uint32_t bits);
+template <> __device__ __forceinline__ float magnitude<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <> __device__ __forceinline__ float magnitude<__half>(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+
+// 8 channels -> 4 bytes of codes, and the scale of their block, whose other half the neighbouring lane has. The scale is what
+// the largest code (6) needs to stand for the block's largest magnitude, rounded to e4m3 (3 bits of mantissa: what one byte
+// for 16 values leaves); a code is the nearest of x / (scale * head), ties to the even one. A quotient on a tie has to stay
+// there, so quotients are rounded as an IEEE division rounds them: one reciprocal for the block, and for each x the product
+// with it and one correction by its remainder (P. Markstein, IBM J. Res. Dev. 34, 1990). A block that saturates, whose products
+// may overflow, divides. The magnitudes are compared as integers, in pairs: a NaN is then the largest, and it
+// shows in all of its block. All lanes of the warp call it.
+template <typename T> __device__ __forceinline__ uint32_t quantise8(const Vec8<T>& raw, float head, uint8_t& sf) {
+  uint32_t top2 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, reinterpret_cast<const uint32_t*>(&raw)[i] & 0x7FFF7FFFu);
+  top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+  const float top = magnitude<T>(max(top2 & 0xFFFFu, top2 >> 16));
+  sf = top != top ? 0x7F : (uint8_t)float_to_e4m3(top / (6.f * head));
+  const float step = e4m3_to_float(sf) * head;
+  uint32_t w = 0;
+  if (step > 0.f) {
+    const float back = 1.f / step;
+    auto over = [&](float x) {
+      const float q = x * back;
+      return fmaf(fmaf(-q, step, x), back, q);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = to_float2(raw.v[i]);
+      const float2 q = sf < 0x7E ? make_float2(over(x.x), over(x.y)) : make_float2(x.x / step, x.y / step);
+      w |= (uint32_t)__nv_cvt_float2_to_fp4x2(q, __NV_E2M1, cudaRoundNearest) << (8 * i);
     }
-    tile[v_sf_byte<D>(t, b)] = sf;
+  }
+  return w;
+}
+
+// Bound: the 16 bytes in and 4.5 out of a thread and row.
+template <typename T, int D, int U> __global__ void __launch_bounds__(256) store_fp4_kernel(const RowArgs a) {
+  const Place<D, U> p(a);
+  pdl_enter();
+  const T* src = reinterpret_cast<const T*>(p.val ? a.v : a.k) + p.h * D + p.c * 8;
+  const long long ld = p.val ? a.ldv : a.ldk;
+  const float* heads = p.val ? a.v_head : a.k_head;
+  const float head = heads != nullptr && p.row0 < a.rows ? heads[p.h] : 1.f;
+  Vec8<T> raw[U];
+  int loc[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    loc[u] = -1;
+    if (p.row0 + u < a.rows) {
+      loc[u] = a.loc[p.row0 + u];
+      (void)MSGL_OOB(loc[u], a.slots);
+      raw[u] = *reinterpret_cast<const Vec8<T>*>(src + (p.row0 + u) * ld);
+    } else {
+      *reinterpret_cast<uint4*>(&raw[u]) = make_uint4(0, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint8_t sf;
+    const uint32_t code = quantise8<T>(raw[u], head, sf);
+    if (loc[u] < 0 || loc[u] >= a.slots) continue;
+    int t;
+    long long at;
+    uint8_t* tile = tile_of<D>(a, loc[u], p.h, t, at);
+    *reinterpret_cast<uint32_t*>(tile + p.code_at + (p.val ? v_token<D>(t) : k_token<D>(t))) = code;
+    if (!(p.c & 1)) tile[p.sf_at + (p.val ? t : k_sf_token<D>(t))] = sf;
+    if (!p.val && p.c == 0 && a.weights != nullptr) a.weights[at] = 0.f;
   }
 }
 
-// The inverse, a block of 16 channels a thread. A slot outside the pool gives zeros.
-template <typename T, int D> __global__ void __launch_bounds__(256) load_fp4_kernel(const RowArgs a) {
+// The inverse; code * scale is exact, the head's factor is applied in fp32 ahead of it. A slot outside the pool gives zeros.
+// Bound: the 16 bytes that a thread writes for a row. blockIdx.y: layer.
+template <typename T, int D, int U> __global__ void __launch_bounds__(256) load_fp4_kernel(const RowArgs a) {
+  const Place<D, U> p(a);
   pdl_enter();
-  constexpr int NB = D / 16;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int b = (int)(id % NB);
-  const long long rest = id / NB;
-  const int h = (int)(rest % a.hk);
-  const long long out_row = rest / a.hk;
-  if (out_row >= (long long)a.rows * a.layers) return;
-  const long long layer = out_row / a.rows, row = out_row - layer * a.rows;
-  const bool val = blockIdx.y != 0;
-  const long long loc = a.loc[row];
-  (void)MSGL_OOB(loc, a.slots);
-  float lo[8] = {}, hi[8] = {};
-  if (loc >= 0 && loc < a.slots) {
-    const long long page = loc / a.page_size;
-    const int off = (int)(loc - page * a.page_size), t = off % kTile;
-    const uint8_t* tile = a.pool + layer * a.layer_bytes + tile_at<D>(page, off, h, a.hk, a.page_size);
-    uint2 code;
-    float s;
-    if (!val) {
-      code = *reinterpret_cast<const uint2*>(tile + k_byte<D>(t, b * 16));
-      s = e4m3_to_float(tile[k_sf_byte<D>(t, b)]) * (a.k_head != nullptr ? a.k_head[h] : 1.f);
-    } else {
-      if (D == 64) {
-        code.x = *reinterpret_cast<const uint32_t*>(tile + v_byte<D>(t, b * 16));
-        code.y = *reinterpret_cast<const uint32_t*>(tile + v_byte<D>(t, b * 16 + 8));
-      } else {
-        code = *reinterpret_cast<const uint2*>(tile + v_byte<D>(t, b * 16));
-      }
-      s = e4m3_to_float(tile[v_sf_byte<D>(t, b)]) * (a.v_head != nullptr ? a.v_head[h] : 1.f);
-    }
+  if (p.row0 >= a.rows) return;
+  const float* heads = p.val ? a.v_head : a.k_head;
+  const float head = heads != nullptr ? heads[p.h] : 1.f;
+  const long long layer = (long long)blockIdx.y * a.layer_bytes;
+  uint32_t code[U];
+  uint8_t sf[U];
+  int loc[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) loc[u] = a.loc[min(p.row0 + u, a.rows - 1)];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    code[u] = 0;
+    sf[u] = 0;
+    (void)MSGL_OOB(loc[u], a.slots);
+    if (loc[u] < 0 || loc[u] >= a.slots) continue;
+    int t;
+    long long at;
+    const uint8_t* tile = tile_of<D>(a, loc[u], p.h, t, at) + layer;
+    code[u] = *reinterpret_cast<const uint32_t*>(tile + p.code_at + (p.val ? v_token<D>(t) : k_token<D>(t)));
+    sf[u] = tile[p.sf_at + (p.val ? t : k_sf_token<D>(t))];
+  }
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.val ? a.v : a.k)) +
+           (((long long)blockIdx.y * a.rows + p.row0) * a.hk + p.h) * D + p.c * 8;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (p.row0 + u >= a.rows) break;
+    const float s = e4m3_to_float(sf[u]) * head;
+    Vec8<T> y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 p = decode2(code.x >> (8 * i)), q = decode2(code.y >> (8 * i));
-      lo[2 * i] = p.x * s; lo[2 * i + 1] = p.y * s;
-      hi[2 * i] = q.x * s; hi[2 * i + 1] = q.y * s;
+      const float2 x = decode2(code[u] >> (8 * i));
+      y.v[i] = Pack2<T>::make(x.x * s, x.y * s);
     }
+    *reinterpret_cast<Vec8<T>*>(dst + (long long)u * a.hk * D) = y;
   }
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(val ? a.v : a.k)) + (out_row * a.hk + h) * D + b * 16;
-  store8(dst, lo);
-  store8(dst + 8, hi);
 }
 
 // ---- eviction --------------------------------------------------------------------------
@@ -122,6 +173,8 @@ struct EvictArgs {
   int32_t* new_lens;        // [requests]
   const int32_t* lens;
   int width, new_width, requests, hk, page_size, pages, budget, recent, sinks;
+  int per;                  // tiles of a page
+  uint32_t per_magic;       // 2^32 / per, rounded up
 };
 
 __device__ __forceinline__ int page_of(const EvictArgs& a, const int32_t* table, int width, int b, int i) {
@@ -138,18 +191,25 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+constexpr uint32_t kZeroKey = 0x80000000u;
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048, kCopies = 4;
+constexpr int kKeysInShared = 49000;   // beside the bins, in the 227 KB of a CTA
 
-// A CTA for each (layer, request, head): the key of the last weight that stays by a radix search (four digits of 8 bits), then
-// the tokens above it, and of those at it the first ones, in their order.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
+// A CTA for each (layer, request, head): the key of the last weight that stays by a radix search of three digits (11, 11, 10
+// bits), then the tokens above it, and of those at it the first ones, in their order: each warp counts and then writes a share
+// of the tokens. KEPT: the keys stay in shared memory; otherwise (requests that are too long for it) every pass reads them
+// again. The few bins of the first digit that the weights of a request fall into are what lanes wait for: there are four copies of
+// them, and zeros (tokens that nothing has looked at yet) are counted in registers.
+template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a, int longest) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[kCopies][kBins];
+  __shared__ int chunk[kSelWarps], sum_above[kSelWarps], sum_tie[kSelWarps];
+  __shared__ int s_digit, s_rank;
   pdl_enter();
-  __shared__ int hist[256];
-  __shared__ int warp_sum_above[32], warp_sum_tie[32];
-  __shared__ uint32_t s_digit;
-  __shared__ int s_rank;
   const int h = blockIdx.x % a.hk, b = blockIdx.x / a.hk % a.requests, layer = blockIdx.x / a.hk / a.requests;
-  const int n = min(max(a.lens[b], 0), a.width * a.page_size);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = min(max(a.lens[b], 0), KEPT ? longest : a.width * a.page_size);
   int32_t* kept = a.kept + (long long)blockIdx.x * a.budget;
   if (layer == 0 && h == 0 && threadIdx.x == 0) a.new_lens[b] = min(n, a.budget);
   if (n <= a.budget) {
@@ -157,126 +217,215 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     return;
   }
   const int lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;   // candidates [lo, hi): more than need
-  const float* weights = a.weights + layer * a.layer_weights;
-  auto key_of = [&](int i) {
-    const long long page = page_of(a, a.table, a.width, b, i);
-    return weight_key(weights[(page * a.hk + h) * a.page_size + i % a.page_size]);
-  };
-  uint32_t bound = 0, mask = 0;
-  int rank = need;          // of the bound among the keys that share its digits so far, from the largest, from 1
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-        const uint32_t key = key_of(i);
-        if ((key & mask) == bound) atomicAdd(&hist[key >> shift & 255], 1);
-      }
-      __syncthreads();
-      if (threadIdx.x < 32) {
-        // lane l has digits 255 - 8 l and down
-        int sum = 0;
-        for (int q = 0; q < 8; ++q) sum += hist[255 - 8 * threadIdx.x - q];
-        int incl = sum;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, incl, o);
-          if ((int)threadIdx.x >= o) incl += up;
-        }
-        int before = incl - sum;
-        if (before < rank && rank <= incl) {
-          for (int q = 0; q < 8; ++q) {
-            const int c = hist[255 - 8 * threadIdx.x - q];
-            if (rank <= before + c) { s_digit = 255 - 8 * threadIdx.x - q; s_rank = rank - before; break; }
-            before += c;
-          }
-        }
-      }
-      __syncthreads();
-      bound |= s_digit << shift;
-      mask |= 255u << shift;
-      rank = s_rank;
-      __syncthreads();
-    }
-  }
-  // tokens in order: what is above the bound, and the first `rank` at it
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < a.sinks; i += kSelThreads) kept[i] = i;
   for (int i = threadIdx.x; i < a.recent; i += kSelThreads) kept[a.budget - a.recent + i] = hi + i;
-  int above = 0, ties = 0;          // so far
-  for (int i0 = lo; i0 < hi && need > 0; i0 += kSelThreads) {
-    const int i = i0 + threadIdx.x;
-    const uint32_t key = i < hi ? key_of(i) : 0;
-    const bool up = i < hi && key > bound, tie = i < hi && key == bound;
-    const uint32_t up_bits = __ballot_sync(0xffffffffu, up), tie_bits = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) { warp_sum_above[warp] = __popc(up_bits); warp_sum_tie[warp] = __popc(tie_bits); }
-    __syncthreads();
-    int ua = above, ta = ties, uall = 0, tall = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) { ua += warp_sum_above[w]; ta += warp_sum_tie[w]; }
-      uall += warp_sum_above[w];
-      tall += warp_sum_tie[w];
+  if (need == 0) return;
+  const float* weights = a.weights + layer * a.layer_weights;
+  const int32_t* table = a.table + (long long)b * a.width;
+  auto column = [&](int i) { return a.per == 1 ? i >> 4 : (int)__umulhi((uint32_t)i >> 4, a.per_magic); };     // i / page_size
+  auto weight_of = [&](int i, int col, int page) {
+    (void)MSGL_OOB(page, a.pages);
+    page = min(max(page, 0), a.pages - 1);
+    return weight_key(weights[((long long)page * a.hk + h) * a.page_size + i - col * a.page_size]);
+  };
+  auto read = [&](int i) { return weight_of(i, column(i), table[column(i)]); };
+  auto key_of = [&](int i) { return KEPT ? keys[i] : read(i); };
+  for (int i = threadIdx.x; i < kCopies * kBins; i += kSelThreads) hist[0][i] = 0;
+  __syncthreads();
+  uint32_t bound = 0, mask = 0;
+  int rank = need;          // of the bound among the keys that share its digits so far, from the largest, from 1
+#pragma unroll 1
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const uint32_t ones = digit == 2 ? 1023u : 2047u;
+    if (digit == 0) {
+      constexpr int U = 8;  // loads under way at once
+      int zeros = 0;
+      for (int i0 = lo + threadIdx.x; i0 < hi; i0 += U * kSelThreads) {
+        uint32_t key[U];
+        int page[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) page[u] = table[column(min(i0 + u * kSelThreads, hi - 1))];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = min(i0 + u * kSelThreads, hi - 1);
+          key[u] = weight_of(i, column(i), page[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u * kSelThreads >= hi) break;
+          if (KEPT) keys[i0 + u * kSelThreads] = key[u];
+          if (key[u] == kZeroKey) ++zeros;
+          else atomicAdd(&hist[lane % kCopies][key[u] >> 21], 1);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) zeros += __shfl_xor_sync(0xffffffffu, zeros, o);
+      if (lane == 0 && zeros > 0) atomicAdd(&hist[0][kZeroKey >> 21], zeros);
+    } else {
+      for (int i = lo + threadIdx.x; i < hi; i += kSelThreads) {
+        const uint32_t key = key_of(i);
+        if ((key & mask) == bound) atomicAdd(&hist[lane % kCopies][key >> shift & ones], 1);
+      }
     }
-    ua += __popc(up_bits & ((1u << lane) - 1));
-    ta += __popc(tie_bits & ((1u << lane) - 1));
-    if (up || (tie && ta < rank)) kept[lo + ua + min(ta, rank)] = i;
-    above += uall;
-    ties += tall;
     __syncthreads();
+    // the largest digits first: thread t has kBins / kSelThreads of them
+    constexpr int PER = kBins / kSelThreads;
+    int mine[PER], sum = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int bin = kBins - 1 - PER * (int)threadIdx.x - q;
+      mine[q] = 0;
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) { mine[q] += hist[k][bin]; hist[k][bin] = 0; }
+      sum += mine[q];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) chunk[warp] = incl;
+    __syncthreads();
+    int before = incl - sum;
+    for (int w = 0; w < warp; ++w) before += chunk[w];
+    if (before < rank && rank <= before + sum) {
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        if (before < rank && rank <= before + mine[q]) { s_digit = kBins - 1 - PER * (int)threadIdx.x - q; s_rank = rank - before; }
+        before += mine[q];
+      }
+    }
+    __syncthreads();
+    bound |= (uint32_t)s_digit << shift;
+    mask |= ones << shift;
+    rank = s_rank;
+  }
+  // what is above the bound, and the first `rank` at it
+  const int share = ((hi - lo + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int i0 = min(lo + warp * share, hi), i1 = min(i0 + share, hi);
+  int above = 0, ties = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t key = i < i1 ? key_of(i) : 0;
+    above += __popc(__ballot_sync(0xffffffffu, i < i1 && key > bound));
+    ties += __popc(__ballot_sync(0xffffffffu, i < i1 && key == bound));
+  }
+  if (lane == 0) { sum_above[warp] = above; sum_tie[warp] = ties; }
+  __syncthreads();
+  above = ties = 0;
+  for (int w = 0; w < warp; ++w) { above += sum_above[w]; ties += sum_tie[w]; }
+  const uint32_t below = (1u << lane) - 1;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t key = i < i1 ? key_of(i) : 0;
+    const bool up = i < i1 && key > bound, tie = i < i1 && key == bound;
+    const uint32_t up_bits = __ballot_sync(0xffffffffu, up), tie_bits = __ballot_sync(0xffffffffu, tie);
+    const int ua = above + __popc(up_bits & below), ta = ties + __popc(tie_bits & below);
+    if (up || (tie && ta < rank)) kept[lo + ua + min(ta, rank)] = i;
+    above += __popc(up_bits);
+    ties += __popc(tie_bits);
   }
 }
 
-// A warp for each tile of 16 rows that stay: every lane collects its own bytes of the new tile. Slots behind the last row keep
-// what they hold.
+// A warp for each tile of 16 rows that stay: every lane collects its own bytes of the new tile, all loads ahead of the stores.
+// Slots behind the last row keep what they hold. Bound: DRAM sectors of 32 bytes, of which rows that lie far apart use part: a
+// row's 144 bytes (D = 128) lie in 15 sectors.
 template <int D> __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a, int tiles, long long units) {
   pdl_enter();
   const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   if (id >= units) return;
-  const int tile = (int)(id % tiles);
-  const long long unit = id / tiles;
-  const int h = (int)(unit % a.hk), b = (int)(unit / a.hk % a.requests);
+  const int unit = (int)(id / tiles), tile = (int)(id - (long long)unit * tiles);
+  const int h = unit % a.hk, b = unit / a.hk % a.requests;
   const long long layer = unit / a.hk / a.requests;
   const int m = a.new_lens[b];
   const int rows = min(kTile, m - tile * kTile);
   if (rows <= 0) return;
   uint8_t* pool = a.pool + layer * a.layer_bytes;
   float* weights = a.weights + layer * a.layer_weights;
-  // lane t: where row t comes from
-  long long from = 0;
-  int t_src = 0;
+  // lane t: where row t comes from, as (tile of the pool) * 16 + row of the tile; rows that are not there come from row 0's place
   const int to_off = tile * kTile % a.page_size;
   const long long to_page = page_of(a, a.new_table, a.new_width, b, tile * kTile);
-  if (lane < rows) {
-    const int i = a.kept[unit * a.budget + tile * kTile + lane];
+  long long from;
+  {
+    const int i = a.kept[(long long)unit * a.budget + tile * kTile + min(lane, rows - 1)];
     const int off = i % a.page_size;
     const long long page = page_of(a, a.table, a.width, b, i);
-    from = tile_at<D>(page, off, h, a.hk, a.page_size);
-    t_src = off % kTile;
-    weights[(to_page * a.hk + h) * a.page_size + to_off + lane] = weights[(page * a.hk + h) * a.page_size + off];
+    from = ((page * a.hk + h) * (a.page_size / kTile) + off / kTile) * kTile + off % kTile;
+    if (lane < rows) weights[(to_page * a.hk + h) * a.page_size + to_off + lane] = weights[(page * a.hk + h) * a.page_size + off];
   }
   uint8_t* to = pool + tile_at<D>(to_page, to_off, h, a.hk, a.page_size);
-  for (int t = 0; t < rows; ++t) {
-    const uint8_t* src = pool + __shfl_sync(0xffffffffu, from, t);
-    const int ts = __shfl_sync(0xffffffffu, t_src, t);
-    for (int i = lane; i < D / 4; i += 32) {      // 4 bytes a lane
-      const int d = i % (D / 8) * 8;
-      const bool val = i >= D / 8;
-      const int s = val ? v_byte<D>(ts, d) : k_byte<D>(ts, d), e = val ? v_byte<D>(t, d) : k_byte<D>(t, d);
-      *reinterpret_cast<uint32_t*>(to + e) = *reinterpret_cast<const uint32_t*>(src + s);
-    }
-    for (int i = lane; i < D / 8; i += 32) {
-      const int blk = i % (D / 16);
-      const bool val = i >= D / 16;
-      to[val ? v_sf_byte<D>(t, blk) : k_sf_byte<D>(t, blk)] = src[val ? v_sf_byte<D>(ts, blk) : k_sf_byte<D>(ts, blk)];
-    }
+  auto source = [&](int t, int& ts) {
+    const long long f = __shfl_sync(0xffffffffu, from, t);
+    ts = (int)(f % kTile);
+    return pool + f / kTile * Tile<D>::bytes;
+  };
+  // keys: rows g and g + 8 of the operand, D / 8 bytes and D / 64 scales of each
+  constexpr int KW = D / 32, SW = D / 64;
+  uint32_t k[2][KW];
+  uint8_t ks[2][SW];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    int ts;
+    const uint8_t* src = source(4 * (g >> 1) + 2 * r + (g & 1), ts);
+    if (D == 64) *reinterpret_cast<uint2*>(k[r]) = *reinterpret_cast<const uint2*>(src + k_byte<D>(ts, j * (D / 4)));
+    else
+#pragma unroll
+      for (int w = 0; w < KW; w += 4)
+        *reinterpret_cast<uint4*>(k[r] + w) = *reinterpret_cast<const uint4*>(src + k_byte<D>(ts, j * (D / 4) + 8 * w));
+#pragma unroll
+    for (int i = 0; i < SW; ++i) ks[r][i] = src[k_sf_byte<D>(ts, j * SW + i)];
+  }
+  // values: tokens 4 j .. 4 j + 3, D / 16 bytes of each; scales of the lane's blocks (D = 64: lanes of even g)
+  constexpr int VW = D / 64, VB = D == 256 ? 2 : 1;
+  uint32_t v[4][VW];
+  uint8_t vs[4][VB];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    int ts;
+    const uint8_t* src = source(4 * j + e, ts);
+    const uint8_t* p = src + v_byte<D>(ts, g * (D / 8));
+    if (D == 64) v[e][0] = *reinterpret_cast<const uint32_t*>(p);
+    else if (D == 128) *reinterpret_cast<uint2*>(v[e]) = *reinterpret_cast<const uint2*>(p);
+    else *reinterpret_cast<uint4*>(v[e]) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < VB; ++i) vs[e][i] = src[v_sf_byte<D>(ts, D == 64 ? g >> 1 : g * VB + i)];
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int t = 4 * (g >> 1) + 2 * r + (g & 1);
+    if (t >= rows) continue;
+    if (D == 64) *reinterpret_cast<uint2*>(to + k_byte<D>(t, j * (D / 4))) = *reinterpret_cast<uint2*>(k[r]);
+    else
+#pragma unroll
+      for (int w = 0; w < KW; w += 4)
+        *reinterpret_cast<uint4*>(to + k_byte<D>(t, j * (D / 4) + 8 * w)) = *reinterpret_cast<uint4*>(k[r] + w);
+#pragma unroll
+    for (int i = 0; i < SW; ++i) to[k_sf_byte<D>(t, j * SW + i)] = ks[r][i];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int t = 4 * j + e;
+    if (t >= rows) continue;
+    uint8_t* p = to + v_byte<D>(t, g * (D / 8));
+    if (D == 64) *reinterpret_cast<uint32_t*>(p) = v[e][0];
+    else if (D == 128) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v[e]);
+    else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(v[e]);
+    if (D != 64 || !(g & 1))
+#pragma unroll
+      for (int i = 0; i < VB; ++i) to[v_sf_byte<D>(t, D == 64 ? g >> 1 : g * VB + i)] = vs[e][i];
   }
 }
 
-bool shape_ok(int hk, int d, int page_size, const void* pool, const char* what) {
-  if (hk > 0 && (d == 64 || d == 128 || d == 256) && page_size > 0 && page_size % kTile == 0 && (uintptr_t)pool % 16 == 0) return true;
+bool shape_ok(int hk, int d, int page_size, long long pages, const void* pool, const char* what) {
+  // slots are 32-bit numbers; a slot's tile times the tiles of a page stays below 2^32 (see per_magic)
+  if (hk > 0 && pages * page_size <= 0x7fffffffll && pages * page_size / kTile * (page_size / kTile) < (1ll << 32) && (d == 64 || d == 128 || d == 256) && page_size > 0 && page_size % kTile == 0 && (uintptr_t)pool % 16 == 0) return true;
   msgl_set_error_text(what);
   return false;
 }
+
+uint32_t magic(int per) { return (uint32_t)(((1ull << 32) + per - 1) / per); }
+int rows_of_a_thread(long long rows, int hk, int d) { return rows * hk * (d / 4) > 148ll * 2048 * 4 ? 4 : 1; }
 
 }  // namespace
 
@@ -284,19 +433,26 @@ MSGL_API int msgl_store_fp4(const void* k, const void* v, long long ldk, long lo
                             const void* v_head, void* weights, int rows, int hk, int d, int page_size, long long pages, int dtype,
                             cudaStream_t stream) {
   if (rows <= 0) return MSGL_OK;
-  if (!shape_ok(hk, d, page_size, pool, "store_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens"))
+  if (!shape_ok(hk, d, page_size, pages, pool, "store_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens, fewer than 2^31 slots"))
     return MSGL_BAD_ARG;
   if (ldk % 8 || ldv % 8 || (uintptr_t)k % 16 || (uintptr_t)v % 16 || (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
     msgl_set_error_text("store_kv_fp4: 16-bit rows on 16-byte boundaries");
     return MSGL_BAD_ARG;
   }
   RowArgs a{k, v, ldk, ldv, (uint8_t*)pool, 0, (const int32_t*)loc, (const float*)k_head, (const float*)v_head, (float*)weights,
-            rows, hk, page_size, 1, pages * page_size};
-  const long long threads = (long long)rows * hk * (d / 16);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2);
-#define STORE(T, D) msgl_launch(store_fp4_kernel<T, D>, grid, dim3(256), 0, stream, a)
-  if (dtype == MSGL_BF16) { if (d == 64) STORE(__nv_bfloat16, 64); else if (d == 128) STORE(__nv_bfloat16, 128); else STORE(__nv_bfloat16, 256); }
-  else { if (d == 64) STORE(__half, 64); else if (d == 128) STORE(__half, 128); else STORE(__half, 256); }
+            rows, hk, page_size / kTile, magic(page_size / kTile), pages * page_size};
+  const int u = rows_of_a_thread(rows, hk, d);
+  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 4);
+  if (threads > 0x7fffff00ll) {
+    msgl_set_error_text("store_kv_fp4: more rows than a launch has threads for");
+    return MSGL_BAD_ARG;
+  }
+  const dim3 grid((unsigned)((threads + 255) / 256));
+#define STORE(T, D, U) msgl_launch(store_fp4_kernel<T, D, U>, grid, dim3(256), 0, stream, a)
+#define STORES(T, D) do { if (u == 1) STORE(T, D, 1); else STORE(T, D, 4); } while (0)
+  if (dtype == MSGL_BF16) { if (d == 64) STORES(__nv_bfloat16, 64); else if (d == 128) STORES(__nv_bfloat16, 128); else STORES(__nv_bfloat16, 256); }
+  else { if (d == 64) STORES(__half, 64); else if (d == 128) STORES(__half, 128); else STORES(__half, 256); }
+#undef STORES
 #undef STORE
   MSGL_CHECK_LAUNCH("store_kv_fp4");
   return MSGL_OK;
@@ -305,19 +461,26 @@ MSGL_API int msgl_store_fp4(const void* k, const void* v, long long ldk, long lo
 MSGL_API int msgl_load_fp4(const void* pool, long long layer_bytes, int layers, const void* loc, const void* k_head, const void* v_head,
                            void* k, void* v, int rows, int hk, int d, int page_size, long long pages, int dtype, cudaStream_t stream) {
   if (rows <= 0 || layers <= 0) return MSGL_OK;
-  if (!shape_ok(hk, d, page_size, pool, "load_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens"))
+  if (!shape_ok(hk, d, page_size, pages, pool, "load_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens, fewer than 2^31 slots"))
     return MSGL_BAD_ARG;
   if (dtype != MSGL_BF16 && dtype != MSGL_F16) {
     msgl_set_error_text("load_kv_fp4: rows of 16 bits");
     return MSGL_BAD_ARG;
   }
   RowArgs a{k, v, 0, 0, (uint8_t*)const_cast<void*>(pool), layer_bytes, (const int32_t*)loc, (const float*)k_head,
-            (const float*)v_head, nullptr, rows, hk, page_size, layers, pages * page_size};
-  const long long threads = (long long)rows * layers * hk * (d / 16);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2);
-#define LOAD(T, D) msgl_launch(load_fp4_kernel<T, D>, grid, dim3(256), 0, stream, a)
-  if (dtype == MSGL_BF16) { if (d == 64) LOAD(__nv_bfloat16, 64); else if (d == 128) LOAD(__nv_bfloat16, 128); else LOAD(__nv_bfloat16, 256); }
-  else { if (d == 64) LOAD(__half, 64); else if (d == 128) LOAD(__half, 128); else LOAD(__half, 256); }
+            (const float*)v_head, nullptr, rows, hk, page_size / kTile, magic(page_size / kTile), pages * page_size};
+  const int u = rows_of_a_thread((long long)rows * layers, hk, d);
+  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 4);
+  if (threads > 0x7fffff00ll || layers > 65535) {
+    msgl_set_error_text("load_kv_fp4: more rows than a launch has threads for");
+    return MSGL_BAD_ARG;
+  }
+  const dim3 grid((unsigned)((threads + 255) / 256), layers);
+#define LOAD(T, D, U) msgl_launch(load_fp4_kernel<T, D, U>, grid, dim3(256), 0, stream, a)
+#define LOADS(T, D) do { if (u == 1) LOAD(T, D, 1); else LOAD(T, D, 4); } while (0)
+  if (dtype == MSGL_BF16) { if (d == 64) LOADS(__nv_bfloat16, 64); else if (d == 128) LOADS(__nv_bfloat16, 128); else LOADS(__nv_bfloat16, 256); }
+  else { if (d == 64) LOADS(__half, 64); else if (d == 128) LOADS(__half, 128); else LOADS(__half, 256); }
+#undef LOADS
 #undef LOAD
   MSGL_CHECK_LAUNCH("load_kv_fp4");
   return MSGL_OK;
@@ -326,9 +489,9 @@ MSGL_API int msgl_load_fp4(const void* pool, long long layer_bytes, int layers, 
 MSGL_API int msgl_evict_fp4(void* pool, long long layer_bytes, void* weights, long long layer_weights, int layers, const void* table,
                             int width, const void* new_table, int new_width, const void* lens, void* kept, void* new_lens,
                             int requests, int hk, int d, int page_size, int pages, int budget, int recent, int sinks,
-                            cudaStream_t stream) {
+                            int max_kv, cudaStream_t stream) {
   if (requests <= 0 || layers <= 0) return MSGL_OK;
-  if (!shape_ok(hk, d, page_size, pool, "evict_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens"))
+  if (!shape_ok(hk, d, page_size, pages, pool, "evict_kv_fp4: heads of 64, 128 or 256 channels and pages of whole tiles of 16 tokens, fewer than 2^31 slots"))
     return MSGL_BAD_ARG;
   if (budget <= 0 || recent < 0 || sinks < 0 || recent + sinks > budget || width <= 0 ||
       (long long)new_width * page_size < budget) {
@@ -337,9 +500,28 @@ MSGL_API int msgl_evict_fp4(void* pool, long long layer_bytes, void* weights, lo
   }
   EvictArgs a{(uint8_t*)pool, layer_bytes, (float*)weights, layer_weights, (const int32_t*)table, (const int32_t*)new_table,
               (int32_t*)kept, (int32_t*)new_lens, (const int32_t*)lens, width, new_width, requests, hk, page_size, pages, budget,
-              recent, sinks};
-  const long long units = (long long)layers * requests * hk;
-  msgl_launch(evict_select_kernel, dim3((unsigned)units), dim3(kSelThreads), 0, stream, a);
+              recent, sinks, page_size / kTile, 0};
+  a.per_magic = magic(a.per);
+  const long long units = (long long)layers * requests * hk, room = (long long)width * page_size;
+  // i / 16 / per by a multiplication is exact while i / 16 times (per_magic * per - 2^32 < per) stays below 2^32
+  if (room / kTile * a.per >= (1ll << 32) || room > 0x7fffffffll || units > 0x7fffffffll) {
+    msgl_set_error_text("evict_kv_fp4: a block table of fewer tokens");
+    return MSGL_BAD_ARG;
+  }
+  const long long longest = max_kv > 0 && max_kv < room ? max_kv : room;
+  if (longest <= kKeysInShared) {
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInShared * 4);
+      if (e != cudaSuccess) { msgl_set_error("evict_kv_fp4 shared memory", e); return MSGL_CUDA_ERROR; }
+      if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    msgl_launch(evict_select_kernel<true>, dim3((unsigned)units), dim3(kSelThreads), (size_t)longest * 4, stream, a, (int)longest);
+  } else {
+    msgl_launch(evict_select_kernel<false>, dim3((unsigned)units), dim3(kSelThreads), 0, stream, a, 0);
+  }
   MSGL_CHECK_LAUNCH("evict_select");
   const int tiles = (budget + kTile - 1) / kTile;
   const dim3 grid((unsigned)((units * tiles + 7) / 8));

@@ -21,54 +21,35 @@ template <int D> struct Tile {
   static constexpr int bytes = 18 * D, v = 8 * D, k_sf = 16 * D, v_sf = 17 * D;
 };
 
-// Byte of the tile that holds channels d (even) and d + 1 of token t's key / value; the 8 bytes of a block of 16 channels are
-// neighbours, except for values of D = 64: two runs of 4 bytes, 64 bytes apart.
-template <int D> __device__ __forceinline__ int k_byte(int t, int d) {
-  const int g = 2 * (t >> 2) + (t & 1), r = (t >> 1) & 1, j = d / (D / 4);
-  const int at = r * (D / 8) + (d % (D / 4)) / 2;
-  return at / 16 * 512 + (4 * g + j) * 16 + at % 16;
+// The byte of a tile that holds channels d (even) and d + 1 of token t's key or value is a sum of a part for the token and one
+// for the channel. The 8 bytes of a block of 16 channels are neighbours, except for values of D = 64: two runs of 4 bytes, 64
+// bytes apart.
+template <int D> __device__ __forceinline__ int k_token(int t) {
+  return (2 * (t >> 2) + (t & 1)) * 64 + ((t >> 1) & 1) * (D == 64 ? 8 : 4 * D);
 }
-template <int D> __device__ __forceinline__ int v_byte(int t, int d) {
-  const int j = t >> 2, e = t & 3, g = d / (D / 8);
-  const int at = e * (D / 16) + (d % (D / 8)) / 2;
-  return Tile<D>::v + at / 16 * 512 + (4 * g + j) * 16 + at % 16;
+template <int D> __device__ __forceinline__ int k_channel(int d) {
+  const int in_lane = d % (D / 4) / 2;
+  return in_lane / 16 * 512 + d / (D / 4) * 16 + in_lane % 16;
 }
-// scale of block b (16 channels)
-template <int D> __device__ __forceinline__ int k_sf_byte(int t, int b) {
-  const int g = 2 * (t >> 2) + (t & 1), r = (t >> 1) & 1, j = b / (D / 64);
-  return Tile<D>::k_sf + (4 * g + j) * (D / 32) + r * (D / 64) + b % (D / 64);
+template <int D> __device__ __forceinline__ int v_token(int t) {
+  return (t >> 2) * 16 + (D == 64 ? (t & 3) * 4 : D == 128 ? (t >> 1 & 1) * 512 + (t & 1) * 8 : (t & 3) * 512);
 }
-template <int D> __device__ __forceinline__ int v_sf_byte(int t, int b) {
-  return Tile<D>::v_sf + (b * 4 + (t >> 2)) * 4 + (t & 3);
+template <int D> __device__ __forceinline__ int v_channel(int d) { return Tile<D>::v + d / (D / 8) * 64 + d % (D / 8) / 2; }
+template <int D> __device__ __forceinline__ int k_byte(int t, int d) { return k_token<D>(t) + k_channel<D>(d); }
+template <int D> __device__ __forceinline__ int v_byte(int t, int d) { return v_token<D>(t) + v_channel<D>(d); }
+// scale of block b (16 channels), the same way
+template <int D> __device__ __forceinline__ int k_sf_token(int t) {
+  return (2 * (t >> 2) + (t & 1)) * (D / 8) + ((t >> 1) & 1) * (D / 64);
 }
+template <int D> __device__ __forceinline__ int k_sf_block(int b) { return Tile<D>::k_sf + b / (D / 64) * (D / 32) + b % (D / 64); }
+template <int D> __device__ __forceinline__ int k_sf_byte(int t, int b) { return k_sf_token<D>(t) + k_sf_block<D>(b); }
+template <int D> __device__ __forceinline__ int v_sf_byte(int t, int b) { return Tile<D>::v_sf + b * 16 + t; }
 
 // Tile of token slot `loc` (page * page_size + offset) and head h; pages hold page_size / 16 tiles of each head.
 template <int D> __device__ __forceinline__ long long tile_at(long long page, int off, int h, int hk, int page_size) {
   return ((page * hk + h) * (page_size / kTile) + off / kTile) * Tile<D>::bytes;
 }
 
-// 16 channels -> 8 bytes of codes and the scale. The scale is the magnitude that the largest code (6) stands for, rounded to
-// e4m3 (3 bits of mantissa: what one byte for 16 values leaves); a code is the nearest of x / (scale * head), ties to the even
-// one. Divisions are IEEE ones: a quotient that lies on a tie has to stay there.
-__device__ __forceinline__ uint2 quantise16(const float (&x)[16], float head, uint8_t& sf) {
-  float top = 0.f;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    top = fmaxf(top, fabsf(x[i]));
-    nan |= x[i] != x[i];
-  }
-  sf = nan ? 0x7F : (uint8_t)float_to_e4m3(top / (6.f * head));   // a NaN of the block shows in all of it
-  const float step = e4m3_to_float(sf) * head;
-  uint32_t w[2] = {0, 0};
-  if (step > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i / 4] |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(x[2 * i] / step, x[2 * i + 1] / step), __NV_E2M1, cudaRoundNearest)
-                  << (8 * (i % 4));
-  }
-  return make_uint2(w[0], w[1]);
-}
 __device__ __forceinline__ float2 decode2(uint32_t byte) {
   const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(byte & 0xFF), __NV_E2M1);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -13,7 +13,7 @@ from ._lib import c_f, c_i, c_ll, c_p, check, lib
 
 _lib.bind("msgl_store_fp4", c_i, [c_p, c_p, c_ll, c_ll] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
-_lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 8 + [c_p])
+_lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 9 + [c_p])
 _lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 6 + [c_i] * 9 + [c_f, c_i, c_p])
 _lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 7)
 _lib.bind("msgl_gather_fp4", c_i, [c_p, c_p, c_ll, c_i] + [c_p] * 4 + [c_ll] + [c_i] * 6 + [c_p])
@@ -121,7 +121,8 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
     check(lib().msgl_evict_fp4(
         cache.data_ptr(), cache.stride(0) if lead else 0, weights.data_ptr(), weights.stride(0) if lead else 0, layers,
         block_table.data_ptr(), block_table.shape[1], new_table.data_ptr(), new_table.shape[1], seq_lens.data_ptr(),
-        kept.data_ptr(), lens.data_ptr(), b, hk, dim, page, pages, budget, recent, sinks, K._stream()), "evict_kv_fp4")
+        kept.data_ptr(), lens.data_ptr(), b, hk, dim, page, pages, budget, recent, sinks, max_kv,
+        K._stream()), "evict_kv_fp4")
     K._count("evict_kv_fp4", "evict_select_kernel + evict_move_kernel", 2)
     return kept, lens
 

@@ -81,6 +81,30 @@ def test_store_and_load(dim, hk, page, dtype):
     assert torch.equal(first, cache)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16"])
+def test_codes_are_those_of_a_division(dtype):
+    """Every finite magnitude of the type over scales of heads that are no powers of two: the code of x / (scale * head) as fp32
+    divides, which the store's quotients have to round to."""
+    bits = torch.arange(1, 0x7F80 if dtype == torch.bfloat16 else 0x7C00, dtype=torch.int32, device="cuda").to(torch.int16)
+    x = bits.view(dtype)
+    x = torch.cat([x, -x])
+    x = x[(x.abs() < 60000.0) & (x.abs() > 1e-4)]
+    x = x[torch.randperm(x.numel(), generator=torch.Generator("cuda").manual_seed(2), device="cuda")]
+    x = torch.cat([x, x[:(-x.numel()) % 128]]).view(-1, 1, 128)
+    rows = x.shape[0]
+    for head in (0.0137, 0.77, 3.1, 29.0, 33.3):
+        cache = torch.zeros(-(-rows // 16), 1, 1, 18 * 128, dtype=torch.uint8, device="cuda")
+        h = torch.tensor([head], device="cuda")
+        ops.store_kv_fp4(x, x, cache, torch.arange(rows, dtype=torch.int32, device="cuda"), h, h)
+        from minisglang_rdna4_b200.ops import ref_fp4
+
+        code, sf = ref_fp4.quantise(x, h)
+        got = ref_fp4.unpack_tiles(cache)
+        for c, s in ((got[0], got[2]), (got[1], got[3])):
+            assert torch.equal(s.reshape(-1, 8)[:rows], sf.reshape(-1, 8))
+            assert torch.equal(c.reshape(-1, 64)[:rows], code.reshape(-1, 64))
+
+
 def test_store_of_special_rows():
     # (2 alone in its block: 2 / 6 lies between the scales 0.3125 and 0.34375, nearer to the second, 6 times which is held)
     cache = torch.full((1, 1, 1, 18 * 64), 0x55, dtype=torch.uint8, device="cuda")
