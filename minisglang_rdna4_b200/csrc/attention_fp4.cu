@@ -974,6 +974,17 @@ int device_sms() {
   return n;
 }
 
+int* status_word() {
+  static int* word[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && word[dev] != nullptr) return word[dev];
+  int* p = nullptr;
+  cudaGetSymbolAddress((void**)&p, g_fp4_status);
+  if (dev >= 0 && dev < 64) word[dev] = p;
+  return p;
+}
+
 int worker_count(int d, int nb) {
   return device_sms() * ctas_of(d, nb) * kWarps;
 }
@@ -1000,8 +1011,7 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
     return MSGL_BAD_ARG;
   }
   const int nb = row_blocks(d, max_q * (hq / hk)), workers = worker_count(d, nb);
-  int* status = nullptr;
-  cudaGetSymbolAddress((void**)&status, g_fp4_status);
+  int* status = status_word();
   float* ws = (float*)workspace;
   const long long parts = 2ll * workers * nb * 8 * (d + 4);
   for (int b0 = 0; b0 < B; b0 += kMost) {

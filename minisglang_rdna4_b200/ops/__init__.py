@@ -20,6 +20,12 @@ def _cuda():
     return cuda
 
 
+def _fp4():
+    from . import kv_fp4
+
+    return kv_fp4
+
+
 def _ref_fp4():
     from . import ref_fp4
 
@@ -163,35 +169,33 @@ def store_kv_fp4(k, v, cache, out_loc, k_scale=None, v_scale=None, weights=None)
     positive; None: 1). Blocks whose magnitude passes ``2688 scale`` saturate; a NaN makes its block NaN. ``weights [pages, Hk,
     page]`` (fp32): the slots' attention weights start at zero. Slots outside the pool are skipped; of a slot that is named
     twice any of the rows' blocks may stay."""
-    from . import kv_fp4 as F4
-
-    _, pages, hk, page, dim = F4.pool_shape(cache)
+    F4 = _fp4()
+    shape = _, pages, hk, page, dim = F4.pool_shape(cache)
     F4.check_here(cache, k, v, out_loc, k_scale, v_scale, weights)
-    F4.check_ints("out_loc", out_loc, None)
-    F4.check_rows("k", k, out_loc.numel(), hk, dim)
-    F4.check_rows("v", v, out_loc.numel(), hk, dim)
-    if k.dtype != v.dtype:
-        raise TypeError(f"k is {k.dtype} and v is {v.dtype}")
-    F4.check_heads("k_scale", k_scale, hk)
-    F4.check_heads("v_scale", v_scale, hk)
+    F4.check_ints("out_loc", out_loc)
+    F4.check_rows(k, v, out_loc.shape[0], hk, dim)
+    F4.check_heads(k_scale, v_scale, hk)
     if weights is not None:
         F4.check_weights(weights, cache, pages, hk, page)
-    (F4 if cache.is_cuda else _ref_fp4()).store_kv_fp4(k, v, cache, out_loc, k_scale, v_scale, weights)
+    if cache.is_cuda:
+        F4.store_kv_fp4(k, v, cache, out_loc, k_scale, v_scale, weights, shape)
+    else:
+        _ref_fp4().store_kv_fp4(k, v, cache, out_loc, k_scale, v_scale, weights)
 
 
 def load_kv_fp4(cache, slots, k_scale=None, v_scale=None, dtype: torch.dtype = torch.bfloat16):
     """Keys and values ``[T, Hk, D]`` of the token slots ``slots [T]`` (int32) in ``dtype`` (bf16 or fp16, rounded once). With
     layers in front of the pool's shape, ``[layers, T, Hk, D]``. Slots outside the pool give zeros."""
-    from . import kv_fp4 as F4
-
-    hk = F4.pool_shape(cache, True)[2]
+    F4 = _fp4()
+    shape = F4.pool_shape(cache, True)
     F4.check_here(cache, slots, k_scale, v_scale)
-    F4.check_ints("slots", slots, None)
-    F4.check_heads("k_scale", k_scale, hk)
-    F4.check_heads("v_scale", v_scale, hk)
+    F4.check_ints("slots", slots)
+    F4.check_heads(k_scale, v_scale, shape[2])
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"load_kv_fp4 gives bf16 or fp16, not {dtype}")
-    return (F4 if cache.is_cuda else _ref_fp4()).load_kv_fp4(cache, slots, k_scale, v_scale, dtype)
+    if cache.is_cuda:
+        return F4.load_kv_fp4(cache, slots, k_scale, v_scale, dtype, shape)
+    return _ref_fp4().load_kv_fp4(cache, slots, k_scale, v_scale, dtype)
 
 
 def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, k_scale=None, v_scale=None, window: int = 0,
@@ -207,28 +211,28 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, 
     heads of its key head, are added to the token's. (A page that several requests of the step share has them added in any
     order.) ``plan``: ``prefill_plan_fp4``; it may be used by a step without ``weights``. ``workspace``: fp32, for parts of split
     requests; one that is too small is replaced for the call."""
-    from . import kv_fp4 as F4
-
-    _, pages, hk, page, dim = F4.pool_shape(cache)
-    F4.check_here(cache, q, block_table, cu_q, seq_lens, k_scale, v_scale, weights)
+    F4 = _fp4()
+    shape = _, pages, hk, page, dim = F4.pool_shape(cache)
+    F4.check_here(cache, q, block_table, cu_q, seq_lens, k_scale, v_scale, weights, workspace)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"queries of bf16 or fp16, not {q.dtype}")
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % hk or q.shape[1] == 0:
         raise ValueError(f"q is [T, a multiple of {hk}, {dim}], not {tuple(q.shape)}")
-    F4.check_ints("seq_lens", seq_lens, None)
-    F4.check_ints("cu_q", cu_q, seq_lens.numel() + 1)
-    F4.check_ints("block_table", block_table, seq_lens.numel(), None)
-    F4.check_heads("k_scale", k_scale, hk)
-    F4.check_heads("v_scale", v_scale, hk)
-    if window < 0 or max_q < 0 or max_kv < 0:
-        raise ValueError("window, max_q and max_kv are not negative")
+    F4.check_ints("seq_lens", seq_lens)
+    F4.check_ints("cu_q", cu_q, seq_lens.shape[0] + 1)
+    F4.check_ints("block_table", block_table, seq_lens.shape[0], 2)
+    F4.check_heads(k_scale, v_scale, hk)
+    if window < 0 or max_q < 0 or max_kv < 0 or block_table.shape[1] == 0:
+        raise ValueError("window, max_q and max_kv are not negative, and a request has a page in its table")
+    if workspace is not None and (workspace.dtype is not torch.float32 or not workspace.is_contiguous()):
+        raise ValueError("a workspace is contiguous fp32")
     if weights is not None:
         F4.check_weights(weights, cache, pages, hk, page)
         if plan is not None:
             raise ValueError("a step that adds to attention weights takes no prefill plan")
     if cache.is_cuda:
-        return F4.paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, max_kv, weights,
-                                      plan, workspace)
+        return F4.paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, weights, plan,
+                                      workspace, shape)
     return _ref_fp4().paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, weights)
 
 
@@ -236,8 +240,7 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window: int = 0):
     """Tables of a prompt step for ``paged_attention_fp4``, for all layers of the step; ``cu_q`` and ``seq_lens`` are the lengths
     on the host (numpy). ``None`` where the step does not take the form for prompts (CPU, few rows for the keys in sight,
     shapes that it does not have)."""
-    from . import kv_fp4 as F4
-
+    F4 = _fp4()
     F4.pool_shape(cache)
     return F4.prefill_plan_fp4(q, cache, cu_q, seq_lens, window) if cache.is_cuda else None
 
@@ -254,14 +257,13 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
 
     Returns ``(kept [(layers,) B, Hk, budget] int32: token indices in order, -1 behind them, new lengths [B] int32)``. Later steps
     go on behind the new lengths, at the positions that their tokens have in the text."""
-    from . import kv_fp4 as F4
-
-    _, pages, hk, page, _ = F4.pool_shape(cache, True)
+    F4 = _fp4()
+    shape = _, pages, hk, page, _ = F4.pool_shape(cache, True)
     F4.check_here(cache, weights, block_table, seq_lens, new_table)
     F4.check_weights(weights, cache, pages, hk, page)
-    F4.check_ints("seq_lens", seq_lens, None)
-    F4.check_ints("block_table", block_table, seq_lens.numel(), None)
-    F4.check_ints("new_table", new_table, seq_lens.numel(), None)
+    F4.check_ints("seq_lens", seq_lens)
+    F4.check_ints("block_table", block_table, seq_lens.shape[0], 2)
+    F4.check_ints("new_table", new_table, seq_lens.shape[0], 2)
     if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError(f"a budget of {budget} with {sinks} first and {recent} last tokens")
     if new_table.shape[1] * page < budget or block_table.shape[1] < 1:
@@ -269,7 +271,7 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     if max_kv < 0:
         raise ValueError("max_kv is not negative")
     if cache.is_cuda:
-        return F4.evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv)
+        return F4.evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv, shape)
     return _ref_fp4().evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks)
 
 

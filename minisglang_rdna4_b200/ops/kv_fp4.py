@@ -2,7 +2,7 @@
 ``csrc/attention_fp4.cu``. The checks hold on the CPU path too (``ops.ref_fp4``)."""
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import numpy as np
 import torch
@@ -29,93 +29,113 @@ def tile_bytes(dim: int) -> int:
     return 18 * dim
 
 
+_SHAPES: Dict[torch.Size, Tuple[int, int, int, int, int]] = {}
+
+
+def _shape_of(shape: torch.Size) -> Tuple[int, int, int, int, int]:
+    if len(shape) not in (4, 5):
+        raise ValueError("a 4-bit K/V pool is uint8 [pages, heads, page / 16, 18 D] (layers in front where they are taken)")
+    pages, hk, tiles, width = shape[-4:]
+    dim = width // 18
+    if dim not in WIDTHS or width % 18 or tiles < 1 or hk < 1 or pages < 1:
+        raise ValueError(f"a 4-bit K/V pool has heads of 64, 128 or 256 channels (tiles of 18 D bytes), not {tuple(shape)}")
+    if len(_SHAPES) > 256:
+        _SHAPES.clear()
+    _SHAPES[shape] = hit = (shape[0] if len(shape) == 5 else 1, pages, hk, tiles * TILE, dim)
+    return hit
+
+
 def pool_shape(cache: torch.Tensor, layered: bool = False) -> Tuple[int, int, int, int, int]:
     """``(layers, pages, heads, page size, D)`` of ``[pages, heads, page / 16, 18 D]`` bytes (``layered``: with or without
     layers in front)."""
-    if cache.dtype != torch.uint8 or cache.dim() not in ((4, 5) if layered else (4,)):
+    shape = cache.shape
+    hit = _SHAPES.get(shape) or _shape_of(shape)
+    if cache.dtype is not torch.uint8 or (len(shape) == 5 and not layered):
         raise ValueError("a 4-bit K/V pool is uint8 [pages, heads, page / 16, 18 D]" + (", layers in front" if layered else ""))
-    layers = cache.shape[0] if cache.dim() == 5 else 1
-    pages, hk, tiles, width = cache.shape[-4:]
-    dim = width // 18
-    if dim not in WIDTHS or width % 18 or tiles < 1 or hk < 1 or pages < 1:
-        raise ValueError(f"a 4-bit K/V pool has heads of 64, 128 or 256 channels (tiles of 18 D bytes), not tiles of {width} bytes")
-    one = cache[0] if cache.dim() == 5 else cache
-    if not one.is_contiguous() or (cache.dim() == 5 and cache.stride(0) % 16) or cache.data_ptr() % 16:
-        raise ValueError("the layers of a 4-bit K/V pool are contiguous, on 16-byte boundaries")
-    return layers, pages, hk, tiles * TILE, dim
+    if cache.data_ptr() % 16 or not cache.is_contiguous():
+        if cache.data_ptr() % 16 or len(shape) == 4 or cache.stride(0) % 16 or not cache[0].is_contiguous():
+            raise ValueError("the layers of a 4-bit K/V pool are contiguous, on 16-byte boundaries")
+    return hit
 
 
-def check_here(*tensors: Optional[torch.Tensor]) -> None:
+def check_here(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """All on one device, on a GPU the current one: the kernels go to its current stream."""
-    first = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != first:
-            raise ValueError(f"tensors on {first} and {t.device}")
-    if first.type == "cuda" and first.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors on {first}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+    here = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    if here >= 0 and here != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on {first.device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
-def check_ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> None:
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(s is not None and s != x for s, x in zip(shape, t.shape)):
-        raise ValueError(f"{name} is int32 of shape {tuple('any' if s is None else s for s in shape)}, not {t.dtype} {tuple(t.shape)}")
+def check_ints(name: str, t: torch.Tensor, rows: Optional[int] = None, dims: int = 1) -> None:
+    if t.dtype is not torch.int32 or t.dim() != dims or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} is int32 with {dims} dimension(s) and {'any number of' if rows is None else rows} rows, not {t.dtype} "
+                         f"{tuple(t.shape)}")
 
 
-def check_heads(name: str, t: Optional[torch.Tensor], hk: int) -> None:
-    if t is not None and (t.dtype != torch.float32 or t.shape != (hk,) or not t.is_contiguous()):
-        raise ValueError(f"{name} is fp32 [{hk}], one factor per key / value head")
+def check_heads(k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor], hk: int) -> None:
+    for t in (k_scale, v_scale):
+        if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != hk or not t.is_contiguous()):
+            raise ValueError(f"k_scale and v_scale are fp32 [{hk}], one factor per key / value head")
 
 
 def check_weights(weights: torch.Tensor, cache: torch.Tensor, pages: int, hk: int, page: int) -> None:
     want = (cache.shape[0],) * (cache.dim() == 5) + (pages, hk, page)
-    one = weights[0] if weights.dim() == 4 else weights
-    if weights.dtype != torch.float32 or tuple(weights.shape) != want or not one.is_contiguous():
+    if (weights.dtype is not torch.float32 or weights.shape != want
+            or not (weights.is_contiguous() or (weights.dim() == 4 and weights[0].is_contiguous()))):
         raise ValueError(f"attention weights are contiguous fp32 {want}, not {weights.dtype} {tuple(weights.shape)}")
 
 
-def check_rows(name: str, x: torch.Tensor, rows: int, hk: int, dim: int) -> None:
-    if x.dtype not in _ROWS:
-        raise TypeError(f"{name}: rows of bf16 or fp16, not {x.dtype}")
-    if x.dim() not in (2, 3) or x.shape[0] != rows or x.numel() != rows * hk * dim:
-        raise ValueError(f"{name} is [{rows}, {hk}, {dim}], not {tuple(x.shape)}")
+def check_rows(k: torch.Tensor, v: torch.Tensor, rows: int, hk: int, dim: int) -> None:
+    if k.dtype is not v.dtype or k.dtype not in _ROWS:
+        raise TypeError(f"rows of bf16 or fp16, keys and values alike, not {k.dtype} and {v.dtype}")
+    for x in (k, v):
+        shape = x.shape
+        if len(shape) not in (2, 3) or shape[0] != rows or (shape[1] != hk * dim if len(shape) == 2 else shape[1:] != (hk, dim)):
+            raise ValueError(f"keys and values are [{rows}, {hk}, {dim}], not {tuple(shape)}")
 
 
-def _row_view(x: torch.Tensor, hk: int, dim: int) -> torch.Tensor:
-    """``[rows, hk * dim]`` whose rows the kernel reads where they lie if they may (16-byte steps), else a copy."""
-    if x.dim() == 3:
-        x = x.flatten(1) if x.stride(1) != dim or x.stride(2) != 1 else x.as_strided((x.shape[0], hk * dim), (x.stride(0), 1))
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
-    return x.clone() if x.data_ptr() % 16 else x
+def _rows(x: torch.Tensor, hk: int, dim: int) -> Tuple[torch.Tensor, int]:
+    """The rows as the kernel can read them and how far they lie apart: where they are if they start on 16 bytes, else a
+    copy."""
+    ld, inner = x.stride(0), x.stride()[1:]
+    if (inner == (dim, 1) or inner == (1,)) and ld % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, ld
+    x = x.reshape(x.shape[0], hk * dim)
+    return (x.clone() if x.is_contiguous() else x.contiguous()), hk * dim
 
 
-def store_kv_fp4(k, v, cache, out_loc, k_scale=None, v_scale=None, weights=None):
-    _, pages, hk, page, dim = pool_shape(cache)
-    t = out_loc.numel()
-    k, v = _row_view(k, hk, dim), _row_view(v, hk, dim)
-    out_loc = out_loc.contiguous()
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def store_kv_fp4(k, v, cache, out_loc, k_scale, v_scale, weights, shape):
+    _, pages, hk, page, dim = shape
+    (k, ldk), (v, ldv), out_loc = _rows(k, hk, dim), _rows(v, hk, dim), _packed(out_loc)
     check(lib().msgl_store_fp4(
-        k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), cache.data_ptr(), out_loc.data_ptr(), K._p(k_scale), K._p(v_scale),
-        K._p(weights), t, hk, dim, page, pages, K._dt(k), K._stream()), "store_kv_fp4")
+        k.data_ptr(), v.data_ptr(), ldk, ldv, cache.data_ptr(), out_loc.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights),
+        out_loc.shape[0], hk, dim, page, pages, K._dt(k), K._stream()), "store_kv_fp4")
     K._count("store_kv_fp4", "store_fp4_kernel")
 
 
-def load_kv_fp4(cache, slots, k_scale, v_scale, dtype):
-    layers, pages, hk, page, dim = pool_shape(cache, True)
-    slots = slots.contiguous()
-    lead = (layers,) if cache.dim() == 5 else ()
-    k, v = (torch.empty(*lead, slots.numel(), hk, dim, dtype=dtype, device=cache.device) for _ in (0, 1))
-    check(lib().msgl_load_fp4(cache.data_ptr(), cache.stride(0) if lead else 0, layers, slots.data_ptr(), K._p(k_scale),
-                              K._p(v_scale), k.data_ptr(), v.data_ptr(), slots.numel(), hk, dim, page, pages, K._dt(k),
-                              K._stream()), "load_kv_fp4")
+def load_kv_fp4(cache, slots, k_scale, v_scale, dtype, shape):
+    layers, pages, hk, page, dim = shape
+    slots, n, layered = _packed(slots), slots.shape[0], cache.dim() == 5
+    both = torch.empty((2, layers, n, hk, dim) if layered else (2, n, hk, dim), dtype=dtype, device=cache.device)
+    k, v = both.unbind(0)
+    check(lib().msgl_load_fp4(cache.data_ptr(), cache.stride(0) if layered else 0, layers, slots.data_ptr(), K._p(k_scale),
+                              K._p(v_scale), k.data_ptr(), v.data_ptr(), n, hk, dim, page, pages, K._DT[dtype], K._stream()),
+          "load_kv_fp4")
     K._count("load_kv_fp4", "load_fp4_kernel")
     return k, v
 
 
-def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv):
-    layers, pages, hk, page, dim = pool_shape(cache, True)
+def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recent, sinks, max_kv, shape):
+    layers, pages, hk, page, dim = shape
     lead = (layers,) if cache.dim() == 5 else ()
     b = seq_lens.numel()
-    block_table, seq_lens, new_table = block_table.contiguous(), seq_lens.contiguous(), new_table.contiguous()
+    block_table, seq_lens, new_table = _packed(block_table), _packed(seq_lens), _packed(new_table)
     kept = torch.empty(*lead, b, hk, budget, dtype=torch.int32, device=cache.device)
     lens = torch.empty(b, dtype=torch.int32, device=cache.device)
     check(lib().msgl_evict_fp4(
@@ -127,21 +147,38 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
     return kept, lens
 
 
-def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, max_kv, weights, plan,
-                        workspace):
-    _, pages, hk, page, dim = pool_shape(cache)
+_NEED: Dict[Tuple, int] = {}
+
+
+def attention_fp4_workspace(rows: int, batch: int, heads: int, kv_heads: int, dim: int, max_q: int, weighed: bool) -> int:
+    """fp32 words that a call of ``paged_attention_fp4`` takes; no call of fewer rows, requests or ``max_q`` takes more, but
+    for the steps of ``max_q`` at which row tiles widen."""
+    key = (rows if weighed else 0, batch, heads, kv_heads, dim, max_q, weighed)
+    hit = _NEED.get(key)
+    if hit is None:
+        if len(_NEED) > 4096:
+            _NEED.clear()
+        _NEED[key] = hit = int(lib().msgl_attention_fp4_workspace(rows, batch, heads, kv_heads, dim, max_q, int(weighed)))
+    return hit
+
+
+def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v_scale, window, max_q, weights, plan, workspace, shape):
+    _, pages, hk, page, dim = shape
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     if block_table.stride(1) != 1:
         block_table = block_table.contiguous()
     if plan is not None:
-        return _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window)
-    cu_q, seq_lens = cu_q.contiguous(), seq_lens.contiguous()
-    t, b, hq = q.shape[0], seq_lens.numel(), q.shape[1]
+        return _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window, shape)
+    cu_q, seq_lens = _packed(cu_q), _packed(seq_lens)
+    t, hq, _ = q.shape
+    b = seq_lens.shape[0]
     if max_q == 0 and t and b:
         max_q = int((cu_q[1:] - cu_q[:-1]).max())
-    need = int(lib().msgl_attention_fp4_workspace(t, b, hq, hk, dim, max_q, weights is not None))
+    if max_q == 0:
+        return out
+    need = attention_fp4_workspace(t, b, hq, hk, dim, max_q, weights is not None)
     if workspace is None or workspace.numel() < need or workspace.data_ptr() % 16:
         workspace = torch.empty(need, dtype=torch.float32, device=q.device)
     check(lib().msgl_attention_fp4(
@@ -183,8 +220,8 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
     return plan
 
 
-def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window):
-    _, pages, hk, page, dim = pool_shape(cache)
+def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window, shape):
+    _, pages, hk, page, dim = shape
     if not isinstance(plan, PromptPlan) or (plan.window, plan.group, plan.dim) != (window, q.shape[1] // hk, dim):
         raise ValueError("the prefill plan was made for another window or other heads")
     if scale <= 0:
