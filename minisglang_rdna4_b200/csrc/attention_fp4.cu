@@ -1,9 +1,10 @@
 // Causal attention over the paged K/V pool of 4 bits (kv_fp4.cuh).
 //
 // A unit is a tile of rows of one request and key head, a row being a (query position, head of the group) pair, with all 16-token
-// tiles that its request's rows see. The tiles of all units in a line are dealt evenly to the warps of the GPU; a warp
-// fetches its tiles into a ring of its own (bulk copies of 18 D bytes) and keeps the softmax of the unit it is in. Units that a
-// warp has whole are written at once, parts of others go to the workspace and a second kernel joins them.
+// tiles that its request's rows see. The tiles of all units in a line are dealt evenly to the CTAs of the GPU, and a CTA's tiles
+// two by two to its warps, each of which fetches its own into a ring (bulk copies of 18 D bytes) and keeps the softmax of the
+// unit it is in. Where a unit ends the warps' sums are joined in shared memory. Units that a CTA has whole are written at
+// once; of the others the parts go to the workspace, and the CTA that brings the last one joins them, in the order of the line.
 //
 // Both products take the cache as their first operand (rows: 16 tokens, or 16 channels), so a row tile is 8 queries wide and
 // no product is spent on more rows than a group of 8 heads has: S^T = K Q^T, O^T = V^T P^T. Codes go e2m1 -> f16 (one
@@ -22,8 +23,8 @@ using namespace msgl::ptx;
 namespace {
 
 constexpr int kWarps = 4;            // of a CTA
-constexpr int kMost = 1024;          // requests of a launch
-constexpr int kFewTiles = 4;         // a warp gets at least so many tiles
+constexpr int kMost = 256;           // requests of a launch
+constexpr int kFewTiles = 8;         // a CTA gets at least so many tiles: a pair for each warp
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUp = 7.f, kSlack = 8.f;   // log2 of the probabilities' factor; by how much a score may pass the maximum
 
@@ -41,9 +42,9 @@ struct Fp4Args {
   const float* v_head;
   float* lse;               // [rows, hq], log2; null without weights
   float* weights;
-  float* parts;             // [2 * workers][rows of a tile][D + 2]
-  long long* line;          // [B + 2]: first tile of every request in the line, total; workers
-  int width, B, hq, hk, group, page_size, per, pages, window, row_tile, workers;   // per: tiles of a page
+  float* parts;             // [2 * workers][blocks of 8 rows][D / 16 + 1 times 16 bytes of a lane][32 lanes]
+  int* arrived;             // [workers]: parts of the unit that begins in a worker's share and goes on; zeros between calls
+  int width, B, hq, hk, group, page_size, per, pages, window, row_tile, row_shift, workers;   // per: tiles of a page; row_tile: 2^row_shift
   float scale;
   int* status;
 };
@@ -56,6 +57,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -90,32 +108,51 @@ struct Request {
   int q0, q_len, n;         // first row, rows, tokens
   int tile0, tiles;         // tiles that its rows see
   int row_tiles;
-  __device__ __forceinline__ void load(const Fp4Args& a, int b) {
-    q0 = a.cu_q[b];
-    q_len = a.cu_q[b + 1] - q0;
-    n = min(max(a.lens[b], 0), a.width * a.page_size);
-    const int lo = a.window > 0 ? max(0, n - q_len - a.window + 1) : 0;
-    tile0 = lo / kTile;
-    tiles = q_len > 0 && n > lo ? (n + kTile - 1) / kTile - tile0 : 0;
-    row_tiles = (max(q_len, 0) * a.group + a.row_tile - 1) / a.row_tile;
+  __device__ __forceinline__ void rows_to(const Fp4Args& a, int row, int row_end) {
+    q0 = row;
+    q_len = row_end - row;
+    row_tiles = (max(q_len, 0) * a.group + a.row_tile - 1) >> a.row_shift;
   }
-  __device__ __forceinline__ long long cost(const Fp4Args& a, bool whole_rows) const {
-    return (long long)tiles * a.hk * (whole_rows ? 1 : row_tiles);
+};
+// In shared memory: first tile of every request, the total behind them; first rows, lengths, tiles in sight.
+struct Line {
+  long long first[kMost + 1];
+  int row[kMost + 1], n[kMost], tile0[kMost], tiles[kMost];
+  __device__ __forceinline__ Request request(const Fp4Args& a, int b) const {
+    Request r;
+    r.rows_to(a, row[b], row[b + 1]);
+    r.n = n[b];
+    r.tile0 = tile0[b];
+    r.tiles = tiles[b];
+    return r;
   }
 };
 
-// First tile of every request in `line` (kMost + 1 entries), the total in line[B].
-__device__ __forceinline__ void lay_line(const Fp4Args& a, long long* line, bool whole_rows) {
+__device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whole_rows) {
   __shared__ long long sums[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32);
-  const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    Request r;
-    r.load(a, b);
-    line[b] = mine;
-    mine += r.cost(a, whole_rows);
+  constexpr int PER = kMost / (kWarps * 32);
+  long long cost[PER], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = (int)threadIdx.x * PER + i;
+    cost[i] = 0;
+    if (b < a.B) {
+      const int row = a.cu_q[b], row_end = a.cu_q[b + 1], len = a.lens[b];
+      Request r;
+      r.rows_to(a, row, row_end);
+      r.n = min(max(len, 0), a.width * a.page_size);
+      const int lo = a.window > 0 ? max(0, r.n - r.q_len - a.window + 1) : 0;
+      r.tile0 = lo / kTile;
+      r.tiles = r.q_len > 0 && r.n > lo ? (r.n + kTile - 1) / kTile - r.tile0 : 0;
+      line.row[b] = row;
+      line.n[b] = r.n;
+      line.tile0[b] = r.tile0;
+      line.tiles[b] = r.tiles;
+      if (b == a.B - 1) line.row[a.B] = row_end;
+      cost[i] = (long long)r.tiles * a.hk * (whole_rows ? 1 : r.row_tiles);
+    }
+    mine += cost[i];
   }
   long long incl = mine;
 #pragma unroll
@@ -126,25 +163,37 @@ __device__ __forceinline__ void lay_line(const Fp4Args& a, long long* line, bool
   if (lane == 31) sums[warp] = incl;
   __syncthreads();
   long long before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += sums[w];
-  for (int b = b0; b < b1; ++b) line[b] += before;
-  if (threadIdx.x == kWarps * 32 - 1) line[a.B] = before + mine;
+#pragma unroll
+  for (int w = 0; w < kWarps - 1; ++w) before += w < warp ? sums[w] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = (int)threadIdx.x * PER + i;
+    if (b < a.B) line.first[b] = before;
+    before += cost[i];
+    if (b == a.B - 1) line.first[a.B] = before;
+  }
   __syncthreads();
 }
 
-// Worker w of W has tiles [begin(w), begin(w + 1)).
+// Divisions of 64 bits are calls; most lines are shorter than 2^32 tiles.
+__device__ __forceinline__ long long quotient(long long x, int y) {
+  return (x >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
+// Worker w of W has tiles [begin(w), begin(w + 1)): `base`, and one more for the first `extra`.
 struct Deal {
   long long base;
   int workers, extra;
-  __device__ __forceinline__ Deal(long long total, int most) {
-    workers = (int)max(1ll, min((long long)most, total / kFewTiles));
-    base = total / workers;
+  __device__ __forceinline__ Deal(long long total, int most, int few) {
+    workers = (int)max(1ll, min((long long)most, quotient(total, few)));
+    base = quotient(total, workers);
     extra = (int)(total - base * workers);
   }
   __device__ __forceinline__ long long begin(int w) const { return w * base + min(w, extra); }
   __device__ __forceinline__ int owner(long long at) const {
     const long long big = (base + 1) * extra;
-    return (int)(at < big ? at / (base + 1) : extra + (at - big) / max(base, 1ll));
+    if ((base >> 31) == 0) return (int)(at < big ? quotient(at, (int)base + 1) : extra + quotient(at - big, max((int)base, 1)));
+    return (int)(at < big ? at / (base + 1) : extra + (at - big) / base);
   }
 };
 
@@ -153,40 +202,51 @@ struct Deal {
 struct Walk {
   int b, head, rt, tile, col, sub;
   Request r;
+  __device__ __forceinline__ void place(const Fp4Args& a) {
+    col = r.tile0 + tile;
+    sub = 0;
+    if (a.per > 1) {
+      const int t = col;
+      col = t / a.per;
+      sub = t - col * a.per;
+    }
+  }
   __device__ __forceinline__ void start_unit(const Fp4Args& a) {
     tile = 0;
-    col = r.tile0 / a.per;
-    sub = r.tile0 - col * a.per;
+    place(a);
   }
-  __device__ __forceinline__ void seek(const Fp4Args& a, const long long* line, long long at, bool whole_rows) {
+  __device__ __forceinline__ void seek(const Fp4Args& a, const Line& line, long long at, bool whole_rows) {
     int lo = 0, hi = a.B - 1;                   // the last request that starts at or before `at` has it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (line[mid] <= at) lo = mid; else hi = mid - 1;
+      if (line.first[mid] <= at) lo = mid; else hi = mid - 1;
     }
     b = lo;
-    r.load(a, b);
-    const long long o = at - line[b];
-    const int unit = (int)(o / max(r.tiles, 1)), row_tiles = whole_rows ? 1 : max(r.row_tiles, 1);
-    tile = (int)(o - (long long)unit * r.tiles);
-    head = unit / row_tiles;
-    rt = unit - head * row_tiles;
-    col = (r.tile0 + tile) / a.per;
-    sub = r.tile0 + tile - col * a.per;
+    r = line.request(a, b);
+    const long long o = at - line.first[b];
+    head = (int)quotient(o, max(r.tiles, 1));
+    tile = (int)(o - (long long)head * r.tiles);
+    rt = 0;
+    if (!whole_rows && r.row_tiles > 1) {
+      const int unit = head;
+      head = unit / r.row_tiles;
+      rt = unit - head * r.row_tiles;
+    }
+    place(a);
   }
   // on to the next unit that has tiles
-  __device__ __forceinline__ void next_unit(const Fp4Args& a, const long long* line, bool whole_rows) {
+  __device__ __forceinline__ void next_unit(const Fp4Args& a, const Line& line, bool whole_rows) {
     if (!whole_rows && ++rt < r.row_tiles) { start_unit(a); return; }
     rt = 0;
     if (++head == a.hk) {
       head = 0;
-      do ++b; while (b < a.B - 1 && line[b] == line[b + 1]);
-      r.load(a, min(b, a.B - 1));
+      do ++b; while (b < a.B - 1 && line.first[b] == line.first[b + 1]);
+      r = line.request(a, min(b, a.B - 1));
     }
     start_unit(a);
   }
   // true where another unit begins
-  __device__ __forceinline__ bool next(const Fp4Args& a, const long long* line, bool whole_rows) {
+  __device__ __forceinline__ bool next(const Fp4Args& a, const Line& line, bool whole_rows) {
     if (++sub == a.per) { sub = 0; ++col; }
     if (++tile < r.tiles) return false;
     next_unit(a, line, whole_rows);
@@ -203,22 +263,26 @@ struct Walk {
 };
 
 // ---- queries ---------------------------------------------------------------------------
-// Lane 4 g + j takes channels j D / 4 .. of row g as the second operand of S^T, scaled by a power of two; returns what the
-// row's scores have to be multiplied by.
+// Lane 4 g + j has channels j D / 4 .. of row g.
 template <typename T, int D>
-__device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, int head, int row, int lane, uint32_t (&qf)[D / 8]) {
+__device__ __forceinline__ void fetch_query(const Fp4Args& a, const Request& r, int head, int row, int lane, Vec8<T> (&raw)[D / 32]) {
   const bool there = row < r.q_len * a.group;
   const int pos = there ? row / a.group : 0;
   const T* src = reinterpret_cast<const T*>(a.q) + ((long long)(r.q0 + pos) * a.hq + head * a.group + (there ? row - pos * a.group : 0)) * D
                  + (lane & 3) * (D / 4);
-  float top = 0.f;
-  Vec8<T> raw[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
+    *reinterpret_cast<uint4*>(&raw[i]) = make_uint4(0, 0, 0, 0);
     if (there) raw[i] = *reinterpret_cast<const Vec8<T>*>(src + 8 * i);
-    else
+  }
+}
+// ... as the second operand of S^T, scaled by a power of two (a negative scale of the scores is the query's sign). Returns
+// what the row's scores have to be multiplied by.
+template <typename T, int D>
+__device__ __forceinline__ float scale_query(const Fp4Args& a, const Vec8<T> (&raw)[D / 32], uint32_t (&qf)[D / 8]) {
+  float top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) raw[i].v[e] = Pack2<T>::make(0.f, 0.f);
+  for (int i = 0; i < D / 32; ++i) {
     float x[8];
     unpack8(raw[i], x);
 #pragma unroll
@@ -228,7 +292,7 @@ __device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, 
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int ex = (int)(__float_as_uint(top) >> 23);            // 0: zeros; 255: infinite
   const int up = top > 0.f && ex < 255 ? min(max(137 - ex, -126), 126) : 0;
-  const float f = copysignf(__uint_as_float((uint32_t)(127 + up) << 23), a.scale);     // a negative scale: on the query
+  const float f = copysignf(__uint_as_float((uint32_t)(127 + up) << 23), a.scale);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     float x[8];
@@ -237,6 +301,12 @@ __device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, 
     for (int e = 0; e < 4; ++e) qf[4 * i + e] = f16x2(x[2 * e] * f, x[2 * e + 1] * f);
   }
   return __uint_as_float((uint32_t)(127 - up) << 23);
+}
+template <typename T, int D>
+__device__ __forceinline__ float load_query(const Fp4Args& a, const Request& r, int head, int row, int lane, uint32_t (&qf)[D / 8]) {
+  Vec8<T> raw[D / 32];
+  fetch_query<T, D>(a, r, head, row, lane, raw);
+  return scale_query<T, D>(a, raw, qf);
 }
 
 template <int D> struct Raw {          // a lane's share of a tile
@@ -279,8 +349,6 @@ template <int D> __device__ __forceinline__ uint32_t key_scale(const Raw<D>& x, 
 // S^T of the tile for NB blocks of 8 rows
 template <int D, int NB> __device__ __forceinline__ void scores(const Raw<D>& x, const uint32_t (&qf)[NB][D / 8], float (&s)[NB][4]) {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-#pragma unroll
   for (int i = 0; i < D / 64; ++i) {                                // blocks of 16 channels: 2 words, 4 products
     const uint32_t s0 = key_scale<D>(x, 0, i), s1 = key_scale<D>(x, 1, i);
 #pragma unroll
@@ -292,31 +360,39 @@ template <int D, int NB> __device__ __forceinline__ void scores(const Raw<D>& x,
       for (int c = 0; c < 2; ++c) {
         const uint32_t a0 = times(h0[2 * c], s0), a1 = times(h1[2 * c], s1), a2 = times(h0[2 * c + 1], s0), a3 = times(h1[2 * c + 1], s1);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma(s[nb], a0, a1, a2, a3, qf[nb][4 * w + 2 * c], qf[nb][4 * w + 2 * c + 1]);
+        for (int nb = 0; nb < NB; ++nb) {
+          if (w == 0 && c == 0) mma_first(s[nb], a0, a1, a2, a3, qf[nb][0], qf[nb][1]);
+          else mma(s[nb], a0, a1, a2, a3, qf[nb][4 * w + 2 * c], qf[nb][4 * w + 2 * c + 1]);
+        }
       }
     }
   }
 }
 
-// CTAs on an SM: what the registers allow without spilling the loop's values
-__host__ __device__ constexpr int ctas_of(int d, int nb) { return d == 256 ? (nb == 1 ? 3 : 2) : nb == 1 ? (d == 64 ? 5 : 4) : nb == 2 ? 3 : 2; }
+// CTAs on an SM: what registers (without spilling the loop's values) and shared memory allow
+__host__ __device__ constexpr int ctas_of(int d, int nb) { return d == 256 || nb > 1 ? 2 : d == 128 ? 3 : 4; }
 
 template <int D, int NB> struct Shape {
-  static constexpr int stages = D == 64 ? 4 : 2;         // of two tiles
+  static constexpr int stages = D == 64 ? 4 : D == 128 ? 3 : 2;        // of two tiles
   static constexpr int ring = kWarps * stages * 2 * Tile<D>::bytes;
+  static constexpr int record = (D / 16 + 1) * 512;                    // a warp's sums of 8 rows: 16 bytes of a lane at a time
+  static constexpr int bars = ring + (kWarps - 1) * record, flag = bars + kWarps * stages * 8, line = flag + 16;
+  static constexpr int smem = line + (int)sizeof(Line);
   static constexpr int ctas = ctas_of(D, NB);
-  static constexpr int smem = ring + kWarps * stages * 8 + 16 + (kMost + 2) * 8;
+  static_assert(ctas * (smem + 1024 + 64) <= 228 * 1024, "shared memory of an SM");
 };
 
 template <typename T, int D, int NB>
 __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention_kernel(const Fp4Args a) {
-  constexpr int STAGES = Shape<D, NB>::stages, BYTES = Tile<D>::bytes;
+  using S = Shape<D, NB>;
+  constexpr int STAGES = S::stages, BYTES = Tile<D>::bytes;
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint8_t* ring = smem + warp * STAGES * 2 * BYTES;
-  const uint32_t bar = smem_u32(smem + Shape<D, NB>::ring) + warp * STAGES * 8;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8);
-  long long* line = reinterpret_cast<long long*>(smem + Shape<D, NB>::ring + kWarps * STAGES * 8 + 16);
+  float4* records = reinterpret_cast<float4*>(smem + S::ring);
+  const uint32_t bar = smem_u32(smem + S::bars) + warp * STAGES * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::flag);
+  Line& line = *reinterpret_cast<Line*>(smem + S::line);
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(bar + 8 * s, 1);
     if (warp == 0) *abort_flag = 0;
@@ -324,32 +400,39 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
   }
   pdl_enter();
   lay_line(a, line, false);
-  const Deal deal(line[a.B], a.workers);
-  if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b <= a.B; b += kWarps * 32) a.line[b] = line[b];
+  // rows of requests without a token in sight belong to no unit
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const Request r = line.request(a, b);
+    if (r.tiles > 0) continue;
+    for (long long i = threadIdx.x; i < (long long)max(r.q_len, 0) * a.hq * (D / 8); i += kWarps * 32)
+      reinterpret_cast<uint4*>(a.out)[(long long)r.q0 * a.hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
   }
-  // neighbours in the line lie on different SMs: a short line is spread over all of them
-  const int worker = warp * gridDim.x + blockIdx.x;
+  const Deal deal(line.first[a.B], a.workers, kFewTiles);
+  const int worker = blockIdx.x;
   if (worker >= deal.workers) return;
   const long long at = deal.begin(worker);
   const int total = (int)(deal.begin(worker + 1) - at);     // tiles
   if (total <= 0) return;
 
-  // Tiles come in pairs, a stage for each. Lane i finds the places of pairs i, 32 + i, ... and fetches them: no step along the
-  // line for each tile.
-  const int pairs = (total + 1) / 2;
+  // Tiles come in pairs, dealt to the warps in turn, a stage for each. Lane i finds the places of the warp's pairs i, 32 + i,
+  // ... and fetches them: no step along the line for each tile.
+  const int pairs = ((total + 1) / 2 - warp + kWarps - 1) / kWarps;
   const uint8_t *mine0 = nullptr, *mine1 = nullptr;
   int fetched = 0;
   auto fetch = [&](int stage) {
     if (fetched % 32 == 0) {
+      const int p = 2 * (warp + kWarps * (fetched + lane));
       Walk w;
-      w.seek(a, line, at + min(2 * (fetched + lane), total - 1), false);
-      mine0 = w.address<D>(a, w.page(a));
-      w.seek(a, line, at + min(2 * (fetched + lane) + 1, total - 1), false);
-      mine1 = w.address<D>(a, w.page(a));
+      w.seek(a, line, at + min(p, total - 1), false);
+      const int page0 = w.page(a);                   // (both pages are asked for before one is used)
+      mine0 = w.address<D>(a, 0);
+      if (p + 1 < total) w.next(a, line, false);
+      const int page1 = w.page(a);
+      mine1 = w.address<D>(a, page1);
+      mine0 += (long long)page0 * a.hk * a.per * BYTES;
     }
     if (lane == fetched % 32) {
-      const bool both = 2 * fetched + 1 < total;
+      const bool both = 2 * (warp + kWarps * fetched) + 1 < total;
       const uint32_t full = bar + 8 * stage, to = smem_u32(ring + stage * 2 * BYTES);
       mbar_expect_tx(full, both ? 2 * BYTES : BYTES);
       bulk_load(to, mine0, BYTES, full);
@@ -357,51 +440,59 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     }
     ++fetched;
   };
-  for (int s = 0; s < STAGES && s < pairs; ++s) fetch(s);
+  const int g = lane >> 2, j = lane & 3;
   Walk get;
   get.seek(a, line, at, false);
+  Vec8<T> raw[NB][D / 32];       // the queries of the first unit are asked for ahead of its tiles
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) fetch_query<T, D>(a, get.r, get.head, get.rt * a.row_tile + nb * 8 + g, lane, raw[nb]);
+  for (int s = 0; s < STAGES && s < pairs; ++s) fetch(s);
 
-  const int g = lane >> 2, j = lane & 3;
-  int done = 0, stage = 0;       // done: tiles; stage: of the next one
+  int done = 0, pair = 2 * warp, stage = 0;       // done: tiles of the CTA's units so far; pair: first tile of the warp's next pair
   uint32_t phase = 0;
   bool ok = true;
   while (done < total) {
-    // ---- one unit, or this warp's part of it
+    // ---- one unit, or this CTA's part of it
     const int first = get.tile, head = get.head, row0 = get.rt * a.row_tile;
-    const int count = min(total - done, get.r.tiles - first);
+    const int count = min(total - done, get.r.tiles - first);       // tiles of it that this CTA has
     const Request r = get.r;
     const int rows = min(a.row_tile, r.q_len * a.group - row0);
     uint32_t qf[NB][D / 8];
-    float c[NB][2];              // factors of the scores of rows 2 j and 2 j + 1, above 0
+    float2 c[NB];                // factors of the scores of rows 2 j and 2 j + 1, above 0
     const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float back = load_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, qf[nb]);
-      c[nb][0] = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j), 1e-37f);
-      c[nb][1] = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j + 4), 1e-37f);
+      if (done > 0) fetch_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, raw[nb]);
+      const float back = scale_query<T, D>(a, raw[nb], qf[nb]);
+      c[nb].x = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j), 1e-37f);
+      c[nb].y = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j + 4), 1e-37f);
     }
-    // m: running maxima; base: what is taken from a score in the exponent
-    float o[NB][D / 16][4], m[NB][2], base[NB][2], l[NB][2];
+    // m: running maxima; base: minus what is taken from a score in the exponent; limit: the score, without its factor, from
+    // which the maximum moves
+    float o[NB][D / 16][4], m[NB][2], limit[NB][2];
+    float2 base[NB], l[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
-      m[nb][0] = m[nb][1] = -INFINITY;
-      base[nb][0] = base[nb][1] = -kUp;
-      l[nb][0] = l[nb][1] = 0.f;
+      m[nb][0] = m[nb][1] = limit[nb][0] = limit[nb][1] = -INFINITY;
+      base[nb] = make_float2(kUp, kUp);
+      l[nb] = make_float2(0.f, 0.f);
     }
     // tokens [lo_all, hi_all) are seen by all rows
     const int pos0 = r.n - r.q_len + row0 / a.group, pos1 = r.n - r.q_len + (row0 + rows - 1) / a.group;
     const int hi_all = pos0 + 1, lo_all = a.window > 0 ? pos1 - a.window + 1 : 0;
 
-    for (int t = 0; t < count;) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, phase, abort_flag, a.status, 401));
+    const int end = done + count;
+    auto arrive = [&](int st, uint32_t ph) { return __all_sync(0xffffffffu, mbar_wait(bar + 8 * st, ph, abort_flag, a.status, 401)); };
+    while (pair < end && ok) {
+      ok = arrive(stage, phase);
       if (!ok) break;
       const uint8_t* tile = ring + stage * 2 * BYTES;
-      // of the stage's tiles one may be another unit's: `from` .. `to` are the tokens of this one, tok0 is the stage's first
-      const int u0 = done & 1, from = u0 * kTile, to = min(2, u0 + count - t) * kTile;
-      const int tok0 = (r.tile0 + first + t - u0) * kTile;
-      if (tok0 + from <= pos1) {                               // else rows behind these see it
+      // of the pair's tiles one may be another unit's: `from` .. `to` are the tokens of this one, tok0 is the pair's first
+      const int from = max(done - pair, 0) * kTile, to = min(2, end - pair) * kTile;
+      const int tok0 = (r.tile0 + first + pair - done) * kTile;
+      if (tok0 + from <= pos1) {                                     // else rows behind these see it
         float s[2][NB][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -429,59 +520,67 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            move |= fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) * c[nb][k] > m[nb][k] + kSlack;
+            move |= fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) > limit[nb][k];
         }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              float top = fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) * c[nb][k];
+              const float factor = k ? c[nb].y : c[nb].x;
+              float top = fmaxf(fmaxf(s[0][nb][k], s[0][nb][2 + k]), fmaxf(s[1][nb][k], s[1][nb][2 + k])) * factor;
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
               top = fmaxf(top, m[nb][k]);
               const float f = m[nb][k] == top ? 1.f : exp2_fast(m[nb][k] - top);
               m[nb][k] = top;
-              base[nb][k] = (top == -INFINITY ? 0.f : top) - kUp;
-              l[nb][k] *= f;
+              limit[nb][k] = (top + kSlack) / factor;
+              (k ? base[nb].y : base[nb].x) = kUp - (top == -INFINITY ? 0.f : top);
+              (k ? l[nb].y : l[nb].x) *= f;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) { o[nb][i][k] *= f; o[nb][i][2 + k] *= f; }
             }
           }
         }
+        uint32_t p[2][NB][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t p0[NB], p1[NB];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const float e0 = exp2_fast(fmaf(s[u][nb][0], c[nb][0], -base[nb][0])), e1 = exp2_fast(fmaf(s[u][nb][1], c[nb][1], -base[nb][1])),
-                        e2 = exp2_fast(fmaf(s[u][nb][2], c[nb][0], -base[nb][0])), e3 = exp2_fast(fmaf(s[u][nb][3], c[nb][1], -base[nb][1]));
-            l[nb][0] += e0 + e2;
-            l[nb][1] += e1 + e3;
-            p0[nb] = transpose8(f16x2(e0, e1));
-            p1[nb] = transpose8(f16x2(e2, e3));
-          }
-          Raw<D> x;
-          load_values<D>(tile + u * BYTES, lane, x);
-          // values of tokens that no row sees may be anything; a NaN that only some rows see must not reach the others
-          uint32_t nan_mask = 0;       // bit 4 i + e: token 4 j + e has no number in block i of the lane's channels
-          if (ragged) {
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float2 e = fma2(make_float2(s[u][nb][2 * h], s[u][nb][2 * h + 1]), c[nb], base[nb]);
+              e.x = exp2_fast(e.x);
+              e.y = exp2_fast(e.y);
+              l[nb] = add2(l[nb], e);
+              p[u][nb][h] = transpose8(f16x2(e.x, e.y));
+            }
+        Raw<D> x[2];
+        load_values<D>(tile, lane, x[0]);
+        load_values<D>(tile + BYTES, lane, x[1]);
+        // values of tokens that no row sees may be anything; a NaN that only some rows see must not reach the others
+        uint32_t nan_mask = 0;       // bit 8 u + 4 i + e: token 4 j + e of tile u has no number in block i of the lane's channels
+        if (ragged) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < (D == 256 ? 2 : 1); ++i)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if ((x.vs[i] >> (8 * e) & 0x7F) == 0x7F) {
-                  nan_mask |= 1u << (4 * i + e);
-                  x.vs[i] &= ~(0xFFu << (8 * e));
+                if ((x[u].vs[i] >> (8 * e) & 0x7F) == 0x7F) {
+                  nan_mask |= 1u << (8 * u + 4 * i + e);
+                  x[u].vs[i] &= ~(0xFFu << (8 * e));
                 }
-          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int w = 0; w < D / 64; ++w) {                  // words of 8 channels of the lane: 4 products
             const int i = D == 256 ? w / 2 : 0;
-            const uint32_t s01 = widen_e4m3(x.vs[i]), s23 = widen_e4m3(x.vs[i] >> 16);
+            const uint32_t s01 = widen_e4m3(x[u].vs[i]), s23 = widen_e4m3(x[u].vs[i] >> 16);
             uint32_t tw[4];                                    // of tokens 4 j .. 4 j + 3
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x.v[k / 4], k % 4); }
+            for (int e = 0; e < 4; ++e) { const int k = e * (D / 64) + w; tw[e] = word(x[u].v[k / 4], k % 4); }
             uint32_t lo01[4], hi01[4], lo23[4], hi23[4];       // pairs of tokens of the even and of the odd channels
             widen((tw[0] & 0x0F0F0F0Fu) | ((tw[1] << 4) & 0xF0F0F0F0u), lo01);
             widen(((tw[0] >> 4) & 0x0F0F0F0Fu) | (tw[1] & 0xF0F0F0F0u), hi01);
@@ -491,74 +590,152 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
             for (int k = 0; k < 4; ++k) {
               const uint32_t a0 = times(lo01[k], s01), a1 = times(hi01[k], s01), a2 = times(lo23[k], s23), a3 = times(hi23[k], s23);
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma(o[nb][4 * w + k], a0, a1, a2, a3, p0[nb], p1[nb]);
+              for (int nb = 0; nb < NB; ++nb) mma(o[nb][4 * w + k], a0, a1, a2, a3, p[u][nb][0], p[u][nb][1]);
             }
           }
-          if (ragged && __any_sync(0xffffffffu, nan_mask != 0)) {
-            for (int jj = 0; jj < 4; ++jj) {
-              const uint32_t bits = __shfl_sync(0xffffffffu, nan_mask, 4 * g + jj);
-              for (int e = 0; e < 4; ++e) {
-                const int tok = u * kTile + 4 * jj + e;
+        }
+        if (ragged && __any_sync(0xffffffffu, nan_mask != 0)) {
+          for (int jj = 0; jj < 4; ++jj) {
+            const uint32_t bits = __shfl_sync(0xffffffffu, nan_mask, 4 * g + jj);
+            for (int t = 0; t < 8; ++t) {                      // tile t / 4, token t % 4 of the lane
+              const int tok = t / 4 * kTile + 4 * jj + t % 4;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
+              for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                  for (int c = 0; c < 2; ++c) {
-                    const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + c) / a.group;
-                    const bool seen = tok < min(min(pos + 1, r.n) - tok0, to) && tok >= from &&
-                                      !(a.window > 0 && tok0 + tok <= pos - a.window);
+                for (int k = 0; k < 2; ++k) {
+                  const int pos = r.n - r.q_len + (row0 + nb * 8 + 2 * j + k) / a.group;
+                  const bool seen = tok < min(min(pos + 1, r.n) - tok0, to) && tok >= from &&
+                                    !(a.window > 0 && tok0 + tok <= pos - a.window);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                      if (seen && (bits >> ((D == 256 ? i / 8 * 4 : 0) + e) & 1)) o[nb][i][c] = o[nb][i][2 + c] = NAN;
-                  }
-              }
+                  for (int i = 0; i < D / 16; ++i)
+                    if (seen && (bits >> (t / 4 * 8 + (D == 256 ? i / 8 * 4 : 0) + t % 4) & 1)) o[nb][i][k] = o[nb][i][2 + k] = NAN;
+                }
             }
           }
         }
       }
-      t += (to - from) / kTile;
-      done += (to - from) / kTile;
-      if (to == 2 * kTile) {
-        __syncwarp();
-        if (fetched < pairs) fetch(stage);
-        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-      }
+      if (to < 2 * kTile && end < total) break;          // the next unit has the pair's other tile
+      __syncwarp();
+      if (fetched < pairs) fetch(stage);
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      pair += 2 * kWarps;
     }
-    if (!ok) break;
+    done = end;
 
-    // ---- rows 2 j and 2 j + 1 of every block: channels g D / 8 .. (D / 8 of them)
-    const bool whole = first == 0 && count == r.tiles;
-    const float vh = a.v_head != nullptr ? a.v_head[head] : 1.f;
+    // ---- the warps' sums are joined in the first one, 8 rows at a time
+    auto write = [&](float4* to, int nb) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) to[i * 32 + lane] = make_float4(o[nb][i][0], o[nb][i][1], o[nb][i][2], o[nb][i][3]);
+      to[D / 16 * 32 + lane] = make_float4(m[nb][0], m[nb][1], l[nb].x, l[nb].y);
+    };
+    auto join = [&](const float4 (&x)[D / 16 + 1], int nb) {
+      const float4 ml = x[D / 16];
+      float f[2], h[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float other = k ? ml.y : ml.x, top = fmaxf(m[nb][k], other);
+        f[k] = m[nb][k] == top ? 1.f : exp2_fast(m[nb][k] - top);
+        h[k] = other == top ? 1.f : exp2_fast(other - top);
+        m[nb][k] = top;
+      }
+      l[nb] = make_float2(l[nb].x * f[0] + ml.z * h[0], l[nb].y * f[1] + ml.w * h[1]);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        o[nb][i][0] = o[nb][i][0] * f[0] + x[i].x * h[0];
+        o[nb][i][1] = o[nb][i][1] * f[1] + x[i].y * h[1];
+        o[nb][i][2] = o[nb][i][2] * f[0] + x[i].z * h[0];
+        o[nb][i][3] = o[nb][i][3] * f[1] + x[i].w * h[1];
+      }
+    };
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      for (int d = 4; d < 32; d <<= 1) {
+        l[nb].x += __shfl_xor_sync(0xffffffffu, l[nb].x, d);
+        l[nb].y += __shfl_xor_sync(0xffffffffu, l[nb].y, d);
+      }
+      if (nb * 8 >= rows) break;
+      __syncthreads();                                   // the records have been read
+      if (warp > 0) write(records + (warp - 1) * (S::record / 16), nb);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll 1
+        for (int w = 0; w < kWarps - 1; ++w) {
+          float4 x[D / 16 + 1];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+          for (int i = 0; i <= D / 16; ++i) x[i] = records[w * (S::record / 16) + i * 32 + lane];
+          join(x, nb);
+        }
+      }
+    }
+    if (warp == 0) {         // (after a wait that ran out too: the counters have to come out even)
+      bool finish = first == 0 && count == r.tiles;
+      if (!finish) {
+        // the unit's other parts: of the workers from the one that it begins with to the one that it ends with
+        const long long u0 = at + (end - count) - first;
+        const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
+        float4* part = reinterpret_cast<float4*>(a.parts);
+        auto place = [&](int w, int nb) { return part + ((long long)(2 * w + (w == w0 ? 1 : 0)) * NB + nb) * (S::record / 16); };
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
-        const int row = nb * 8 + 2 * j + c;
-        if (row >= rows) continue;
-        if (whole) {
-          const float f = l[nb][c] > 0.f || l[nb][c] != l[nb][c] ? vh / l[nb][c] : 0.f;
-          const int qi = (row0 + row) / a.group;
-          const long long to = (long long)(r.q0 + qi) * a.hq + head * a.group + (row0 + row - qi * a.group);
-          T* dst = reinterpret_cast<T*>(a.out) + to * D + g * (D / 8);
+        for (int nb = 0; nb < NB; ++nb)
+          if (nb * 8 < rows) write(place(worker, nb), nb);
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) {
+          __threadfence();
+          before = atomicAdd(a.arrived + w0, 1);
+        }
+        before = __shfl_sync(0xffffffffu, before, 0);
+        finish = before == w1 - w0;
+        if (finish) {
+          __threadfence();
+          if (lane == 0) a.arrived[w0] = 0;
 #pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            float y[8];
+          for (int nb = 0; nb < NB; ++nb) {
+            if (nb * 8 >= rows) break;
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { y[2 * e] = o[nb][4 * i + e][c] * f; y[2 * e + 1] = o[nb][4 * i + e][2 + c] * f; }
-            store8(dst + 8 * i, y);
+            for (int i = 0; i < D / 16; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+            float4 x[2][D / 16 + 1];                     // one part is on its way while the other is added
+            auto ask = [&](int w, float4 (&x)[D / 16 + 1]) {
+              const float4* from = place(min(w, w1), nb) + lane;
+#pragma unroll
+              for (int i = 0; i <= D / 16; ++i) x[i] = __ldcg(from + i * 32);
+            };
+            ask(w0, x[0]);
+#pragma unroll 1
+            for (int w = w0; w <= w1; w += 2) {
+              ask(w + 1, x[1]);
+              join(x[0], nb);
+              if (w == w1) break;
+              ask(w + 2, x[0]);
+              join(x[1], nb);
+            }
           }
-          if (a.lse != nullptr && g == 0) a.lse[to] = (m[nb][c] == -INFINITY ? 0.f : m[nb][c]) - kUp + log2f(l[nb][c]);
-        } else {
-          float* part = a.parts + ((long long)(2 * worker + (first == 0 ? 1 : 0)) * a.row_tile + row) * (D + 4);
+        }
+      }
+      if (finish) {
+        // rows 2 j and 2 j + 1 of every block: channels g D / 8 .. (D / 8 of them)
+        const float vh = a.v_head != nullptr ? a.v_head[head] : 1.f;
 #pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            float y[8];
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { y[2 * e] = o[nb][4 * i + e][c]; y[2 * e + 1] = o[nb][4 * i + e][2 + c]; }
-            store8(part + g * (D / 8) + 8 * i, y);
+          for (int k = 0; k < 2; ++k) {
+            const int row = nb * 8 + 2 * j + k;
+            if (row >= rows) continue;
+            const float sum = k ? l[nb].y : l[nb].x, f = sum > 0.f || sum != sum ? vh / sum : 0.f;
+            const int qi = (row0 + row) / a.group;
+            const long long to = (long long)(r.q0 + qi) * a.hq + head * a.group + (row0 + row - qi * a.group);
+            T* dst = reinterpret_cast<T*>(a.out) + to * D + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { y[2 * e] = o[nb][4 * i + e][k] * f; y[2 * e + 1] = o[nb][4 * i + e][2 + k] * f; }
+              store8(dst + 8 * i, y);
+            }
+            if (a.lse != nullptr && g == 0) a.lse[to] = (m[nb][k] == -INFINITY ? 0.f : m[nb][k]) - kUp + log2f(sum);
           }
-          if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[nb][c], l[nb][c]);
         }
       }
     }
@@ -570,85 +747,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
   }
 }
 
-// Rows of units that several workers share, or that see nothing: the parts joined. SPREAD warps of a CTA take the parts of one
-// (row, query head) in turn.
-template <typename T, int D, int SPREAD> __global__ void __launch_bounds__(256) fp4_join_kernel(const Fp4Args a, int total_rows) {
-  constexpr int E = D / 32, AHEAD = 4;
-  __shared__ float sum[8][D + 2];
-  pdl_enter();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long id = (long long)blockIdx.x * (8 / SPREAD) + warp / SPREAD;
-  const int row = (int)(id / a.hq), qh = (int)(id - (long long)row * a.hq), mine = warp % SPREAD;
-  // of another launch, or of no request; the CTA's rows may differ in it
-  bool there = id < (long long)total_rows * a.hq && row >= a.cu_q[0] && row < a.cu_q[a.B], empty = false;
-  float m = -INFINITY, l = 0.f, y[E] = {};
-  int head = 0;
-  if (there) {
-    int lo = 0, hi = a.B - 1;                             // the last request that starts at or before the row
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
-    }
-    Request r;
-    r.load(a, lo);
-    empty = r.tiles == 0;
-    if (!empty) {
-      const Deal deal(a.line[a.B], a.workers);
-      head = qh / a.group;
-      const int in_unit = (row - r.q0) * a.group + qh - head * a.group;
-      const int rt = in_unit / a.row_tile, in_tile = in_unit - rt * a.row_tile;
-      const long long u0 = a.line[lo] + ((long long)head * r.row_tiles + rt) * r.tiles;
-      const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
-      there = w0 != w1;                                   // else written by its worker
-      for (int wb = w0 + mine; there && wb <= w1; wb += AHEAD * SPREAD) {
-        float2 ml[AHEAD];
-        float x[AHEAD][E];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const int w = wb + i * SPREAD;
-          ml[i] = make_float2(-INFINITY, 0.f);
-          const float* part = a.parts + ((long long)(2 * w + (w == w0 ? 1 : 0)) * a.row_tile + in_tile) * (D + 4);
-          if (w <= w1) ml[i] = *reinterpret_cast<const float2*>(part + D);
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[i][e] = w <= w1 ? part[lane * E + e] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const float top = fmaxf(m, ml[i].x);
-          const float f0 = m == top ? 1.f : exp2_fast(m - top), f1 = ml[i].x == top ? 1.f : exp2_fast(ml[i].x - top);
-          m = top;
-          l = l * f0 + ml[i].y * f1;
-#pragma unroll
-          for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + x[i][e] * f1;
-        }
-      }
-    }
-  }
-  if (SPREAD > 1) {
-    if (mine != 0) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum[warp][lane * E + e] = y[e];
-      if (lane == 0) { sum[warp][D] = m; sum[warp][D + 1] = l; }
-    }
-    __syncthreads();
-    if (mine != 0) return;
-    for (int k = 1; k < SPREAD; ++k) {
-      const float* o = sum[warp + k];
-      const float top = fmaxf(m, o[D]), f0 = m == top ? 1.f : exp2_fast(m - top), f1 = o[D] == top ? 1.f : exp2_fast(o[D] - top);
-      m = top;
-      l = l * f0 + o[D + 1] * f1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = y[e] * f0 + o[lane * E + e] * f1;
-    }
-  }
-  if (!there) return;
-  const float f = l > 0.f || l != l ? (a.v_head != nullptr ? a.v_head[head] : 1.f) / l : 0.f;
-  if (a.lse != nullptr && lane == 0 && !empty) a.lse[id] = (m == -INFINITY ? 0.f : m) - kUp + log2f(l);
-  T* dst = reinterpret_cast<T*>(a.out) + id * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<typename Pack2<T>::type*>(dst + e) = Pack2<T>::make(y[e] * f, y[e + 1] * f);
-}
-
 // What the rows give every token: the keys once more, with the rows' final maxima and sums. A tile's keys go through all rows of
 // their (request, key head) pair, so a token's sum is taken by one lane in one order. MANY false: up to 8 rows, in registers;
 // warps deal out the tiles of all pairs. MANY: CTAs do; the pair's queries lie in shared memory, kChunk blocks of 8 rows at
@@ -658,7 +756,7 @@ template <int D, bool MANY> struct WeightsShape {
   static constexpr int chunk = !MANY ? 0 : D == 256 ? 4 : 8;           // blocks of 8 rows
   static constexpr int ctas = D == 256 ? 2 : 4;
   static constexpr int ring = kWarps * stages * key_bytes, bars = ring, slots = bars + kWarps * stages * 8;
-  static constexpr int flag = slots + kWarps * stages * 4, line = flag + 16, queries = line + (kMost + 2) * 8;
+  static constexpr int flag = slots + kWarps * stages * 4, line = flag + 16, queries = (line + (int)sizeof(Line) + 15) / 16 * 16;
   static constexpr int rows = queries + chunk * 16 * D, smem = rows + chunk * 8 * 8;
 };
 
@@ -693,7 +791,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
   const uint32_t bar = smem_u32(smem + S::bars) + warp * STAGES * 8;
   int* slots = reinterpret_cast<int*>(smem + S::slots) + warp * STAGES;        // of the pool: the stages' tiles
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::flag);
-  long long* line = reinterpret_cast<long long*>(smem + S::line);
+  Line& line = *reinterpret_cast<Line*>(smem + S::line);
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(bar + 8 * s, 1);
     if (warp == 0) *abort_flag = 0;
@@ -701,7 +799,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
   }
   pdl_enter();
   lay_line(a, line, true);
-  const Deal deal(line[a.B], MANY ? gridDim.x : gridDim.x * kWarps);
+  const Deal deal(line.first[a.B], MANY ? gridDim.x : gridDim.x * kWarps, MANY ? 8 : 4);
   const int worker = MANY ? blockIdx.x : warp * gridDim.x + blockIdx.x;
   if (worker >= deal.workers) return;
   long long at = deal.begin(worker);
@@ -931,7 +1029,7 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
     for (int i = 0; i < 8; ++i) *reinterpret_cast<uint2*>(vt + ((long long)h * 128 + 64 + g * 8 + i) * t_cap + t0 + 4 * j) = make_uint2(0, 0);
 }
 
-template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows, int sms, cudaStream_t stream) {
+template <typename T, int D, int NB> int launch(const Fp4Args& a, int sms, cudaStream_t stream) {
   using S = Shape<D, NB>;
   static bool ready[64] = {}, weights_ready[64] = {};
   int dev = 0;
@@ -941,14 +1039,8 @@ template <typename T, int D, int NB> int launch(const Fp4Args& a, int total_rows
     if (e != cudaSuccess) { msgl_set_error("paged_attention_fp4 shared memory", e); return MSGL_CUDA_ERROR; }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  msgl_launch(fp4_attention_kernel<T, D, NB>, dim3(a.workers / kWarps), dim3(kWarps * 32), S::smem, stream, a);
+  msgl_launch(fp4_attention_kernel<T, D, NB>, dim3(a.workers), dim3(kWarps * 32), S::smem, stream, a);
   MSGL_CHECK_LAUNCH("paged_attention_fp4");
-  // a row's parts are some workers / (requests * key heads * row tiles): up to four for a warp
-  const long long rows = (long long)total_rows * a.hq, each = (long long)a.workers * a.row_tile / (rows > 0 ? rows : 1);
-  if (each < 8) msgl_launch(fp4_join_kernel<T, D, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a, total_rows);
-  else if (each < 16) msgl_launch(fp4_join_kernel<T, D, 2>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, total_rows);
-  else msgl_launch(fp4_join_kernel<T, D, 8>, dim3((unsigned)rows), dim3(256), 0, stream, a, total_rows);
-  MSGL_CHECK_LAUNCH("paged_attention_fp4 join");
   if (a.weights != nullptr) {
     using W = WeightsShape<D, (NB > 1)>;
     if (dev < 0 || dev >= 64 || !weights_ready[dev]) {
@@ -974,6 +1066,8 @@ int device_sms() {
   return n;
 }
 
+long long parts_words(int d, int nb, int workers) { return 2ll * workers * nb * (d / 16 + 1) * 128; }
+
 int* status_word() {
   static int* word[64] = {};
   int dev = 0;
@@ -986,22 +1080,22 @@ int* status_word() {
 }
 
 int worker_count(int d, int nb) {
-  return device_sms() * ctas_of(d, nb) * kWarps;
+  return device_sms() * ctas_of(d, nb);
 }
 
 }  // namespace
 
-// fp32 words of the workspace: the parts, the line (64 bits each), the rows' sums with weights.
-MSGL_API long long msgl_attention_fp4_workspace(int total_rows, int B, int hq, int hk, int d, int max_q, int weighed) {
+// fp32 words of the workspace: the parts; the rows' sums with weights. `workers`: words of `arrived`.
+MSGL_API long long msgl_attention_fp4_workspace(int total_rows, int hq, int hk, int d, int max_q, int weighed, int* workers) {
   if (hk <= 0) return 0;
-  const int nb = row_blocks(d, max_q * (hq / hk));
-  const long long parts = 2ll * worker_count(d, nb) * nb * 8 * (d + 4);
-  return parts + 2ll * ((B < kMost ? B : kMost) + 2) + (weighed ? (long long)total_rows * hq : 0);
+  const int nb = row_blocks(d, max_q * (hq / hk)), most = worker_count(d, nb);
+  *workers = most;
+  return parts_words(d, nb, most) + (weighed ? (long long)total_rows * hq : 0);
 }
 
 MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, const void* table, long long table_stride, int width,
                                 const void* cu_q, const void* lens, const void* k_head, const void* v_head, void* weights,
-                                void* workspace, int total_rows, int B, int hq, int hk, int d, int page_size, int pages, int max_q,
+                                void* workspace, void* arrived, int total_rows, int B, int hq, int hk, int d, int page_size, int pages, int max_q,
                                 int window, float scale, int dtype, cudaStream_t stream) {
   if (B <= 0 || total_rows <= 0) return MSGL_OK;
   if (hk <= 0 || hq <= 0 || hq % hk || (d != 64 && d != 128 && d != 256) || page_size <= 0 || page_size % kTile ||
@@ -1013,7 +1107,6 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
   const int nb = row_blocks(d, max_q * (hq / hk)), workers = worker_count(d, nb);
   int* status = status_word();
   float* ws = (float*)workspace;
-  const long long parts = 2ll * workers * nb * 8 * (d + 4);
   for (int b0 = 0; b0 < B; b0 += kMost) {
     Fp4Args a{};
     a.B = B - b0 < kMost ? B - b0 : kMost;
@@ -1021,13 +1114,13 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
     a.table = (const int32_t*)table + b0 * table_stride; a.table_stride = table_stride; a.width = width;
     a.cu_q = (const int32_t*)cu_q + b0; a.lens = (const int32_t*)lens + b0;
     a.k_head = (const float*)k_head; a.v_head = (const float*)v_head; a.weights = (float*)weights;
-    a.parts = ws; a.line = (long long*)(ws + parts);
-    a.lse = weights != nullptr ? ws + parts + 2ll * ((B < kMost ? B : kMost) + 2) : nullptr;
+    a.parts = ws; a.arrived = (int*)arrived;
+    a.lse = weights != nullptr ? ws + parts_words(d, nb, workers) : nullptr;
     a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages; a.window = window;
-    a.row_tile = 8 * nb; a.workers = workers; a.scale = scale; a.status = status;
+    a.row_tile = 8 * nb; a.row_shift = nb == 1 ? 3 : nb == 2 ? 4 : 5; a.workers = workers; a.scale = scale; a.status = status;
     int rc = MSGL_BAD_ARG;
     const int sms = device_sms();
-#define RUN(T, D, N) rc = launch<T, D, N>(a, total_rows, sms, stream)
+#define RUN(T, D, N) rc = launch<T, D, N>(a, sms, stream)
 #define WIDTHS(T)                                                                                                          \
   if (d == 64) { if (nb == 1) RUN(T, 64, 1); else if (nb == 2) RUN(T, 64, 2); else RUN(T, 64, 4); }                         \
   else if (d == 128) { if (nb == 1) RUN(T, 128, 1); else if (nb == 2) RUN(T, 128, 2); else RUN(T, 128, 4); }                \

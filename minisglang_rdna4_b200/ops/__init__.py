@@ -20,10 +20,14 @@ def _cuda():
     return cuda
 
 
-def _fp4():
-    from . import kv_fp4
+_kv_fp4 = None
 
-    return kv_fp4
+
+def _fp4():
+    global _kv_fp4
+    if _kv_fp4 is None:          # an import statement at every call would cost as much as all checks of arguments
+        from . import kv_fp4 as _kv_fp4
+    return _kv_fp4
 
 
 def _ref_fp4():

@@ -2,6 +2,7 @@
 ``csrc/attention_fp4.cu``. The checks hold on the CPU path too (``ops.ref_fp4``)."""
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, Optional, Tuple
 
 import numpy as np
@@ -14,8 +15,8 @@ from ._lib import c_f, c_i, c_ll, c_p, check, lib
 _lib.bind("msgl_store_fp4", c_i, [c_p, c_p, c_ll, c_ll] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 9 + [c_p])
-_lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 6 + [c_i] * 9 + [c_f, c_i, c_p])
-_lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 7)
+_lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 7 + [c_i] * 9 + [c_f, c_i, c_p])
+_lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 6 + [c_p])
 _lib.bind("msgl_gather_fp4", c_i, [c_p, c_p, c_ll, c_i] + [c_p] * 4 + [c_ll] + [c_i] * 6 + [c_p])
 _lib.bind("msgl_attention_fp4_status", c_i, [c_i])
 
@@ -147,18 +148,19 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
     return kept, lens
 
 
-_NEED: Dict[Tuple, int] = {}
+_NEED: Dict[Tuple, Tuple[int, int]] = {}
 
 
-def attention_fp4_workspace(rows: int, batch: int, heads: int, kv_heads: int, dim: int, max_q: int, weighed: bool) -> int:
-    """fp32 words that a call of ``paged_attention_fp4`` takes; no call of fewer rows, requests or ``max_q`` takes more, but
-    for the steps of ``max_q`` at which row tiles widen."""
-    key = (rows if weighed else 0, batch, heads, kv_heads, dim, max_q, weighed)
+def attention_fp4_workspace(rows: int, heads: int, kv_heads: int, dim: int, max_q: int, weighed: bool) -> Tuple[int, int]:
+    """fp32 words that a call of ``paged_attention_fp4`` takes as its workspace, and its counters."""
+    key = (rows if weighed else 0, heads, kv_heads, dim, max_q, weighed, torch._C._cuda_getDevice())
     hit = _NEED.get(key)
     if hit is None:
         if len(_NEED) > 4096:
             _NEED.clear()
-        _NEED[key] = hit = int(lib().msgl_attention_fp4_workspace(rows, batch, heads, kv_heads, dim, max_q, int(weighed)))
+        workers = ctypes.c_int()
+        words = int(lib().msgl_attention_fp4_workspace(rows, heads, kv_heads, dim, max_q, int(weighed), ctypes.addressof(workers)))
+        _NEED[key] = hit = (words, workers.value)
     return hit
 
 
@@ -178,14 +180,15 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v
         max_q = int((cu_q[1:] - cu_q[:-1]).max())
     if max_q == 0:
         return out
-    need = attention_fp4_workspace(t, b, hq, hk, dim, max_q, weights is not None)
+    need, workers = attention_fp4_workspace(t, hq, hk, dim, max_q, weights is not None)
     if workspace is None or workspace.numel() < need or workspace.data_ptr() % 16:
         workspace = torch.empty(need, dtype=torch.float32, device=q.device)
     check(lib().msgl_attention_fp4(
         q.data_ptr(), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        cu_q.data_ptr(), seq_lens.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights), workspace.data_ptr(), t, b, hq, hk, dim,
-        page, pages, max_q, window, scale, K._dt(q), K._stream()), "paged_attention_fp4")
-    K._count("paged_attention_fp4", "fp4_attention_kernel", 2 + (weights is not None))
+        cu_q.data_ptr(), seq_lens.data_ptr(), K._p(k_scale), K._p(v_scale), K._p(weights), workspace.data_ptr(),
+        K._stream_counters(q.device, workers).data_ptr(), t, b, hq, hk, dim, page, pages, max_q, window, scale, K._dt(q),
+        K._stream()), "paged_attention_fp4")
+    K._count("paged_attention_fp4", "fp4_attention_kernel", 1 + (weights is not None))
     return out
 
 
