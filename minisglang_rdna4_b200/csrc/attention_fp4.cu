@@ -128,11 +128,14 @@ struct Line {
   }
 };
 
-__device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whole_rows) {
+// Returns the tiles of a unit where all have as many, else 0.
+__device__ __forceinline__ int lay_line(const Fp4Args& a, Line& line, bool whole_rows) {
   __shared__ long long sums[kWarps];
+  __shared__ int least[kWarps], most[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int PER = kMost / (kWarps * 32);
   long long cost[PER], mine = 0;
+  int low = 0x7fffffff, high = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = (int)threadIdx.x * PER + i;
@@ -151,6 +154,7 @@ __device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whol
       line.tiles[b] = r.tiles;
       if (b == a.B - 1) line.row[a.B] = row_end;
       cost[i] = (long long)r.tiles * a.hk * (whole_rows ? 1 : r.row_tiles);
+      if (r.tiles > 0) { low = min(low, r.tiles); high = max(high, r.tiles); }
     }
     mine += cost[i];
   }
@@ -160,11 +164,17 @@ __device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whol
     const long long up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
-  if (lane == 31) sums[warp] = incl;
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 31) { sums[warp] = incl; least[warp] = low; most[warp] = high; }
   __syncthreads();
   long long before = incl - mine;
 #pragma unroll
-  for (int w = 0; w < kWarps - 1; ++w) before += w < warp ? sums[w] : 0;
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? sums[w] : 0;
+    low = min(low, least[w]);
+    high = max(high, most[w]);
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = (int)threadIdx.x * PER + i;
@@ -173,6 +183,7 @@ __device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whol
     if (b == a.B - 1) line.first[a.B] = before;
   }
   __syncthreads();
+  return low == high ? high : 0;
 }
 
 // Divisions of 64 bits are calls; most lines are shorter than 2^32 tiles.
@@ -180,17 +191,39 @@ __device__ __forceinline__ long long quotient(long long x, int y) {
   return (x >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
 }
 
-// Worker w of W has tiles [begin(w), begin(w + 1)): `base`, and one more for the first `extra`.
+// Worker w of W has tiles [begin(w), begin(w + 1)): `base`, and one more for the first `extra`. Short units that are all as
+// long (`pieces` > 0) are cut into so many pieces each instead: a CTA then has one unit only, and no second one to wait for.
 struct Deal {
   long long base;
-  int workers, extra;
-  __device__ __forceinline__ Deal(long long total, int most, int few) {
+  int workers, extra, pieces, tiles;
+  __device__ __forceinline__ Deal(long long total, int most, int few, int same = 0) {
     workers = (int)max(1ll, min((long long)most, quotient(total, few)));
     base = quotient(total, workers);
     extra = (int)(total - base * workers);
+    pieces = 0;
+    tiles = same;
+    if (same > 0 && base < 3 * few) {
+      const int units = (int)quotient(total, same);
+      const int p = min(most / units, (same + few - 1) / few);
+      if (p > 0) {
+        pieces = p;
+        workers = units * p;
+        base = (same + p - 1) / p;
+      }
+    }
   }
-  __device__ __forceinline__ long long begin(int w) const { return w * base + min(w, extra); }
+  __device__ __forceinline__ long long begin(int w) const {
+    if (pieces > 0) {
+      const int unit = w / pieces;
+      return (long long)unit * tiles + min((w - unit * pieces) * (int)base, tiles);
+    }
+    return w * base + min(w, extra);
+  }
   __device__ __forceinline__ int owner(long long at) const {
+    if (pieces > 0) {
+      const int unit = (int)quotient(at, tiles);
+      return unit * pieces + (int)(at - (long long)unit * tiles) / (int)base;
+    }
     const long long big = (base + 1) * extra;
     if ((base >> 31) == 0) return (int)(at < big ? quotient(at, (int)base + 1) : extra + quotient(at - big, max((int)base, 1)));
     return (int)(at < big ? at / (base + 1) : extra + (at - big) / base);
@@ -399,7 +432,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     fence_barrier_init();
   }
   pdl_enter();
-  lay_line(a, line, false);
+  const int same = lay_line(a, line, false);
   // rows of requests without a token in sight belong to no unit
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     const Request r = line.request(a, b);
@@ -407,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     for (long long i = threadIdx.x; i < (long long)max(r.q_len, 0) * a.hq * (D / 8); i += kWarps * 32)
       reinterpret_cast<uint4*>(a.out)[(long long)r.q0 * a.hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
   }
-  const Deal deal(line.first[a.B], a.workers, kFewTiles);
+  const Deal deal(line.first[a.B], a.workers, kFewTiles, same);
   const int worker = blockIdx.x;
   if (worker >= deal.workers) return;
   const long long at = deal.begin(worker);
@@ -462,7 +495,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      if (done > 0) fetch_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, raw[nb]);
       const float back = scale_query<T, D>(a, raw[nb], qf[nb]);
       c[nb].x = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j), 1e-37f);
       c[nb].y = fmaxf(kh * __shfl_sync(0xffffffffu, back, 8 * j + 4), 1e-37f);
@@ -621,6 +653,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
       pair += 2 * kWarps;
     }
     done = end;
+    if (done < total) {                                              // the next unit's queries are asked for
+      get.next_unit(a, line, false);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) fetch_query<T, D>(a, get.r, get.head, get.rt * a.row_tile + nb * 8 + g, lane, raw[nb]);
+    }
 
     // ---- the warps' sums are joined in the first one, 8 rows at a time
     auto write = [&](float4* to, int nb) {
@@ -739,7 +776,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
         }
       }
     }
-    if (done < total) get.next_unit(a, line, false);
   }
   if (!ok) {     // copies may be in flight: they land before the shared memory goes
     const uint64_t t0 = globaltimer_ns();
