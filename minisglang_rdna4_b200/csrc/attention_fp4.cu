@@ -118,6 +118,8 @@ struct Request {
 struct Line {
   long long first[kMost + 1];
   int row[kMost + 1], n[kMost], tile0[kMost], tiles[kMost];
+  int piece[kMost + 1];     // first piece of every request, where units are cut into pieces of `cut` tiles
+  int cut;                  // else 0
   __device__ __forceinline__ Request request(const Fp4Args& a, int b) const {
     Request r;
     r.rows_to(a, row[b], row[b + 1]);
@@ -128,18 +130,41 @@ struct Line {
   }
 };
 
-// Returns the tiles of a unit where all have as many, else 0.
-__device__ __forceinline__ int lay_line(const Fp4Args& a, Line& line, bool whole_rows) {
-  __shared__ long long sums[kWarps];
-  __shared__ int least[kWarps], most[kWarps];
+// Sum of v over the CTA's threads in front of this one; `all`: over all of them.
+template <typename V> __device__ __forceinline__ V scan(V v, V* sums, V& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  V incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  V before = incl - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? sums[w] : V(0);
+    all += sums[w];
+  }
+  return before;
+}
+
+// `few` > 0: units may be cut into pieces of their own. The tiles of all units are dealt evenly then only if there are many: a
+// CTA with the end of one unit and the beginning of another has two units to wait for, which counts where they are short.
+// B200, us, dealt -> cut, 32 query and 8 key heads of 128: one request of 700 tokens 16.4 -> 12.4, 8 of 100 to 300 16.6 -> 12.5.
+__device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whole_rows, int few) {
+  __shared__ long long sums[kWarps];
+  __shared__ int sums32[2][kWarps];
   constexpr int PER = kMost / (kWarps * 32);
-  long long cost[PER], mine = 0;
-  int low = 0x7fffffff, high = 0;
+  long long cost[PER], mine = 0, total;
+  int units[PER], tiles[PER], my_units = 0, all_units;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = (int)threadIdx.x * PER + i;
     cost[i] = 0;
+    units[i] = tiles[i] = 0;
     if (b < a.B) {
       const int row = a.cu_q[b], row_end = a.cu_q[b + 1], len = a.lens[b];
       Request r;
@@ -153,28 +178,14 @@ __device__ __forceinline__ int lay_line(const Fp4Args& a, Line& line, bool whole
       line.tile0[b] = r.tile0;
       line.tiles[b] = r.tiles;
       if (b == a.B - 1) line.row[a.B] = row_end;
-      cost[i] = (long long)r.tiles * a.hk * (whole_rows ? 1 : r.row_tiles);
-      if (r.tiles > 0) { low = min(low, r.tiles); high = max(high, r.tiles); }
+      tiles[i] = r.tiles;
+      units[i] = r.tiles > 0 ? a.hk * (whole_rows ? 1 : r.row_tiles) : 0;
+      cost[i] = (long long)r.tiles * units[i];
     }
     mine += cost[i];
+    my_units += units[i];
   }
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  low = __reduce_min_sync(0xffffffffu, low);
-  high = __reduce_max_sync(0xffffffffu, high);
-  if (lane == 31) { sums[warp] = incl; least[warp] = low; most[warp] = high; }
-  __syncthreads();
-  long long before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    before += w < warp ? sums[w] : 0;
-    low = min(low, least[w]);
-    high = max(high, most[w]);
-  }
+  long long before = scan(mine, sums, total);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = (int)threadIdx.x * PER + i;
@@ -182,8 +193,27 @@ __device__ __forceinline__ int lay_line(const Fp4Args& a, Line& line, bool whole
     before += cost[i];
     if (b == a.B - 1) line.first[a.B] = before;
   }
+  int cut = 0;
+  if (few > 0) {
+    scan(my_units, sums32[0], all_units);
+    if (all_units <= a.workers / 2 && total < 3ll * few * a.workers) {
+      // so many pieces at most: one more for each unit than tiles / cut
+      cut = max(few, (int)((total + a.workers - all_units - 1) / (a.workers - all_units)));
+      int pieces = 0, all;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) pieces += units[i] * ((tiles[i] + cut - 1) / cut);
+      int at = scan(pieces, sums32[1], all);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = (int)threadIdx.x * PER + i;
+        if (b < a.B) line.piece[b] = at;
+        at += units[i] * ((tiles[i] + cut - 1) / cut);
+        if (b == a.B - 1) line.piece[a.B] = at;
+      }
+    }
+  }
+  if (threadIdx.x == 0) line.cut = cut;
   __syncthreads();
-  return low == high ? high : 0;
 }
 
 // Divisions of 64 bits are calls; most lines are shorter than 2^32 tiles.
@@ -191,42 +221,39 @@ __device__ __forceinline__ long long quotient(long long x, int y) {
   return (x >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
 }
 
-// Worker w of W has tiles [begin(w), begin(w + 1)): `base`, and one more for the first `extra`. Short units that are all as
-// long (`pieces` > 0) are cut into so many pieces each instead: a CTA then has one unit only, and no second one to wait for.
+// Worker w of W has tiles [begin(w), begin(w + 1)): `base`, and one more for the first `extra`.
 struct Deal {
   long long base;
-  int workers, extra, pieces, tiles;
-  __device__ __forceinline__ Deal(long long total, int most, int few, int same = 0) {
+  int workers, extra;
+  __device__ __forceinline__ Deal(long long total, int most, int few) {
     workers = (int)max(1ll, min((long long)most, quotient(total, few)));
     base = quotient(total, workers);
     extra = (int)(total - base * workers);
-    pieces = 0;
-    tiles = same;
-    if (same > 0 && base < 3 * few) {
-      const int units = (int)quotient(total, same);
-      const int p = min(most / units, (same + few - 1) / few);
-      if (p > 0) {
-        pieces = p;
-        workers = units * p;
-        base = (same + p - 1) / p;
-      }
-    }
   }
-  __device__ __forceinline__ long long begin(int w) const {
-    if (pieces > 0) {
-      const int unit = w / pieces;
-      return (long long)unit * tiles + min((w - unit * pieces) * (int)base, tiles);
-    }
-    return w * base + min(w, extra);
-  }
+  __device__ __forceinline__ long long begin(int w) const { return w * base + min(w, extra); }
   __device__ __forceinline__ int owner(long long at) const {
-    if (pieces > 0) {
-      const int unit = (int)quotient(at, tiles);
-      return unit * pieces + (int)(at - (long long)unit * tiles) / (int)base;
-    }
     const long long big = (base + 1) * extra;
     if ((base >> 31) == 0) return (int)(at < big ? quotient(at, (int)base + 1) : extra + quotient(at - big, max((int)base, 1)));
     return (int)(at < big ? at / (base + 1) : extra + (at - big) / base);
+  }
+};
+// Worker w's piece of a unit: its tiles, and the workers that have the unit.
+struct Piece {
+  long long begin;
+  int count, w0, w1;
+  __device__ __forceinline__ Piece(const Line& line, int B, int w) {
+    count = 0;
+    if (w >= line.piece[B]) return;
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (line.piece[mid] <= w) lo = mid; else hi = mid - 1;
+    }
+    const int tiles = line.tiles[lo], cut = line.cut, each = (tiles + cut - 1) / cut, at = w - line.piece[lo], unit = at / each;
+    w0 = line.piece[lo] + unit * each;
+    w1 = w0 + each - 1;
+    begin = line.first[lo] + (long long)unit * tiles + (w - w0) * cut;
+    count = min(cut, tiles - (w - w0) * cut);
   }
 };
 
@@ -432,7 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     fence_barrier_init();
   }
   pdl_enter();
-  const int same = lay_line(a, line, false);
+  lay_line(a, line, false, kFewTiles);
   // rows of requests without a token in sight belong to no unit
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     const Request r = line.request(a, b);
@@ -440,11 +467,20 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
     for (long long i = threadIdx.x; i < (long long)max(r.q_len, 0) * a.hq * (D / 8); i += kWarps * 32)
       reinterpret_cast<uint4*>(a.out)[(long long)r.q0 * a.hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
   }
-  const Deal deal(line.first[a.B], a.workers, kFewTiles, same);
   const int worker = blockIdx.x;
-  if (worker >= deal.workers) return;
-  const long long at = deal.begin(worker);
-  const int total = (int)(deal.begin(worker + 1) - at);     // tiles
+  const Deal deal(line.first[a.B], a.workers, kFewTiles);
+  long long at = 0;
+  int total = 0, piece0 = 0, piece1 = 0;      // tiles; workers of the unit where units are cut
+  if (line.cut > 0) {
+    const Piece p(line, a.B, worker);
+    at = p.begin;
+    total = p.count;
+    piece0 = p.w0;
+    piece1 = p.w1;
+  } else if (worker < deal.workers) {
+    at = deal.begin(worker);
+    total = (int)(deal.begin(worker + 1) - at);
+  }
   if (total <= 0) return;
 
   // Tiles come in pairs, dealt to the warps in turn, a stage for each. Lane i finds the places of the warp's pairs i, 32 + i,
@@ -709,7 +745,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
       if (!finish) {
         // the unit's other parts: of the workers from the one that it begins with to the one that it ends with
         const long long u0 = at + (end - count) - first;
-        const int w0 = deal.owner(u0), w1 = deal.owner(u0 + r.tiles - 1);
+        const int w0 = line.cut > 0 ? piece0 : deal.owner(u0), w1 = line.cut > 0 ? piece1 : deal.owner(u0 + r.tiles - 1);
         float4* part = reinterpret_cast<float4*>(a.parts);
         auto place = [&](int w, int nb) { return part + ((long long)(2 * w + (w == w0 ? 1 : 0)) * NB + nb) * (S::record / 16); };
 #pragma unroll
@@ -834,7 +870,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     fence_barrier_init();
   }
   pdl_enter();
-  lay_line(a, line, true);
+  lay_line(a, line, true, 0);
   const Deal deal(line.first[a.B], MANY ? gridDim.x : gridDim.x * kWarps, MANY ? 8 : 4);
   const int worker = MANY ? blockIdx.x : warp * gridDim.x + blockIdx.x;
   if (worker >= deal.workers) return;
@@ -1065,9 +1101,9 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
     for (int i = 0; i < 8; ++i) *reinterpret_cast<uint2*>(vt + ((long long)h * 128 + 64 + g * 8 + i) * t_cap + t0 + 4 * j) = make_uint2(0, 0);
 }
 
-template <typename T, int D, int NB> int launch(const Fp4Args& a, int sms, cudaStream_t stream) {
+template <typename T, int D, int NB> int launch(const Fp4Args& a, cudaStream_t stream) {
   using S = Shape<D, NB>;
-  static bool ready[64] = {}, weights_ready[64] = {};
+  static bool ready[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
@@ -1077,20 +1113,28 @@ template <typename T, int D, int NB> int launch(const Fp4Args& a, int sms, cudaS
   }
   msgl_launch(fp4_attention_kernel<T, D, NB>, dim3(a.workers), dim3(kWarps * 32), S::smem, stream, a);
   MSGL_CHECK_LAUNCH("paged_attention_fp4");
-  if (a.weights != nullptr) {
-    using W = WeightsShape<D, (NB > 1)>;
-    if (dev < 0 || dev >= 64 || !weights_ready[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(fp4_weights_kernel<T, D, (NB > 1)>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::smem);
-      if (e != cudaSuccess) { msgl_set_error("paged_attention_fp4 weights shared memory", e); return MSGL_CUDA_ERROR; }
-      if (dev >= 0 && dev < 64) weights_ready[dev] = true;
-    }
-    msgl_launch(fp4_weights_kernel<T, D, (NB > 1)>, dim3(sms * W::ctas), dim3(kWarps * 32), W::smem, stream, a);
-    MSGL_CHECK_LAUNCH("paged_attention_fp4 weights");
-  }
   return MSGL_OK;
 }
 
-int row_blocks(int d, int rows) { return rows <= 8 ? 1 : rows <= 16 || d == 256 ? 2 : 4; }
+// Blocks of 8 rows in a row tile: two, so that keys and values are widened once for 16 rows, where the registers have room.
+// B200, us: some 25 rows each of 3 requests of 5 to 9 thousand tokens, 32 heads of 128, with weights: four blocks (spilling) 154,
+// two 126; 16 heads a key head of 256, 20 requests of 2 to 6 thousand: two (spilling) 83, one 58.
+int row_blocks(int d, int rows) { return rows <= 8 || d == 256 ? 1 : 2; }
+
+template <typename T, int D, bool MANY> int launch_weights(const Fp4Args& a, int sms, cudaStream_t stream) {
+  using W = WeightsShape<D, MANY>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(fp4_weights_kernel<T, D, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::smem);
+    if (e != cudaSuccess) { msgl_set_error("paged_attention_fp4 weights shared memory", e); return MSGL_CUDA_ERROR; }
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  msgl_launch(fp4_weights_kernel<T, D, MANY>, dim3(sms * W::ctas), dim3(kWarps * 32), W::smem, stream, a);
+  MSGL_CHECK_LAUNCH("paged_attention_fp4 weights");
+  return MSGL_OK;
+}
 
 int device_sms() {
   static int sms[64] = {};
@@ -1153,16 +1197,18 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
     a.parts = ws; a.arrived = (int*)arrived;
     a.lse = weights != nullptr ? ws + parts_words(d, nb, workers) : nullptr;
     a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages; a.window = window;
-    a.row_tile = 8 * nb; a.row_shift = nb == 1 ? 3 : nb == 2 ? 4 : 5; a.workers = workers; a.scale = scale; a.status = status;
+    a.row_tile = 8 * nb; a.row_shift = nb == 1 ? 3 : 4; a.workers = workers; a.scale = scale; a.status = status;
     int rc = MSGL_BAD_ARG;
     const int sms = device_sms();
-#define RUN(T, D, N) rc = launch<T, D, N>(a, sms, stream)
-#define WIDTHS(T)                                                                                                          \
-  if (d == 64) { if (nb == 1) RUN(T, 64, 1); else if (nb == 2) RUN(T, 64, 2); else RUN(T, 64, 4); }                         \
-  else if (d == 128) { if (nb == 1) RUN(T, 128, 1); else if (nb == 2) RUN(T, 128, 2); else RUN(T, 128, 4); }                \
-  else { if (nb == 1) RUN(T, 256, 1); else RUN(T, 256, 2); }
-    if (dtype == MSGL_BF16) { WIDTHS(__nv_bfloat16) } else { WIDTHS(__half) }
-#undef WIDTHS
+    const bool many = max_q * (hq / hk) > 8;
+#define RUN(T, D)                                                                                                            \
+  do {                                                                                                                       \
+    rc = nb == 1 ? launch<T, D, 1>(a, stream) : launch<T, D, D == 256 ? 1 : 2>(a, stream);                                    \
+    if (rc == MSGL_OK && weights != nullptr)                                                                                 \
+      rc = many ? launch_weights<T, D, true>(a, sms, stream) : launch_weights<T, D, false>(a, sms, stream);                  \
+  } while (0)
+    if (dtype == MSGL_BF16) { if (d == 64) RUN(__nv_bfloat16, 64); else if (d == 128) RUN(__nv_bfloat16, 128); else RUN(__nv_bfloat16, 256); }
+    else { if (d == 64) RUN(__half, 64); else if (d == 128) RUN(__half, 128); else RUN(__half, 256); }
 #undef RUN
     if (rc != MSGL_OK) return rc;
   }

@@ -71,7 +71,9 @@ def attention(q, k, v, table, cu_q, lens, scale, window=0):
     """``(out, tolerance of out for one rounding of the probabilities to 11 bits and of out to q's type, weights of each token
     [request: [heads, tokens]], their tolerance)``. The tolerances follow the arithmetic: products of 4-bit keys and 16-bit
     queries are exact, D of them are summed in 32 bits (each addition off by at most 2^-23 of the sum of magnitudes), a score
-    that is off by d changes its weight by a share of 2 d, the exponential and the sums of weights add 2^-19."""
+    that is off by d changes its weight by a share of 2 d, the exponential and the sums of weights add 2^-19. Probabilities are
+    held in f16 after a factor of 2^7: those below 2^-14 / 2^7 of the largest are subnormal, in steps of 2^-24, so off by up to
+    2^-25 / 2^7 = 2^-32 of a sum of weights that is at least 1 (the largest is): 2^-32 times the magnitudes in sight."""
     t, hq, dim = q.shape
     hk, page = k.shape[1], k.shape[2]
     q = q.cpu()
@@ -98,6 +100,7 @@ def attention(q, k, v, table, cu_q, lens, scale, window=0):
         o = w @ vv.nan_to_num()
         out[cu[b]:cu[b + 1]] = o.transpose(0, 1)
         tol[cu[b]:cu[b + 1]] = (o.abs() * half_step + (share + 2.0 ** -11) * (w @ vv.nan_to_num().abs())
+                                + 2.0 ** -32 * ((~hidden).double() @ vv.nan_to_num().abs())
                                 + torch.finfo(torch.float16).tiny * (q.dtype == torch.float16)).transpose(0, 1) + 1e-12
         weights.append(w.unflatten(0, (hk, -1)).sum((1, 2)))
         weights_tol.append((w * share).unflatten(0, (hk, -1)).sum((1, 2)))
