@@ -24,6 +24,7 @@ class AttnMetadata:
     mask_swa: Optional[torch.Tensor] = None   # the mask sliding-window layers take instead (a mask replaces the window rule)
     workspace: Optional[torch.Tensor] = None
     prefill_plan: Optional[object] = None  # ops.cuda.PrefillPlan of a prefill-phase step on a GPU
+    fp4_plans: Optional[object] = None     # attention.paged.Fp4Plans of a prefill-phase step over a 4-bit pool
     layer_plans: Optional[object] = None   # the same for layers with reaches of their own, made when one asks for it
 
 

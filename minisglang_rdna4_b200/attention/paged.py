@@ -37,13 +37,28 @@ class LayerPlans:
         return self._plans[key]
 
 
+class Fp4Plans:
+    """Tables of the form for prompts over a 4-bit pool, one set per window of the step's layers."""
+
+    def __init__(self, cu_q, seq_lens) -> None:
+        self._lens, self._plans = (cu_q, seq_lens), {}
+
+    def of(self, q, cache, window: int):
+        from ..env import ENV
+
+        if window not in self._plans:
+            self._plans[window] = None if ENV.DISABLE_TC_PREFILL.value else ops.prefill_plan_fp4(q, cache, *self._lens, window)
+        return self._plans[window]
+
+
 class PagedAttentionBackend(BaseAttnBackend):
     def __init__(self, num_q_heads: int, num_kv_heads: int, head_dim: int, device,
-                 max_batch: int = 0, max_seq_len: int = 0, single_split: bool = False, heads=None, talk=None) -> None:
+                 max_batch: int = 0, max_seq_len: int = 0, single_split: bool = False, heads=None, talk=None, fp4: bool = False) -> None:
         """``heads``: ``(query heads, row width)`` per layer where layers differ; ``talk``: ``(query heads, key / value heads,
-        row width)`` of those whose heads mix their weights."""
+        row width)`` of those whose heads mix their weights; ``fp4``: the pool has 4 bits (``FP4KVCache``)."""
         self.hq, self.hk, self.d = num_q_heads, num_kv_heads, head_dim
         self.layered = bool(heads)
+        self.fp4 = fp4
         self.device = device
         # The number of KV splits of a decode step, and whether its tiles are dealt to the SMs instead, depend only on
         # the batch size and the longest sequence the pool can hold; the deal itself depends on the lengths of all
@@ -54,7 +69,12 @@ class PagedAttentionBackend(BaseAttnBackend):
         self.single_split = single_split
         self._workspace: Optional[torch.Tensor] = None
         self._talk_workspace: Optional[torch.Tensor] = None
-        if torch.device(device).type == "cuda":
+        if fp4 and torch.device(device).type == "cuda":
+            from ..ops.kv_fp4 import attention_fp4_workspace
+
+            words = max(attention_fp4_workspace(1, num_q_heads, num_kv_heads, head_dim, rows, False)[0] for rows in (1, 64))
+            self._workspace = torch.empty(words, dtype=torch.float32, device=device)
+        elif torch.device(device).type == "cuda":
             from ..ops import cuda as K
 
             hq, d = max(heads, key=lambda s: s[0] * (s[1] + 1)) if heads else (num_q_heads, head_dim)
@@ -71,8 +91,13 @@ class PagedAttentionBackend(BaseAttnBackend):
         step whatever its size, so that a row's result does not depend on how its prompt was chunked;
         a short extend over a long cached prefix reads the pool in place with the general kernel).
         Decode and verification steps stay on the general kernel."""
-        plan = layer_plans = None
-        if self.layered:
+        plan = layer_plans = fp4_plans = None
+        if self.fp4:
+            if mask is not None or not causal:
+                raise NotImplementedError("attention over a 4-bit K/V pool is causal and takes no mask")
+            if host_cu_q is not None and batch.is_prefill and not batch.spec_verify and self._workspace is not None:
+                fp4_plans = Fp4Plans(host_cu_q, host_seq_lens)
+        elif self.layered:
             if mask is not None or not causal:
                 raise NotImplementedError("layers with windows and chunks of their own take no attention mask")
             if host_cu_q is not None and batch.is_prefill and not batch.spec_verify and self._workspace is not None:
@@ -91,7 +116,7 @@ class PagedAttentionBackend(BaseAttnBackend):
             cu_q=cu_q, seq_lens=seq_lens, block_table=block_table, max_q=max_q, max_kv=max_kv,
             decode=(max_q == 1 and plan is None), causal=causal, mask=mask, mask_window=mask_window, mask_swa=mask_swa,
             workspace=self._workspace,
-            prefill_plan=plan, layer_plans=layer_plans,
+            prefill_plan=plan, layer_plans=layer_plans, fp4_plans=fp4_plans,
         )
 
     def forward_heads(self, q, layer: int, batch: Batch, *, scale: float, window: int = 0, chunk: int = 0,
@@ -134,6 +159,12 @@ class PagedAttentionBackend(BaseAttnBackend):
         # a sliding-window layer with a pool of its own reads that pool through the step's second block table
         pool = ctx.swa_kv_cache if swa else ctx.kv_cache
         block_table = batch.swa_block_table if swa else md.block_table
+        if self.fp4:
+            cache = pool.plane(layer)
+            plan = md.fp4_plans.of(q, cache, window) if md.fp4_plans is not None else None
+            return ops.paged_attention_fp4(q, cache, block_table, md.cu_q, md.seq_lens, scale, k_scale=pool.k_scale[layer],
+                                           v_scale=pool.v_scale[layer], window=window, max_q=md.max_q, max_kv=md.max_kv, plan=plan,
+                                           workspace=md.workspace)
         fp8 = getattr(pool, "fp8", False)
         if md.prefill_plan is not None and not window:
             from ..ops import cuda as K

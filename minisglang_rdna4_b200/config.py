@@ -35,7 +35,7 @@ class EngineConfig:
     moe_backend: str = "auto"
     model_source: str = "huggingface"
     cache_type: str = "radix"                # radix | naive
-    kv_cache_dtype: str = "auto"             # auto | bf16 | fp8
+    kv_cache_dtype: str = "auto"             # auto | bf16 | fp8 | nvfp4
     quantization: Optional[str] = None       # force a scheme for dummy weights: mxfp4|nvfp4|fp8|fp8_block|int4
     device: str = "auto"                     # auto | cuda | cpu
     seed: int = 0

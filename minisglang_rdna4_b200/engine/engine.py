@@ -23,7 +23,7 @@ from ..attention import create_attention_backend
 from ..config import EngineConfig
 from ..core import Batch, Context, set_global_ctx
 from ..env import ENV
-from ..kvcache import LayeredKVCache, MHAKVCache
+from ..kvcache import FP4KVCache, LayeredKVCache, MHAKVCache
 from ..models import create_model
 from ..models.config import NAMED_CONFIGS, ModelConfig
 from ..parallel import comm as comm_mod
@@ -217,6 +217,9 @@ class Engine:
             ENV.KV_FP8.value or (mc.quant is not None and mc.quant.kv_cache_fp8)))
         self.kv_calibrating = bool(ENV.KV_FP8_CALIBRATE.value)
         self.kv_fp8 = bool(kv_fp8) and not self.kv_calibrating
+        self.kv_fp4 = config.kv_cache_dtype == "nvfp4" and not self.kv_calibrating
+        if self.kv_fp4:
+            self._refuse_fp4_pool()
         # sliding-window layers in a pool of their own (MSGL_SWA_POOL): the layers are re-numbered per pool
         self.swa = None
         self.swa_kv_cache = None
@@ -308,6 +311,15 @@ class Engine:
                                            widths=mc.latent_widths)
         elif self._head_geometry:
             self.kv_cache = LayeredKVCache(self.num_pages, self.page_size, self._head_geometry, self.dtype, self.device)
+        elif self.kv_fp4:
+            self.kv_cache = FP4KVCache(self.kv_layers, self.num_pages, self.page_size, self.kv_heads_local, mc.head_dim,
+                                       self.dtype, self.device)
+            from ..kvcache.fp8_scales import resolve_kv_scales
+
+            ks, vs, source = resolve_kv_scales(config.model_path, self.kv_layers, mc.num_kv_heads, config.tp_rank, config.tp_size)
+            if source != "identity":               # descales of e4m3 are the largest magnitude over 448: over 2688 here
+                self.kv_cache.set_scales(ks / 6, vs / 6)
+            logger.info_rank0("factors of the 4-bit K/V heads: %s", source if source != "identity" else "default")
         else:
             self.kv_cache = MHAKVCache(
                 self.kv_layers, self.num_pages, self.page_size, self.kv_heads_local, mc.head_dim,
@@ -371,7 +383,7 @@ class Engine:
             max_batch=config.max_running_req, max_seq_len=self.max_seq_len,
             single_split=config.spec_algorithm != "none", latent=mc.latent_layers,
             heads=[(1 if m.talk else div_even(m.heads, config.tp_size), m.row_pad) for m in mc.head_layers],
-            talk=[(m.heads, m.kv_heads, m.row_pad) for m in mc.head_layers if m.talk],
+            talk=[(m.heads, m.kv_heads, m.row_pad) for m in mc.head_layers if m.talk], fp4=self.kv_fp4,
         )
         self.ctx.comm = comm_mod.get_comm()
         self._spec_exact = config.spec_algorithm != "none" and dev_kind == "cuda"
@@ -450,9 +462,30 @@ class Engine:
         logger.info_rank0(
             "engine ready: %s, %d pages x %d tokens, max_seq_len %d, dtype %s, kv %s",
             mc.model_type, self.num_pages, self.page_size, self.max_seq_len, self.dtype,
-            "fp8" if self.kv_fp8 else str(self.dtype))
+            "nvfp4" if self.kv_fp4 else "fp8" if self.kv_fp8 else str(self.dtype))
 
     # ------------------------------------------------------------------ boot helpers
+    def _refuse_fp4_pool(self) -> None:
+        """What a 4-bit K/V pool does not go with, named before anything is allocated."""
+        cfg, mc = self.config, self.model_config
+        why = None
+        if cfg.spec_algorithm != "none":
+            why = "speculative decoding (its verification rows have to come out as decode rows do)"
+        elif mc.latent_layers or mc.layered or mc.has_fp32_kernels or (ENV.MLA_LATENT.value and mc.is_mla):
+            why = f"the cache of {mc.model_type}"
+        elif mc.canvas_length:
+            why = "block diffusion (its attention is not causal)"
+        elif ENV.SWA_POOL.value and mc.swa_layers:
+            why = "a pool of their own for sliding-window layers (MSGL_SWA_POOL)"
+        elif mc.global_head_dim and len({mc.attn_geometry(i) for i in range(mc.num_kv_layers)}) > 1:
+            why = "layers whose heads differ"
+        elif mc.head_dim not in (64, 128, 256):
+            why = f"heads of {mc.head_dim} channels"
+        elif cfg.page_size % 16:
+            why = f"pages of {cfg.page_size} tokens (whole tiles of 16)"
+        if why:
+            raise ValueError(f"--kv-cache-dtype nvfp4 does not go with {why}")
+
     def _init_communication(self) -> None:
         cfg = self.config
         comm = comm_mod.reset_comm()
@@ -570,6 +603,8 @@ class Engine:
         itemsize = 1 if self.kv_fp8 else torch.empty((), dtype=self.dtype).element_size()
         per_page = MHAKVCache.token_bytes(self.kv_layers, self.kv_heads_local, mc.head_dim,
                                           itemsize) * self.page_size
+        if self.kv_fp4:
+            per_page = FP4KVCache.token_bytes(self.kv_layers, self.kv_heads_local, mc.head_dim) * self.page_size
         if self._main_geometry:
             per_page = MHAKVCache.token_bytes(self.kv_layers, 1, max(h * d for h, d in self._main_geometry),
                                               itemsize) * self.page_size

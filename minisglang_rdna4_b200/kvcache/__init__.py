@@ -4,6 +4,7 @@ from __future__ import annotations
 from .base import BaseCacheHandle, BaseKVCachePool, BasePrefixCache, SizeInfo
 from .naive_cache import NaivePrefixCache
 from .radix_cache import RadixPrefixCache, SnapshotRadixCache
+from .fp4_pool import FP4KVCache
 from .mha_pool import LayeredKVCache, MHAKVCache
 
 
@@ -26,6 +27,7 @@ __all__ = [
     "NaivePrefixCache",
     "RadixPrefixCache",
     "SnapshotRadixCache",
+    "FP4KVCache",
     "LayeredKVCache",
     "MHAKVCache",
     "create_prefix_cache",

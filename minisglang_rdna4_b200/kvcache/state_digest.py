@@ -45,6 +45,12 @@ def kv_digests(pool, pages: np.ndarray, length: int, name: str = "kv") -> Dict[K
     n_pages = (length + ps - 1) // ps
     idx = torch.as_tensor(np.asarray(pages[:n_pages], dtype=np.int64), device=pool.device)
     for layer in range(pool.num_layers):
+        if getattr(pool, "fp4", False):
+            slots = (idx[:, None] * ps + torch.arange(ps, device=idx.device)).flatten()[:length]
+            k, v = (pool.gather(layer, slots, which).reshape(length, -1) for which in (0, 1))
+            for seg, start in enumerate(range(0, length, SEG)):
+                out[(name, layer, seg)] = _sha(torch.stack([k[start:start + SEG], v[start:start + SEG]]))
+            continue
         # [pages, heads, page, dim] -> [positions, heads, dim]
         k = pool.k_cache(layer)[idx].permute(0, 2, 1, 3).reshape(n_pages * ps, -1)[:length]
         v = pool.v_cache(layer)[idx].permute(0, 2, 1, 3).reshape(n_pages * ps, -1)[:length]

@@ -2,7 +2,7 @@
 backend in the global context (python/minisgl/layers/attention.py:19-141)."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Dict, Optional
 
 import torch
 
@@ -12,6 +12,20 @@ from ..models.config import RotaryConfig
 from ..quant.method import ActQ, LinearInput
 from .base import BaseOP
 from .rotary import get_rope_cache
+
+
+_COUNTING: Dict[torch.device, torch.Tensor] = {}
+
+
+def _counting(n: int, device) -> torch.Tensor:
+    """``0 .. n - 1`` (int32), shared by all layers and steps."""
+    have = _COUNTING.get(device)
+    if have is None or have.numel() < n:
+        have = torch.arange(max(n, 16384), dtype=torch.int32, device=device)
+        if have.is_cuda and torch.cuda.is_current_stream_capturing():
+            return have[:n]                  # a graph's memory: not for the steps outside of it
+        _COUNTING[device] = have
+    return have[:n]
 
 
 class AttentionLayer(BaseOP):
@@ -50,6 +64,17 @@ class AttentionLayer(BaseOP):
         if self._kv_donor is not None:          # qkv holds the queries only
             q = ops.q_norm_rope(qkv, q_norm_w, batch.positions, self._cos_sin, self._hq, self._d,
                                 self._rotary.rotary_dim, self._eps, self._rotary.interleaved)
+            out = ctx.attn_backend.forward(q, layer, batch, scale=self._scale, window=self._window, swa=self._swa)
+            return out.reshape(out.shape[0], self._hq * self._d)
+        if getattr(pool, "fp4", False):
+            # normed and rotated into rows of the step first (a pool of one-token pages), then quantised
+            t = qkv.shape[0]
+            rows = torch.empty((2, t, self._hk, 1, self._d), dtype=qkv.dtype, device=qkv.device)
+            k, v = rows.unbind(0)
+            q = ops.qk_norm_rope_store(
+                qkv, q_norm_w, k_norm_w, batch.positions, self._cos_sin, self._hq, self._hk, self._d, self._rotary.rotary_dim,
+                self._eps, k, v, _counting(t, qkv.device), None, None, self._rotary.interleaved)
+            pool.store_kv(k.squeeze(2), v.squeeze(2), out_loc, layer)
             out = ctx.attn_backend.forward(q, layer, batch, scale=self._scale, window=self._window, swa=self._swa)
             return out.reshape(out.shape[0], self._hq * self._d)
         k_scale = pool.k_scale[layer] if pool.fp8 else None

@@ -166,7 +166,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, seq_lens, scale: flo
 
 # ---------------------------------------------------------------------------- K/V pool of 4 bits
 def store_kv_fp4(k, v, cache, out_loc, k_scale=None, v_scale=None, weights=None) -> None:
-    """Quantises rows ``k``, ``v [T, Hk, D]`` (bf16 or fp16, any row stride) and writes them to the token slots ``out_loc [T]``
+    """Quantises rows ``k``, ``v [T, Hk, D]`` (bf16 or fp16, on a CPU fp32 too; any row stride) and writes them to the token slots ``out_loc [T]``
     (int32) of a pool of 4 bits: ``cache [pages, Hk, page / 16, 18 D]`` bytes (D 64, 128 or 256).
 
     A value is an e2m1 code times an e4m3 scale of its 16 channels times the head's ``k_scale`` / ``v_scale [Hk]`` (fp32,
@@ -206,7 +206,7 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, 
                         max_q: int = 0, max_kv: int = 0, weights=None, plan=None, workspace=None):
     """Causal attention over a pool of 4 bits (``store_kv_fp4``): decode steps, prompts behind a prefix, rows that look back.
 
-    ``q [T, Hq, D]`` (bf16 or fp16); request b has the rows ``cu_q[b]:cu_q[b + 1]`` (int32), the last positions of its
+    ``q [T, Hq, D]`` (bf16 or fp16, on a CPU fp32 too); request b has the rows ``cu_q[b]:cu_q[b + 1]`` (int32), the last positions of its
     ``seq_lens[b]`` tokens, whose pages are ``block_table[b]`` (int32). ``window`` > 0: a row sees that many positions, its own
     included. A row that sees nothing gives zeros. ``max_q`` (rows of the longest request; 0: read from the device) may be
     larger than what the step has; ``max_kv`` likewise.
@@ -218,7 +218,7 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, 
     F4 = _fp4()
     shape = _, pages, hk, page, dim = F4.pool_shape(cache)
     F4.check_here(cache, q, block_table, cu_q, seq_lens, k_scale, v_scale, weights, workspace)
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dtype not in (torch.bfloat16, torch.float16) and (q.is_cuda or q.dtype is not torch.float32):
         raise TypeError(f"queries of bf16 or fp16, not {q.dtype}")
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % hk or q.shape[1] == 0:
         raise ValueError(f"q is [T, a multiple of {hk}, {dim}], not {tuple(q.shape)}")

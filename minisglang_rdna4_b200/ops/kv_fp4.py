@@ -89,7 +89,7 @@ def check_weights(weights: torch.Tensor, cache: torch.Tensor, pages: int, hk: in
 
 
 def check_rows(k: torch.Tensor, v: torch.Tensor, rows: int, hk: int, dim: int) -> None:
-    if k.dtype is not v.dtype or k.dtype not in _ROWS:
+    if k.dtype is not v.dtype or (k.dtype not in _ROWS and (k.is_cuda or k.dtype is not torch.float32)):
         raise TypeError(f"rows of bf16 or fp16, keys and values alike, not {k.dtype} and {v.dtype}")
     for x in (k, v):
         shape = x.shape

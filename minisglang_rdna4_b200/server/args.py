@@ -45,7 +45,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--gdn-radix", dest="gdn_radix", action="store_true", default=True)
     p.add_argument("--no-gdn-radix", dest="gdn_radix", action="store_false")
     p.add_argument("--moe-backend", default="auto")
-    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "bf16", "fp8"])
+    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "bf16", "fp8", "nvfp4"])
     p.add_argument("--quantization", default=None, choices=[None, "mxfp4", "nvfp4", "fp8", "fp8_block", "int4"])
     p.add_argument("--shell-mode", action="store_true")
     p.add_argument("--chat-template", default=None)

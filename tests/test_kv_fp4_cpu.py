@@ -137,7 +137,7 @@ def test_refusals():
         with pytest.raises((TypeError, ValueError)):
             ops.load_kv_fp4(**{**dict(cache=cache, slots=loc), **kw})
     good = dict(q=q, cache=cache, block_table=table, cu_q=cu, seq_lens=lens, scale=1.0)
-    for kw in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[:, :0]), dict(block_table=table.long()),
+    for kw in (dict(q=q.double()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[:, :0]), dict(block_table=table.long()),
                dict(block_table=table[:1]), dict(cu_q=cu[:2]), dict(seq_lens=lens.long()), dict(window=-1), dict(max_q=-1),
                dict(weights=weights[:, :1]), dict(weights=weights, plan=object()), dict(k_scale=ks[:1]), dict(v_scale=vs.half())):
         with pytest.raises((TypeError, ValueError)):
@@ -171,3 +171,69 @@ def test_a_conversation_is_stored_weighed_and_cut():
         at = kept[0, h // 2].long().tolist() + [n]
         w = torch.softmax(q[n, h].double() @ kk[at, h // 2].T * 0.125, -1)
         assert (out[0, h].double() - w @ vv[at, h // 2]).abs().max() < 2.0 ** -7
+
+
+def _config(**kw):
+    from minisglang_rdna4_b200.models.config import ModelConfig
+
+    d = dict(model_type="qwen3", hidden_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+             intermediate_size=256, vocab_size=512, max_position_embeddings=1024, rms_norm_eps=1e-6, rope_theta=10000.0,
+             tie_word_embeddings=True, architectures=["Qwen3ForCausalLM"])
+    return ModelConfig.from_hf({**d, **kw})
+
+
+def _engine(**kw):
+    from minisglang_rdna4_b200.llm import LLM
+
+    return LLM(**{**dict(model_config=_config(), use_dummy_weight=True, kv_cache_dtype="nvfp4", device="cpu", page_size=16,
+                         max_running_req=4, num_page_override=64, seed=0), **kw})
+
+
+def test_engine_serves_from_a_pool_of_4_bits():
+    from minisglang_rdna4_b200 import SamplingParams
+    from minisglang_rdna4_b200.kvcache import FP4KVCache
+
+    llm = _engine()
+    pool = llm.engine.kv_cache
+    assert isinstance(pool, FP4KVCache) and pool.bytes_per_token == 2 * 2 * 72
+    sp = SamplingParams(temperature=0.0, max_tokens=5, ignore_eos=True)
+    prompts = [list(range(3, 60)), [7, 8, 9]]
+    first = [o.token_ids for o in llm.generate(prompts, sp)]
+    again = [o.token_ids for o in llm.generate(prompts, sp)]          # from the prefix cache
+    assert first == again and all(len(t) == 5 for t in first)
+    assert (pool._buf[:, :-1] != 0).any()
+    llm.cache.check_integrity()
+    llm.shutdown()
+
+
+@pytest.mark.parametrize("kw", [dict(page_size=8), dict(spec_algorithm="ngram"), dict(model_config="wide")])
+def test_engine_names_what_the_pool_does_not_go_with(kw):
+    if kw.get("model_config"):
+        kw = dict(model_config=_config(head_dim=32))
+    with pytest.raises(ValueError, match="nvfp4"):
+        _engine(**kw)
+
+
+def test_pool():
+    from minisglang_rdna4_b200.kvcache import FP4KVCache
+
+    pool = FP4KVCache(3, 6, 16, 2, 64, torch.bfloat16, "cpu", weights=True)
+    k, v = (torch.randn(20, 2, 64).bfloat16() for _ in range(2))
+    loc = torch.arange(3, 23, dtype=torch.int32)
+    pool.store_kv(k, v, loc, 1)
+    for which, x in ((0, k), (1, v)):
+        want = plain.rounded(x, pool.k_scale[1])
+        assert torch.equal(pool.gather(1, loc, which).double(), want.bfloat16().double())
+        assert (pool.gather(0, loc, which) == 0).all()
+    pool.weights[:, :, :, :] = torch.rand(pool.weights.shape)
+    kept, lens = pool.evict(ints([[0, 1]]), ints([23]), ints([[4]]), 10, 3, 1)
+    assert kept.shape == (3, 1, 2, 10) and lens.tolist() == [10]
+    assert torch.equal(pool.gather(1, ints([64 + 9]), 0), pool.gather(1, ints([22]), 0))
+    for bad in (dict(head_dim=96), dict(page_size=24)):
+        with pytest.raises(ValueError):
+            FP4KVCache(**{**dict(num_layers=1, num_pages=2, page_size=16, num_kv_heads=1, head_dim=64, dtype=torch.bfloat16,
+                                 device="cpu"), **bad})
+    with pytest.raises(ValueError):
+        FP4KVCache(1, 2, 16, 1, 64, torch.bfloat16, "cpu").evict(ints([[0]]), ints([5]), ints([[1]]), 4, 1)
+    with pytest.raises(NotImplementedError):
+        pool.k_cache(0)
