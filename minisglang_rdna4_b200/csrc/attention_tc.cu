@@ -1153,8 +1153,8 @@ MSGL_API int msgl_attn_prefill_tc(const void* q, long long q_row_stride, void* o
     return MSGL_BAD_ARG;
   }
   const bool ext = d != kD || window > 0 || chunk > 0 || softcap > 0.f || gate != nullptr;
-  if ((ext || pos_form) && (dtype != MSGL_BF16 || kv_fp8 == 1)) {
-    msgl_set_error_text("prefill attention: reaches, soft caps, gates, rows of 64 and unpaired query heads need bf16");
+  if ((ext || pos_form) && (kv_fp8 == 1 || (dtype != MSGL_BF16 && (kv_fp8 != 2 || softcap > 0.f)))) {
+    msgl_set_error_text("prefill attention: reaches, soft caps, gates, rows of 64 and unpaired query heads need bf16, or without caps rows of a 4-bit pool");
     return MSGL_BAD_ARG;
   }
   if (hq % hk || (!pos_form && bias == nullptr && (hq / hk) % 2) || (d != 64 && d != 128) || scale <= 0.f || (gate != nullptr && ldg % 8) ||
@@ -1235,6 +1235,9 @@ MSGL_API int msgl_attn_prefill_tc(const void* q, long long q_row_stride, void* o
     return MSGL_OK;
   }
   const bool fixcap = softcap > 0.f && softcap * kLog2eTc <= kFixedCap && dtype == MSGL_BF16;
+  if (dtype == MSGL_F16 && (ext || pos_form))
+    return pos_form ? launch_tc<__half, true, TC_EXTENDED>(mq, mk, mv, mg, a, stream)
+                    : launch_tc<__half, false, TC_EXTENDED>(mq, mk, mv, mg, a, stream);
   if (pos_form) {
     return fixcap ? launch_tc<__nv_bfloat16, true, TC_FIXED_CAP>(mq, mk, mv, mg, a, stream)
                   : launch_tc<__nv_bfloat16, true, TC_EXTENDED>(mq, mk, mv, mg, a, stream);

@@ -204,11 +204,10 @@ class PromptPlan(K.PrefillPlan):
 
 
 def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
-    """The tcgen05 form of prompts: heads of 128 channels in pairs that share a key head, any types of 16 bits; for bf16 also of
-    64 channels, unpaired heads and windows."""
+    """The tcgen05 form of prompts: heads of 64 or 128 channels."""
     hk, dim = cache.shape[1], cache.shape[3] // 18
     group = q.shape[1] // hk
-    if dim == 256 or (q.dtype != torch.bfloat16 and (dim != 128 or group % 2 or window > 0)):
+    if dim == 256:
         return None
     cu_q, seq_lens = (np.minimum(np.asarray(x, dtype=np.int64), 1 << 30) for x in (cu_q, seq_lens))
     b = seq_lens.size

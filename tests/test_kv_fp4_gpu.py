@@ -185,7 +185,8 @@ def test_rows(dim, hq, hk, weighed):
 
 
 PROMPTS = [(8, 2, 128, torch.bfloat16, 0), (8, 2, 128, torch.float16, 0), (7, 1, 128, torch.bfloat16, 0), (6, 6, 64, torch.bfloat16, 0),
-           (8, 4, 64, torch.bfloat16, 0), (8, 2, 128, torch.bfloat16, 100), (5, 1, 64, torch.bfloat16, 300)]
+           (8, 4, 64, torch.bfloat16, 0), (8, 2, 128, torch.bfloat16, 100), (5, 1, 64, torch.bfloat16, 300),
+           (7, 1, 128, torch.float16, 0), (6, 6, 64, torch.float16, 0), (8, 4, 64, torch.float16, 40), (8, 2, 128, torch.float16, 100)]
 
 
 @pytest.mark.parametrize("hq,hk,dim,dtype,window", PROMPTS, ids=["-".join(map(str, p)) for p in PROMPTS])
@@ -225,7 +226,6 @@ def test_steps_that_take_no_prompt_form():
     assert ops.prefill_plan_fp4(q, cache, n(0, 200), n(100)) is None              # more rows than tokens
     assert ops.prefill_plan_fp4(q[:20], cache, n(0, 20), n(50000)) is None        # few rows for the keys
     assert ops.prefill_plan_fp4(q[:0], cache, n(0), n()) is None
-    assert ops.prefill_plan_fp4(q.half(), cache, n(0, 200), n(200), 64) is None
     wide = torch.zeros(4, 2, 1, 18 * 256, dtype=torch.uint8, device="cuda")
     assert ops.prefill_plan_fp4(torch.zeros(200, 4, 256, device="cuda").half(), wide, n(0, 200), n(200)) is None
 
