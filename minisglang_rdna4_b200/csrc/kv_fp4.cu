@@ -21,22 +21,21 @@ struct RowArgs {
   long long slots;
 };
 
-// A thread has 8 channels of a key or value (a 16-byte access; D / 4 threads for a row and head, the key's first) in U rows that
-// follow each other, so that their loads are under way at once: four where the rows fill the GPU twice all the same, else one.
-// B200, us, store + load of 8192 rows, 8 heads of 128: one row 31.7, four 23.6; 64 rows: 6.2, four 8.9.
+// A thread has 8 channels of a key and of its value (16-byte accesses; D / 8 threads for a row and head) in U rows that follow
+// each other, so that their loads are under way at once: four where the rows fill the GPU all the same, else one.
 template <int D, int U> struct Place {
   int h, c, row0;           // c: channels 8 c .. 8 c + 7
-  int code_at, sf_at;       // the channels' part of where they lie in a tile
-  bool val;
+  int code_at[2], sf_at[2]; // the channels' part of where they lie in a tile, of keys and of values
   __device__ __forceinline__ Place(const RowArgs& a) {
-    const uint32_t id = blockIdx.x * 256 + threadIdx.x, items = (D / 4) * a.hk;
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, items = (D / 8) * a.hk;
     const uint32_t row = id / items, item = id - row * items;
     row0 = (int)row * U;
     c = (int)(item % (D / 8));
-    val = item / (D / 8) & 1;
-    h = (int)(item / (D / 4));
-    code_at = val ? v_channel<D>(8 * c) : k_channel<D>(8 * c);
-    sf_at = val ? v_sf_byte<D>(0, c / 2) : k_sf_block<D>(c / 2);
+    h = (int)(item / (D / 8));
+    code_at[0] = k_channel<D>(8 * c);
+    code_at[1] = v_channel<D>(8 * c);
+    sf_at[0] = k_sf_block<D>(c / 2);
+    sf_at[1] = v_sf_byte<D>(0, c / 2);
   }
 };
 // Tile of a slot, the slot's place in an [pages, hk, page] array, and its token in the tile.
@@ -84,80 +83,91 @@ template <typename T> __device__ __forceinline__ uint32_t quantise8(const Vec8<T
   return w;
 }
 
-// Bound: the 16 bytes in and 4.5 out of a thread and row.
+// Bound: the 32 bytes in and 9 out of a thread and row.
 template <typename T, int D, int U> __global__ void __launch_bounds__(256) store_fp4_kernel(const RowArgs a) {
   const Place<D, U> p(a);
   pdl_enter();
-  const T* src = reinterpret_cast<const T*>(p.val ? a.v : a.k) + p.h * D + p.c * 8;
-  const long long ld = p.val ? a.ldv : a.ldk;
-  const float* heads = p.val ? a.v_head : a.k_head;
-  const float head = heads != nullptr && p.row0 < a.rows ? heads[p.h] : 1.f;
-  Vec8<T> raw[U];
+  const bool any = p.row0 < a.rows;
+  Vec8<T> raw[U][2];
   int loc[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
+    const int row = p.row0 + u;
     loc[u] = -1;
-    if (p.row0 + u < a.rows) {
-      loc[u] = a.loc[p.row0 + u];
+    if (row < a.rows) {
+      loc[u] = a.loc[row];
       (void)MSGL_OOB(loc[u], a.slots);
-      raw[u] = *reinterpret_cast<const Vec8<T>*>(src + (p.row0 + u) * ld);
-    } else {
-      *reinterpret_cast<uint4*>(&raw[u]) = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      *reinterpret_cast<uint4*>(&raw[u][w]) = make_uint4(0, 0, 0, 0);
+      if (row < a.rows)
+        raw[u][w] = *reinterpret_cast<const Vec8<T>*>(reinterpret_cast<const T*>(w ? a.v : a.k) + row * (w ? a.ldv : a.ldk) + p.h * D + p.c * 8);
     }
   }
+  const float head[2] = {any && a.k_head != nullptr ? a.k_head[p.h] : 1.f, any && a.v_head != nullptr ? a.v_head[p.h] : 1.f};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    uint8_t sf;
-    const uint32_t code = quantise8<T>(raw[u], head, sf);
+    uint32_t code[2];
+    uint8_t sf[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) code[w] = quantise8<T>(raw[u][w], head[w], sf[w]);
     if (loc[u] < 0 || loc[u] >= a.slots) continue;
     int t;
     long long at;
     uint8_t* tile = tile_of<D>(a, loc[u], p.h, t, at);
-    *reinterpret_cast<uint32_t*>(tile + p.code_at + (p.val ? v_token<D>(t) : k_token<D>(t))) = code;
-    if (!(p.c & 1)) tile[p.sf_at + (p.val ? t : k_sf_token<D>(t))] = sf;
-    if (!p.val && p.c == 0 && a.weights != nullptr) a.weights[at] = 0.f;
+    *reinterpret_cast<uint32_t*>(tile + p.code_at[0] + k_token<D>(t)) = code[0];
+    *reinterpret_cast<uint32_t*>(tile + p.code_at[1] + v_token<D>(t)) = code[1];
+    if (!(p.c & 1)) {
+      tile[p.sf_at[0] + k_sf_token<D>(t)] = sf[0];
+      tile[p.sf_at[1] + t] = sf[1];
+    }
+    if (p.c == 0 && a.weights != nullptr) a.weights[at] = 0.f;
   }
 }
 
 // The inverse; code * scale is exact, the head's factor is applied in fp32 ahead of it. A slot outside the pool gives zeros.
-// Bound: the 16 bytes that a thread writes for a row. blockIdx.y: layer.
+// Bound: the 32 bytes that a thread writes for a row. blockIdx.y: layer.
 template <typename T, int D, int U> __global__ void __launch_bounds__(256) load_fp4_kernel(const RowArgs a) {
   const Place<D, U> p(a);
   pdl_enter();
   if (p.row0 >= a.rows) return;
-  const float* heads = p.val ? a.v_head : a.k_head;
-  const float head = heads != nullptr ? heads[p.h] : 1.f;
+  const float head[2] = {a.k_head != nullptr ? a.k_head[p.h] : 1.f, a.v_head != nullptr ? a.v_head[p.h] : 1.f};
   const long long layer = (long long)blockIdx.y * a.layer_bytes;
-  uint32_t code[U];
-  uint8_t sf[U];
+  uint32_t code[U][2];
+  uint8_t sf[U][2];
   int loc[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) loc[u] = a.loc[min(p.row0 + u, a.rows - 1)];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    code[u] = 0;
-    sf[u] = 0;
+    code[u][0] = code[u][1] = 0;
+    sf[u][0] = sf[u][1] = 0;
     (void)MSGL_OOB(loc[u], a.slots);
     if (loc[u] < 0 || loc[u] >= a.slots) continue;
     int t;
     long long at;
     const uint8_t* tile = tile_of<D>(a, loc[u], p.h, t, at) + layer;
-    code[u] = *reinterpret_cast<const uint32_t*>(tile + p.code_at + (p.val ? v_token<D>(t) : k_token<D>(t)));
-    sf[u] = tile[p.sf_at + (p.val ? t : k_sf_token<D>(t))];
+    code[u][0] = *reinterpret_cast<const uint32_t*>(tile + p.code_at[0] + k_token<D>(t));
+    code[u][1] = *reinterpret_cast<const uint32_t*>(tile + p.code_at[1] + v_token<D>(t));
+    sf[u][0] = tile[p.sf_at[0] + k_sf_token<D>(t)];
+    sf[u][1] = tile[p.sf_at[1] + t];
   }
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.val ? a.v : a.k)) +
-           (((long long)blockIdx.y * a.rows + p.row0) * a.hk + p.h) * D + p.c * 8;
+  const long long to = (((long long)blockIdx.y * a.rows + p.row0) * a.hk + p.h) * D + p.c * 8;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (p.row0 + u >= a.rows) break;
-    const float s = e4m3_to_float(sf[u]) * head;
-    Vec8<T> y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = decode2(code[u] >> (8 * i));
-      y.v[i] = Pack2<T>::make(x.x * s, x.y * s);
+    for (int w = 0; w < 2; ++w) {
+      const float s = e4m3_to_float(sf[u][w]) * head[w];
+      Vec8<T> y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = decode2(code[u][w] >> (8 * i));
+        y.v[i] = Pack2<T>::make(x.x * s, x.y * s);
+      }
+      *reinterpret_cast<Vec8<T>*>(reinterpret_cast<T*>(const_cast<void*>(w ? a.v : a.k)) + to + (long long)u * a.hk * D) = y;
     }
-    *reinterpret_cast<Vec8<T>*>(dst + (long long)u * a.hk * D) = y;
   }
 }
 
@@ -425,7 +435,7 @@ bool shape_ok(int hk, int d, int page_size, long long pages, const void* pool, c
 }
 
 uint32_t magic(int per) { return (uint32_t)(((1ull << 32) + per - 1) / per); }
-int rows_of_a_thread(long long rows, int hk, int d) { return rows * hk * (d / 4) > 148ll * 2048 * 4 ? 4 : 1; }
+int rows_of_a_thread(long long rows, int hk, int d) { return rows * hk * (d / 8) > 148ll * 2048 * 2 ? 4 : 1; }
 
 }  // namespace
 
@@ -442,7 +452,7 @@ MSGL_API int msgl_store_fp4(const void* k, const void* v, long long ldk, long lo
   RowArgs a{k, v, ldk, ldv, (uint8_t*)pool, 0, (const int32_t*)loc, (const float*)k_head, (const float*)v_head, (float*)weights,
             rows, hk, page_size / kTile, magic(page_size / kTile), pages * page_size};
   const int u = rows_of_a_thread(rows, hk, d);
-  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 4);
+  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 8);
   if (threads > 0x7fffff00ll) {
     msgl_set_error_text("store_kv_fp4: more rows than a launch has threads for");
     return MSGL_BAD_ARG;
@@ -470,7 +480,7 @@ MSGL_API int msgl_load_fp4(const void* pool, long long layer_bytes, int layers, 
   RowArgs a{k, v, 0, 0, (uint8_t*)const_cast<void*>(pool), layer_bytes, (const int32_t*)loc, (const float*)k_head,
             (const float*)v_head, nullptr, rows, hk, page_size / kTile, magic(page_size / kTile), pages * page_size};
   const int u = rows_of_a_thread((long long)rows * layers, hk, d);
-  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 4);
+  const long long threads = (long long)((rows + u - 1) / u) * hk * (d / 8);
   if (threads > 0x7fffff00ll || layers > 65535) {
     msgl_set_error_text("load_kv_fp4: more rows than a launch has threads for");
     return MSGL_BAD_ARG;
