@@ -924,17 +924,23 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     if (fetched < count) fetch();
     __syncwarp();
   };
-  // weights that the two rows 2 j, 2 j + 1 of a block give tokens of rows g and g + 8
-  auto given = [&](const Request& r, int row0, int tok0, const float (&s)[4], float cA, float cB, float eA, float eB, float& s0, float& s1) {
-    const int posA = r.n - r.q_len + (row0 + 2 * j) / a.group, posB = r.n - r.q_len + (row0 + 2 * j + 1) / a.group;
+  // weights that the two rows 2 j, 2 j + 1 of a block give tokens of rows g and g + 8. A row that is not there has an infinite
+  // log of its sum.
+  auto given = [&](const Request& r, int row0, int tok0, const float (&s)[4], float2 c, float2 e, float& s0, float& s1) {
+    const float2 minus = make_float2(-e.x, -e.y);
+    float2 p0 = fma2(make_float2(s[0], s[1]), c, minus), p1 = fma2(make_float2(s[2], s[3]), c, minus);
+    const int ahead = r.n - r.q_len;                       // position of the first row
+    if (tok0 + kTile - 1 > ahead || (a.window > 0 && tok0 <= r.n - 1 - a.window)) {     // else all rows see all tokens
+      const int posA = ahead + (row0 + 2 * j) / a.group, posB = ahead + (row0 + 2 * j + 1) / a.group;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = tok0 + token_of(g, i >> 1), pos = i & 1 ? posB : posA;
-      const float c = i & 1 ? cB : cA, e = i & 1 ? eB : eA;
-      const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
-      const float p = seen && e != INFINITY ? exp2_fast(s[i] * c - e) : 0.f;
-      if (i < 2) s0 += p; else s1 += p;
+      for (int i = 0; i < 4; ++i) {
+        const int tok = tok0 + token_of(g, i >> 1), pos = i & 1 ? posB : posA;
+        const bool seen = tok <= min(pos, r.n - 1) && !(a.window > 0 && tok <= pos - a.window);
+        if (!seen) (i < 2 ? (i & 1 ? p0.y : p0.x) : (i & 1 ? p1.y : p1.x)) = -INFINITY;
+      }
     }
+    s0 += exp2_fast(p0.x) + exp2_fast(p0.y);
+    s1 += exp2_fast(p1.x) + exp2_fast(p1.y);
   };
   auto give = [&](const Request& r, int tok0, float s0, float s1) {
 #pragma unroll
@@ -957,25 +963,24 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     for (int s = 0; s < min(STAGES, count); ++s) fetch();
     __syncwarp();
     uint32_t qf[D / 8];
-    float cA = 0.f, cB = 0.f, eA = 0.f, eB = 0.f;
+    float2 c = {}, e = {};
     bool fresh = true;
     while (done < count) {
       if (fresh) {
         const float back = load_query<T, D>(a, get.r, get.head, g, lane, qf);
         const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[get.head] : 1.f);
-        cA = kh * __shfl_sync(0xffffffffu, back, 8 * j);
-        cB = kh * __shfl_sync(0xffffffffu, back, 8 * j + 4);
-        eA = lse_of(get.r, get.head, 2 * j);
-        eB = lse_of(get.r, get.head, 2 * j + 1);
+        c = make_float2(kh * __shfl_sync(0xffffffffu, back, 8 * j), kh * __shfl_sync(0xffffffffu, back, 8 * j + 4));
+        e = make_float2(lse_of(get.r, get.head, 2 * j), lse_of(get.r, get.head, 2 * j + 1));
       }
       next_keys();
       if (!ok) break;
-      float s[4] = {};
+      float s[4];
+      mma_first(s, k[0][0], k[0][1], k[0][2], k[0][3], qf[0], qf[1]);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
+      for (int i = 1; i < D / 16; ++i) mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
       const int tok0 = (get.r.tile0 + get.tile) * kTile;
       float s0 = 0.f, s1 = 0.f;
-      given(get.r, 0, tok0, s, cA, cB, eA, eB, s0, s1);
+      given(get.r, 0, tok0, s, c, e, s0, s1);
       give(get.r, tok0, s0, s1);
       if (done < count) fresh = get.next(a, line, true);
     }
@@ -1010,15 +1015,16 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
           if (!ok) break;
           float s0 = 0.f, s1 = 0.f;
           for (int nb = 0; nb < blocks; ++nb) {
-            float s[4] = {};
+            float s[4];
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
               const uint4 q = queries[(nb * (D / 32) + i) * 32 + lane];
-              mma(s, k[2 * i][0], k[2 * i][1], k[2 * i][2], k[2 * i][3], q.x, q.y);
+              if (i == 0) mma_first(s, k[0][0], k[0][1], k[0][2], k[0][3], q.x, q.y);
+              else mma(s, k[2 * i][0], k[2 * i][1], k[2 * i][2], k[2 * i][3], q.x, q.y);
               mma(s, k[2 * i + 1][0], k[2 * i + 1][1], k[2 * i + 1][2], k[2 * i + 1][3], q.z, q.w);
             }
             const float4 c = *reinterpret_cast<const float4*>(rowc + nb * 8 + 2 * j);
-            given(r, row0 + nb * 8, tok0, s, c.x, c.z, c.y, c.w, s0, s1);
+            given(r, row0 + nb * 8, tok0, s, make_float2(c.x, c.z), make_float2(c.y, c.w), s0, s1);
           }
           give(r, tok0, s0, s1);
         }
