@@ -824,7 +824,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
 
 // What the rows give every token: the keys once more, with the rows' final maxima and sums. A tile's keys go through all rows of
 // their (request, key head) pair, so a token's sum is taken by one lane in one order. MANY false: up to 8 rows, in registers;
-// warps deal out the tiles of all pairs. MANY: CTAs do; the pair's queries lie in shared memory, kChunk blocks of 8 rows at
+// warps deal out the tiles of all pairs (should a request have more rows than the caller said, its row tiles follow each other and
+// add to a token in any order). MANY: CTAs do; the pair's queries lie in shared memory, kChunk blocks of 8 rows at
 // a time, and the warps take the CTA's tiles in turn. A warp has four tiles' keys under way.
 template <int D, bool MANY> struct WeightsShape {
   static constexpr int stages = 4, key_bytes = 9 * D;                  // codes and scales
@@ -873,7 +874,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     fence_barrier_init();
   }
   pdl_wait();
-  lay_line(a, line, true, 0);
+  lay_line(a, line, MANY, 0);
   const Deal deal(line.first[a.B], MANY ? gridDim.x : gridDim.x * kWarps, MANY ? 8 : 4);
   const int worker = MANY ? blockIdx.x : warp * gridDim.x + blockIdx.x;
   if (worker >= deal.workers) return;
@@ -888,7 +889,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
   auto fetch = [&]() {
     if (fetched % 32 == 0) {
       Walk w;
-      w.seek(a, line, first + (long long)min(fetched + lane, count - 1) * step, true);
+      w.seek(a, line, first + (long long)min(fetched + lane, count - 1) * step, MANY);
       mine = (w.page(a) * a.hk + w.head) * a.per + w.sub;
     }
     if (lane == fetched % 32) {
@@ -957,7 +958,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     return a.lse[(long long)(r.q0 + qi) * a.hq + head * a.group + row - qi * a.group];
   };
   Walk get;
-  get.seek(a, line, at, true);
+  get.seek(a, line, at, MANY);
   if constexpr (!MANY) {
     count = (int)(end - at);
     for (int s = 0; s < min(STAGES, count); ++s) fetch();
@@ -967,10 +968,10 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
     bool fresh = true;
     while (done < count) {
       if (fresh) {
-        const float back = load_query<T, D>(a, get.r, get.head, g, lane, qf);
+        const float back = load_query<T, D>(a, get.r, get.head, 8 * get.rt + g, lane, qf);
         const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[get.head] : 1.f);
         c = make_float2(kh * __shfl_sync(0xffffffffu, back, 8 * j), kh * __shfl_sync(0xffffffffu, back, 8 * j + 4));
-        e = make_float2(lse_of(get.r, get.head, 2 * j), lse_of(get.r, get.head, 2 * j + 1));
+        e = make_float2(lse_of(get.r, get.head, 8 * get.rt + 2 * j), lse_of(get.r, get.head, 8 * get.rt + 2 * j + 1));
       }
       next_keys();
       if (!ok) break;
@@ -980,9 +981,9 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
       for (int i = 1; i < D / 16; ++i) mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
       const int tok0 = (get.r.tile0 + get.tile) * kTile;
       float s0 = 0.f, s1 = 0.f;
-      given(get.r, 0, tok0, s, c, e, s0, s1);
+      given(get.r, 8 * get.rt, tok0, s, c, e, s0, s1);
       give(get.r, tok0, s0, s1);
-      if (done < count) fresh = get.next(a, line, true);
+      if (done < count) fresh = get.next(a, line, false);
     }
   } else {
     uint4* queries = reinterpret_cast<uint4*>(smem + S::queries);      // [block][D / 32 pieces of 16 bytes][lane]

@@ -228,6 +228,7 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, 
     F4.check_heads(k_scale, v_scale, hk)
     if window < 0 or max_q < 0 or max_kv < 0 or block_table.shape[1] == 0:
         raise ValueError("window, max_q and max_kv are not negative, and a request has a page in its table")
+    window = min(window, 1 << 30)          # more than any request has
     if workspace is not None and (workspace.dtype is not torch.float32 or not workspace.is_contiguous()):
         raise ValueError("a workspace is contiguous fp32")
     if weights is not None:
@@ -246,6 +247,7 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window: int = 0):
     shapes that it does not have)."""
     F4 = _fp4()
     F4.pool_shape(cache)
+    window = min(window, 1 << 30)
     return F4.prefill_plan_fp4(q, cache, cu_q, seq_lens, window) if cache.is_cuda else None
 
 

@@ -93,7 +93,7 @@ def attention(q, k, v, table, cu_q, lens, scale, window=0):
         if window:
             hidden = hidden | (i <= p - window)
         s = (qq @ kk.nan_to_num().transpose(1, 2) * scale).masked_fill(hidden, -math.inf)
-        size = (qq.abs() @ kk.nan_to_num().abs().transpose(1, 2) * scale).masked_fill(hidden, 0.0)
+        size = (qq.abs() @ kk.nan_to_num().abs().transpose(1, 2) * abs(scale)).masked_fill(hidden, 0.0)
         off = dim * 2.0 ** -23 * (size.amax(-1, keepdim=True) if n else torch.zeros(hq, m, 1))
         w = torch.softmax(s, -1).masked_fill(hidden, 0.0)
         share = 2 * off + 2.0 ** -19

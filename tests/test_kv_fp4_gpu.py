@@ -216,6 +216,8 @@ def test_prompts(hq, hk, dim, dtype, window):
     assert ((out.cpu().double() - want).abs() <= tol).all(), float(((out.cpu().double() - want).abs() / tol).max())
     with pytest.raises(ValueError):
         ops.paged_attention_fp4(q, cache, table, cu, ints(lens), 0.1, window=window + 1, max_q=300, plan=plan)
+    with pytest.raises(ValueError):
+        ops.paged_attention_fp4(q, cache, table, cu, ints(lens), -0.1, window=window, max_q=300, plan=plan)
 
 
 def test_steps_that_take_no_prompt_form():
@@ -239,6 +241,21 @@ def test_bounds_may_be_loose_or_read_from_the_device():
     for kw in (dict(max_q=9, max_kv=4096), dict(max_q=0, max_kv=0)):
         attend([70, 200], [1, 4], 8, 2, 128, weighed=True, **kw)
     attend([70, 200], [1, 1], 8, 2, 128, weighed=True, max_q=0, max_kv=1 << 20)
+
+
+def test_more_rows_than_said_and_windows_without_an_end():
+    attend([70, 200, 33], [3, 9, 33], 8, 2, 128, weighed=True, max_q=1)
+    attend([70, 200], [1, 4], 8, 2, 64, weighed=True, window=(1 << 40) + 1)
+
+
+def test_more_requests_than_a_launch_takes():
+    lens = [(29 * i) % 70 for i in range(700)]
+    attend(lens, [1] * 700, 4, 2, 64, weighed=True)
+    attend([n + 3 for n in lens], [(7 * i) % 4 for i in range(700)], 4, 2, 64, weighed=True)
+
+
+def test_a_scale_below_zero():
+    attend([70, 200], [1, 4], 8, 2, 128, weighed=True, scale=-0.1)
 
 
 def test_large_scores():
