@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
       const float kh = fabsf(a.scale) * kLog2e * (a.k_head != nullptr ? a.k_head[head] : 1.f);
       for (int row0 = 0; row0 < rows; row0 += 8 * S::chunk) {
         __syncthreads();                                               // the last chunk has been used
-        const int blocks = min(S::chunk, (rows - row0 + 7) / 8);
+        const int blocks = min(S::chunk, (rows - row0 + 15) / 16 * 2);   // an even number: rows that are not there weigh nothing
         for (int nb = warp; nb < blocks; nb += kWarps) {
           uint32_t qf[D / 8];
           const float back = load_query<T, D>(a, r, head, row0 + nb * 8 + g, lane, qf);
@@ -1015,17 +1015,23 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
           next_keys();
           if (!ok) break;
           float s0 = 0.f, s1 = 0.f;
-          for (int nb = 0; nb < blocks; ++nb) {
-            float s[4];
+          for (int nb = 0; nb < blocks; nb += 2) {         // two chains of products side by side
+            float s[2][4];
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-              const uint4 q = queries[(nb * (D / 32) + i) * 32 + lane];
-              if (i == 0) mma_first(s, k[0][0], k[0][1], k[0][2], k[0][3], q.x, q.y);
-              else mma(s, k[2 * i][0], k[2 * i][1], k[2 * i][2], k[2 * i][3], q.x, q.y);
-              mma(s, k[2 * i + 1][0], k[2 * i + 1][1], k[2 * i + 1][2], k[2 * i + 1][3], q.z, q.w);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint4 q = queries[((nb + u) * (D / 32) + i) * 32 + lane];
+                if (i == 0) mma_first(s[u], k[0][0], k[0][1], k[0][2], k[0][3], q.x, q.y);
+                else mma(s[u], k[2 * i][0], k[2 * i][1], k[2 * i][2], k[2 * i][3], q.x, q.y);
+                mma(s[u], k[2 * i + 1][0], k[2 * i + 1][1], k[2 * i + 1][2], k[2 * i + 1][3], q.z, q.w);
+              }
             }
-            const float4 c = *reinterpret_cast<const float4*>(rowc + nb * 8 + 2 * j);
-            given(r, row0 + nb * 8, tok0, s, make_float2(c.x, c.z), make_float2(c.y, c.w), s0, s1);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float4 c = *reinterpret_cast<const float4*>(rowc + (nb + u) * 8 + 2 * j);
+              given(r, row0 + (nb + u) * 8, tok0, s[u], make_float2(c.x, c.z), make_float2(c.y, c.w), s0, s1);
+            }
           }
           give(r, tok0, s0, s1);
         }
