@@ -13,6 +13,14 @@
 // maximum and sum of the softmax are fp32. Probabilities go into the second product as f16 (11 bits) after a factor of 2^7,
 // so that they are normal numbers down to 2^-21 of the largest; the maximum moves only when a score passes it by 2^8, which
 // the factor leaves room for (2^15).
+//
+// Bound: instructions. A tile of 16 tokens of 128 channels takes a warp about 290, of which 209 widen and multiply: 64 conversions
+// and 64 products with scales for 4096 values are what 4 bits cost over 8. At 0.6 of them a cycle and scheduler (the ALU half
+// busy with conversions) an SM takes 15 bytes a clock of the 23 that DRAM has for it. B200: 4 requests of 70 to 120 thousand
+// tokens, 8 key heads of 128, 103 us, 4.4 TB/s; 256 of 500 to 2300 117 us, 3.6 TB/s; 64 of them 39 us, 2.7 TB/s (4 us until the
+// first tiles come, 5 for the joins). Tried on the first: 16 warps an SM with 128 registers in place of 12 with 168 (105 to 107),
+// 20 with 96 (spills, 127), the next pair's scores between this pair's values (105), parts joined by a second kernel (105), by all
+// warps of the last CTA (101, but the 64 requests 43).
 #include "kv_fp4.cuh"
 #include "ptx.cuh"
 
@@ -825,12 +833,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
 // What the rows give every token: the keys once more, with the rows' final maxima and sums. A tile's keys go through all rows of
 // their (request, key head) pair, so a token's sum is taken by one lane in one order. MANY false: up to 8 rows, in registers;
 // warps deal out the tiles of all pairs (should a request have more rows than the caller said, its row tiles follow each other and
-// add to a token in any order). MANY: CTAs do; the pair's queries lie in shared memory, kChunk blocks of 8 rows at
-// a time, and the warps take the CTA's tiles in turn. A warp has four tiles' keys under way.
+// add to a token in any order). MANY: CTAs do; the pair's queries lie in shared memory, `chunk` blocks of 8 rows at
+// a time, and the warps take the CTA's tiles in turn. A warp has four tiles' keys under way. Bound: instructions; 48 requests of 900
+// to 5000 tokens 39 us beside the attention's 41. The scores that the first kernel has could be kept instead, 32 bytes written and
+// read for a token and 4 query heads against the 72 of its key, but in a captured step they would need memory for the longest request
+// that may come.
 template <int D, bool MANY> struct WeightsShape {
   static constexpr int stages = 4, key_bytes = 9 * D;                  // codes and scales
-  static constexpr int chunk = !MANY ? 0 : D == 256 ? 4 : 8;           // blocks of 8 rows
-  static constexpr int ctas = D == 256 ? 2 : 4;
+  static constexpr int chunk = !MANY ? 0 : D == 256 ? 4 : 16;          // blocks of 8 rows
+  static constexpr int ctas = D == 256 ? 2 : MANY ? 3 : 4;
   static constexpr int ring = kWarps * stages * key_bytes, bars = ring, slots = bars + kWarps * stages * 8;
   static constexpr int flag = slots + kWarps * stages * 4, line = flag + 16, queries = (line + (int)sizeof(Line) + 15) / 16 * 16;
   static constexpr int rows = queries + chunk * 16 * D, smem = rows + chunk * 8 * 8;
