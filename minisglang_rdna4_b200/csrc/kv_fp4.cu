@@ -188,6 +188,7 @@ struct EvictArgs {
   int width, new_width, requests, hk, page_size, pages, budget, recent, sinks;
   int per;                  // tiles of a page
   uint32_t per_magic;       // 2^32 / per, rounded up
+  int wide;                 // four weights may be read at once
 };
 
 __device__ __forceinline__ int page_of(const EvictArgs& a, const int32_t* table, int width, int b, int i) {
@@ -216,7 +217,7 @@ constexpr int kKeysInShared = 49000;   // beside the bins, in the 227 KB of a CT
 // them, and zeros (tokens that nothing has looked at yet) are counted in registers. 384 requests' heads of 12 to 40 thousand
 // tokens 83 us, one CTA an SM; reading the weights in every pass, in four digits of 8 bits, 298.
 template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const EvictArgs a, int longest) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ int hist[kCopies][kBins];
   __shared__ int chunk[kSelWarps], sum_above[kSelWarps], sum_tie[kSelWarps];
   __shared__ int s_digit, s_rank;
@@ -237,13 +238,24 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
   const float* weights = a.weights + layer * a.layer_weights;
   const int32_t* table = a.table + (long long)b * a.width;
   auto column = [&](int i) { return a.per == 1 ? i >> 4 : (int)__umulhi((uint32_t)i >> 4, a.per_magic); };     // i / page_size
-  auto weight_of = [&](int i, int col, int page) {
+  // Four tokens at a time, i a multiple of four: all in one page. Key 0 (no weight has it, and no digit of one begins as it does)
+  // stands for a token that is no candidate.
+  const int lo4 = lo & ~3;
+  auto read4 = [&](int i, int col, int page) {
     (void)MSGL_OOB(page, a.pages);
     page = min(max(page, 0), a.pages - 1);
-    return weight_key(weights[((long long)page * a.hk + h) * a.page_size + i - col * a.page_size]);
+    const float* at = weights + ((long long)page * a.hk + h) * a.page_size + i - col * a.page_size;
+    const float4 w = a.wide ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+    uint4 k = make_uint4(weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w));
+    if (i < lo || i + 4 > hi) {
+      if (i < lo || i >= hi) k.x = 0;
+      if (i + 1 < lo || i + 1 >= hi) k.y = 0;
+      if (i + 2 < lo || i + 2 >= hi) k.z = 0;
+      if (i + 3 < lo || i + 3 >= hi) k.w = 0;
+    }
+    return k;
   };
-  auto read = [&](int i) { return weight_of(i, column(i), table[column(i)]); };
-  auto key_of = [&](int i) { return KEPT ? keys[i] : read(i); };
+  auto keys4 = [&](int i) { return KEPT ? *reinterpret_cast<const uint4*>(keys + i) : read4(i, column(i), table[column(i)]); };
   for (int i = threadIdx.x; i < kCopies * kBins; i += kSelThreads) hist[0][i] = 0;
   __syncthreads();
   uint32_t bound = 0, mask = 0;
@@ -253,33 +265,45 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
     const uint32_t ones = digit == 2 ? 1023u : 2047u;
     if (digit == 0) {
-      constexpr int U = 8;  // loads under way at once
+      constexpr int U = 4;  // loads under way at once
       int zeros = 0;
-      for (int i0 = lo + threadIdx.x; i0 < hi; i0 += U * kSelThreads) {
-        uint32_t key[U];
+      for (int i0 = lo4 + 4 * (int)threadIdx.x; i0 < hi; i0 += 4 * U * kSelThreads) {
+        uint4 key[U];
         int page[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) page[u] = table[column(min(i0 + u * kSelThreads, hi - 1))];
+        for (int u = 0; u < U; ++u) page[u] = table[column(min(i0 + 4 * u * kSelThreads, hi - 1))];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int i = min(i0 + u * kSelThreads, hi - 1);
-          key[u] = weight_of(i, column(i), page[u]);
+          const int i = min(i0 + 4 * u * kSelThreads, (hi - 1) & ~3);
+          key[u] = read4(i, column(i), page[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (i0 + u * kSelThreads >= hi) break;
-          if (KEPT) keys[i0 + u * kSelThreads] = key[u];
-          if (key[u] == kZeroKey) ++zeros;
-          else atomicAdd(&hist[lane % kCopies][key[u] >> 21], 1);
+          if (i0 + 4 * u * kSelThreads >= hi) break;
+          if (KEPT) *reinterpret_cast<uint4*>(keys + i0 + 4 * u * kSelThreads) = key[u];
+          auto count = [&](uint32_t k) {
+            if (k == kZeroKey) ++zeros;
+            else if (k != 0) atomicAdd(&hist[lane % kCopies][k >> 21], 1);
+          };
+          count(key[u].x);
+          count(key[u].y);
+          count(key[u].z);
+          count(key[u].w);
         }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) zeros += __shfl_xor_sync(0xffffffffu, zeros, o);
       if (lane == 0 && zeros > 0) atomicAdd(&hist[0][kZeroKey >> 21], zeros);
     } else {
-      for (int i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-        const uint32_t key = key_of(i);
-        if ((key & mask) == bound) atomicAdd(&hist[lane % kCopies][key >> shift & ones], 1);
+      for (int i = lo4 + 4 * (int)threadIdx.x; i < hi; i += 4 * kSelThreads) {
+        const uint4 k = keys4(i);
+        auto count = [&](uint32_t key) {
+          if ((key & mask) == bound) atomicAdd(&hist[lane % kCopies][key >> shift & ones], 1);
+        };
+        count(k.x);
+        count(k.y);
+        count(k.z);
+        count(k.w);
       }
     }
     __syncthreads();
@@ -317,27 +341,47 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
     rank = s_rank;
   }
   // what is above the bound, and the first `rank` at it
-  const int share = ((hi - lo + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-  const int i0 = min(lo + warp * share, hi), i1 = min(i0 + share, hi);
+  const int share = ((hi - lo4 + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+  const int i0 = min(lo4 + warp * share, hi), i1 = min(i0 + share, hi);
   int above = 0, ties = 0;
-  for (int i = i0 + lane; i - lane < i1; i += 32) {
-    const uint32_t key = i < i1 ? key_of(i) : 0;
-    above += __popc(__ballot_sync(0xffffffffu, i < i1 && key > bound));
-    ties += __popc(__ballot_sync(0xffffffffu, i < i1 && key == bound));
+  for (int i = i0 + 4 * lane; i < i1; i += 128) {
+    const uint4 k = keys4(i);
+    above += (k.x > bound) + (k.y > bound) + (k.z > bound) + (k.w > bound);
+    ties += (k.x == bound) + (k.y == bound) + (k.z == bound) + (k.w == bound);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    above += __shfl_xor_sync(0xffffffffu, above, o);
+    ties += __shfl_xor_sync(0xffffffffu, ties, o);
   }
   if (lane == 0) { sum_above[warp] = above; sum_tie[warp] = ties; }
   __syncthreads();
   above = ties = 0;
   for (int w = 0; w < warp; ++w) { above += sum_above[w]; ties += sum_tie[w]; }
-  const uint32_t below = (1u << lane) - 1;
-  for (int i = i0 + lane; i - lane < i1; i += 32) {
-    const uint32_t key = i < i1 ? key_of(i) : 0;
-    const bool up = i < i1 && key > bound, tie = i < i1 && key == bound;
-    const uint32_t up_bits = __ballot_sync(0xffffffffu, up), tie_bits = __ballot_sync(0xffffffffu, tie);
-    const int ua = above + __popc(up_bits & below), ta = ties + __popc(tie_bits & below);
-    if (up || (tie && ta < rank)) kept[lo + ua + min(ta, rank)] = i;
-    above += __popc(up_bits);
-    ties += __popc(tie_bits);
+  for (int i = i0 + 4 * lane; i - 4 * lane < i1; i += 128) {
+    const uint4 k = i < i1 ? keys4(i) : make_uint4(0, 0, 0, 0);
+    if (!__any_sync(0xffffffffu, k.x >= bound || k.y >= bound || k.z >= bound || k.w >= bound)) continue;
+    const int mine = (k.x > bound) + (k.y > bound) + (k.z > bound) + (k.w > bound) +
+                     ((k.x == bound) + (k.y == bound) + (k.z == bound) + (k.w == bound) << 16);
+    int incl = mine;         // above the bound, and at it, in 16 bits each
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    int ua = above + (incl - mine & 0xFFFF), ta = ties + (incl - mine >> 16);
+    auto put = [&](uint32_t key, int t) {
+      if (key > bound || (key == bound && ta < rank)) kept[lo + ua + min(ta, rank)] = t;
+      ua += key > bound;
+      ta += key == bound;
+    };
+    put(k.x, i);
+    put(k.y, i + 1);
+    put(k.z, i + 2);
+    put(k.w, i + 3);
+    const int all = __shfl_sync(0xffffffffu, incl, 31);
+    above += all & 0xFFFF;
+    ties += all >> 16;
   }
 }
 
@@ -517,9 +561,10 @@ MSGL_API int msgl_evict_fp4(void* pool, long long layer_bytes, void* weights, lo
               (int32_t*)kept, (int32_t*)new_lens, (const int32_t*)lens, width, new_width, requests, hk, page_size, pages, budget,
               recent, sinks, page_size / kTile, 0};
   a.per_magic = magic(a.per);
+  a.wide = (uintptr_t)weights % 16 == 0 && layer_weights % 4 == 0;
   const long long units = (long long)layers * requests * hk, room = (long long)width * page_size;
   // i / 16 / per by a multiplication is exact while i / 16 times (per_magic * per - 2^32 < per) stays below 2^32
-  if (room / kTile * a.per >= (1ll << 32) || room > 0x7fffffffll || units > 0x7fffffffll) {
+  if (room / kTile * a.per >= (1ll << 32) || room > 0x7fff0000ll || units > 0x7fffffffll) {
     msgl_set_error_text("evict_kv_fp4: a block table of fewer tokens");
     return MSGL_BAD_ARG;
   }
@@ -533,7 +578,7 @@ MSGL_API int msgl_evict_fp4(void* pool, long long layer_bytes, void* weights, lo
       if (e != cudaSuccess) { msgl_set_error("evict_kv_fp4 shared memory", e); return MSGL_CUDA_ERROR; }
       if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    msgl_launch(evict_select_kernel<true>, dim3((unsigned)units), dim3(kSelThreads), (size_t)longest * 4, stream, a, (int)longest);
+    msgl_launch(evict_select_kernel<true>, dim3((unsigned)units), dim3(kSelThreads), (size_t)((longest + 3) / 4 * 16), stream, a, (int)longest);
   } else {
     msgl_launch(evict_select_kernel<false>, dim3((unsigned)units), dim3(kSelThreads), 0, stream, a, 0);
   }

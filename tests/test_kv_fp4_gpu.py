@@ -366,6 +366,28 @@ def test_evict(lens, budget, recent, sinks, dim, page, layers):
         assert torch.equal(a, want) and torch.equal(w.nan_to_num(-7.0), want_w.nan_to_num(-7.0))
 
 
+@pytest.mark.parametrize("lens,budget,recent,sinks", [([131, 997, 4099], 65, 7, 3), ([50021], 1025, 3, 13), ([18, 19, 20, 21, 22], 17, 1, 15)],
+                         ids=["short", "beyond_shared_memory", "one_candidate"])
+@pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "on_4_bytes"])
+def test_evict_weights_anywhere(lens, budget, recent, sinks, offset):
+    """Ends of the candidates inside groups of four tokens; weights that begin on 4 bytes, their layers an odd distance apart."""
+    hk, page, dim, layers, slim = 2, 32, 64, 2, -(-budget // 32)
+    table, pages = tables(lens, page, spare=len(lens) * slim + 1)
+    new = torch.tensor([p for p in range(pages) if p not in set(table.flatten().tolist())][:len(lens) * slim],
+                       dtype=torch.int32, device="cuda").view(len(lens), slim)
+    g = torch.Generator("cuda").manual_seed(2)
+    cache = torch.randint(0, 256, (layers, pages, hk, page // 16, 18 * dim), generator=g, device="cuda", dtype=torch.uint8)
+    stride = pages * hk * page + 3 * offset
+    weights = torch.zeros(layers * stride + 8, device="cuda")[offset:].as_strided((layers, pages, hk, page), (stride, hk * page, page, 1))
+    weights.copy_(torch.round(torch.rand(weights.shape, generator=g, device="cuda") ** 3 * 40))
+    want, want_w = cache.clone(), weights.clone()
+    from minisglang_rdna4_b200.ops import ref_fp4
+
+    kept, _ = ops.evict_kv_fp4(cache, weights, table, ints(lens), new, budget, recent, sinks)
+    stay, _ = ref_fp4.evict_kv_fp4(want, want_w, table, ints(lens), new, budget, recent, sinks)
+    assert torch.equal(kept, stay) and torch.equal(cache, want) and torch.equal(weights, want_w)
+
+
 def test_a_conversation_is_stored_weighed_and_cut():
     """Store, weighed attention, eviction, new tokens, attention again, in a captured graph and eagerly."""
     page, hk, hq, dim, lens, budget = 16, 2, 8, 128, [700, 90, 1500], 128
