@@ -475,6 +475,8 @@ class Engine:
             why = f"the cache of {mc.model_type}"
         elif mc.canvas_length:
             why = "block diffusion (its attention is not causal)"
+        elif mc.vision is not None and mc.image_bidirectional and ENV.IMAGE_BIDIRECTIONAL.value:
+            why = "images whose tokens see each other (MSGL_IMAGE_BIDIRECTIONAL=0 lets them look back only)"
         elif ENV.SWA_POOL.value and mc.swa_layers:
             why = "a pool of their own for sliding-window layers (MSGL_SWA_POOL)"
         elif mc.global_head_dim and len({mc.attn_geometry(i) for i in range(mc.num_kv_layers)}) > 1:

@@ -177,6 +177,8 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v
     t, hq, _ = q.shape
     b = seq_lens.shape[0]
     if max_q == 0 and t and b:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("max_q of 0 is read from the device, outside of a graph's capture")
         max_q = int((cu_q[1:] - cu_q[:-1]).max())
     if max_q == 0:
         return out
@@ -198,9 +200,9 @@ def attention_fp4_status(reset=True) -> int:
 
 
 class PromptPlan(K.PrefillPlan):
-    """The tables, and the window that they are for."""
+    """The tables, and what they are for: window, heads, rows, tokens of the longest request."""
 
-    __slots__ = ("window", "group", "dim")
+    __slots__ = ("window", "group", "dim", "rows", "longest")
 
 
 def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
@@ -218,7 +220,7 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a prefill plan is made of lengths on the host, outside of a graph's capture")
     plan = PromptPlan(cu_q, seq_lens, q.device, window, tile=256 if group % 2 else 128)
-    plan.window, plan.group, plan.dim = window, group, dim
+    plan.window, plan.group, plan.dim, plan.rows, plan.longest = window, group, dim, int(cu_q[b]), int(seq_lens.max())
     return plan
 
 
@@ -226,6 +228,10 @@ def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window, 
     _, pages, hk, page, dim = shape
     if not isinstance(plan, PromptPlan) or (plan.window, plan.group, plan.dim) != (window, q.shape[1] // hk, dim):
         raise ValueError("the prefill plan was made for another window or other heads")
+    if (plan.tables.device != q.device or plan.rows > q.shape[0] or plan.n_req > block_table.shape[0]
+            or plan.longest > block_table.shape[1] * page):
+        raise ValueError(f"the prefill plan was made for {plan.n_req} requests of up to {plan.longest} tokens, {plan.rows} rows, on "
+                         f"{plan.tables.device}")
     if scale <= 0:
         raise ValueError("the form for prompts takes a scale above 0")
     if torch.cuda.is_current_stream_capturing():

@@ -237,3 +237,27 @@ def test_pool():
         FP4KVCache(1, 2, 16, 1, 64, torch.bfloat16, "cpu").evict(ints([[0]]), ints([5]), ints([[1]]), 4, 1)
     with pytest.raises(NotImplementedError):
         pool.k_cache(0)
+
+
+REFUSED = {"speculative decoding": dict(spec_algorithm="ngram"), "cache of": dict(latent_layers=[1]), "block diffusion": dict(canvas_length=8),
+           "images": dict(vision=object()), "heads differ": dict(global_head_dim=512), "96 channels": dict(head_dim=96),
+           "pages of 8": dict(page_size=8)}
+
+
+@pytest.mark.parametrize("why", [""] + list(REFUSED))
+def test_what_the_engine_refuses(why):
+    from types import SimpleNamespace
+
+    from minisglang_rdna4_b200.engine.engine import Engine
+
+    fields = dict(spec_algorithm="none", page_size=16, latent_layers=[], layered=False, has_fp32_kernels=False, is_mla=False,
+                  canvas_length=0, vision=None, image_bidirectional=True, swa_layers=[], global_head_dim=0, num_kv_layers=2, head_dim=128,
+                  model_type="some", attn_geometry=lambda i: (i, i))
+    fields.update(REFUSED.get(why, {}))
+    both = SimpleNamespace(**fields)
+    engine = SimpleNamespace(config=both, model_config=both)
+    if why:
+        with pytest.raises(ValueError, match=f"nvfp4 does not go with .*{why}"):
+            Engine._refuse_fp4_pool(engine)
+    else:
+        Engine._refuse_fp4_pool(engine)

@@ -220,6 +220,36 @@ def test_prompts(hq, hk, dim, dtype, window):
         ops.paged_attention_fp4(q, cache, table, cu, ints(lens), -0.1, window=window, max_q=300, plan=plan)
 
 
+def test_plan_of_another_step():
+    """A plan whose rows, requests or tokens the step does not have is refused on the host."""
+    n = lambda *x: torch.tensor(x, dtype=torch.int32).numpy()  # noqa: E731
+    cache = torch.zeros(40, 2, 2, 18 * 128, dtype=torch.uint8, device="cuda")
+    q = torch.zeros(300, 4, 128, device="cuda", dtype=torch.bfloat16)
+    table, cu, lens = torch.arange(20, dtype=torch.int32, device="cuda").view(2, 10), ints([0, 100, 300]), ints([150, 310])
+    plan = ops.prefill_plan_fp4(q, cache, n(0, 100, 300), n(150, 310))
+    ops.paged_attention_fp4(q, cache, table, cu, lens, 0.1, max_q=200, plan=plan)
+    for fewer_rows, fewer_requests, fewer_pages in ((q[:299], table, table), (q, table[:1], table), (q, table, table[:, :9])):
+        b = 1 if fewer_requests.shape[0] == 1 else 2
+        t = fewer_pages[:b]
+        with pytest.raises(ValueError, match="made for 2 requests"):
+            ops.paged_attention_fp4(fewer_rows, cache, t, cu[:b + 1], lens[:b], 0.1, max_q=200, plan=plan)
+
+
+def test_longest_request_is_not_read_in_a_capture():
+    cache = torch.zeros(4, 2, 1, 18 * 64, dtype=torch.uint8, device="cuda")
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16)
+    args = (q, cache, ints([[0]]), ints([0, 1]), ints([5]), 0.1)
+    ops.paged_attention_fp4(*args, max_q=1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="max_q of 0"):
+            ops.paged_attention_fp4(*args)
+        out = ops.paged_attention_fp4(*args, max_q=1)
+    graph.replay()
+    assert torch.isfinite(out).all()
+
+
 def test_steps_that_take_no_prompt_form():
     cache = torch.zeros(4, 2, 1, 18 * 128, dtype=torch.uint8, device="cuda")
     n = lambda *x: torch.tensor(x, dtype=torch.int32).numpy()  # noqa: E731
