@@ -1163,16 +1163,6 @@ template <typename T, int D, bool MANY> int launch_weights(const Fp4Args& a, int
   return MSGL_OK;
 }
 
-int device_sms() {
-  static int sms[64] = {};
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && sms[dev]) return sms[dev];
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  if (dev >= 0 && dev < 64) sms[dev] = n;
-  return n;
-}
-
 long long parts_words(int d, int nb, int workers) { return 2ll * workers * nb * (d / 16 + 1) * 128; }
 
 int* status_word() {

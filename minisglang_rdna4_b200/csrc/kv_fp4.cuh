@@ -55,5 +55,15 @@ __device__ __forceinline__ float2 decode2(uint32_t byte) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+inline int device_sms() {
+  static int sms[64] = {};
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && sms[dev]) return sms[dev];
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 0 && dev < 64) sms[dev] = n;
+  return n;
+}
+
 }  // namespace fp4
 }  // namespace msgl

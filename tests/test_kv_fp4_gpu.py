@@ -396,6 +396,26 @@ def test_evict(lens, budget, recent, sinks, dim, page, layers):
         assert torch.equal(a, want) and torch.equal(w.nan_to_num(-7.0), want_w.nan_to_num(-7.0))
 
 
+@pytest.mark.parametrize("requests", [13, 32, 33])
+def test_evict_more_than_runs_at_once(requests):
+    """(layer, request, head) units in several waves: requests in the order of their lengths, equal, empty and short ones among them."""
+    hk, page, dim, layers, budget = 4, 16, 64, 5, 40
+    lens = [(i * 37) % 200 if i % 4 else 120 for i in range(requests)]
+    table, pages = tables(lens, page, spare=3 * requests + 1)
+    new = torch.tensor([p for p in range(pages) if p not in set(table.flatten().tolist())][:3 * requests],
+                       dtype=torch.int32, device="cuda").view(requests, 3)
+    g = torch.Generator("cuda").manual_seed(3)
+    cache = torch.randint(0, 256, (layers, pages, hk, 1, 18 * dim), generator=g, device="cuda", dtype=torch.uint8)
+    weights = torch.round(torch.rand(layers, pages, hk, page, generator=g, device="cuda") * 50)
+    want, want_w = cache.clone(), weights.clone()
+    from minisglang_rdna4_b200.ops import ref_fp4
+
+    kept, now = ops.evict_kv_fp4(cache, weights, table, ints(lens), new, budget, 5, 2)
+    stay, want_now = ref_fp4.evict_kv_fp4(want, want_w, table, ints(lens), new, budget, 5, 2)
+    assert torch.equal(now, want_now.to(now)) and torch.equal(kept, stay)
+    assert torch.equal(cache, want) and torch.equal(weights, want_w)
+
+
 @pytest.mark.parametrize("lens,budget,recent,sinks", [([131, 997, 4099], 65, 7, 3), ([50021], 1025, 3, 13), ([18, 19, 20, 21, 22], 17, 1, 15)],
                          ids=["short", "beyond_shared_memory", "one_candidate"])
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "on_4_bytes"])
