@@ -1145,7 +1145,8 @@ template <typename T, int D, int NB> int launch(const Fp4Args& a, cudaStream_t s
 
 // Blocks of 8 rows in a row tile: two, so that keys and values are widened once for 16 rows, where the registers have room.
 // B200, us: some 25 rows each of 3 requests of 5 to 9 thousand tokens, 32 heads of 128, with weights: four blocks (spilling) 154,
-// two 126; 16 heads a key head of 256, 20 requests of 2 to 6 thousand: two (spilling) 83, one 58.
+// two 126; four warps of 16 rows each that share widened tiles through shared memory the same as two (they wait for one another);
+// 16 heads a key head of 256, 20 requests of 2 to 6 thousand: two (spilling) 83, one 58.
 int row_blocks(int d, int rows) { return rows <= 8 || d == 256 ? 1 : 2; }
 
 template <typename T, int D, bool MANY> int launch_weights(const Fp4Args& a, int sms, cudaStream_t stream) {
