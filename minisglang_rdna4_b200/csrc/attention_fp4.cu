@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NB>::ctas) fp4_attention
 // warps deal out the tiles of all pairs (should a request have more rows than the caller said, its row tiles follow each other and
 // add to a token in any order). MANY: CTAs do; the pair's queries lie in shared memory, `chunk` blocks of 8 rows at
 // a time, and the warps take the CTA's tiles in turn. A warp has four tiles' keys under way. Bound: instructions; 48 requests of 900
-// to 5000 tokens 39 us beside the attention's 41. The scores that the first kernel has could be kept instead, 32 bytes written and
+// to 5000 tokens 33 us beside the attention's 52 (one chain of products 35; five CTAs an SM the same). The scores that the first kernel has could be kept instead, 32 bytes written and
 // read for a token and 4 query heads against the 72 of its key, but in a captured step they would need memory for the longest request
 // that may come.
 template <int D, bool MANY> struct WeightsShape {
@@ -986,10 +986,16 @@ __global__ void __launch_bounds__(kWarps * 32, WeightsShape<D, MANY>::ctas) fp4_
       }
       next_keys();
       if (!ok) break;
-      float s[4];
+      float s[4], s2[4];               // two chains of products
       mma_first(s, k[0][0], k[0][1], k[0][2], k[0][3], qf[0], qf[1]);
+      mma_first(s2, k[1][0], k[1][1], k[1][2], k[1][3], qf[2], qf[3]);
 #pragma unroll
-      for (int i = 1; i < D / 16; ++i) mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
+      for (int i = 2; i < D / 16; i += 2) {
+        mma(s, k[i][0], k[i][1], k[i][2], k[i][3], qf[2 * i], qf[2 * i + 1]);
+        mma(s2, k[i + 1][0], k[i + 1][1], k[i + 1][2], k[i + 1][3], qf[2 * i + 2], qf[2 * i + 3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += s2[i];
       const int tok0 = (get.r.tile0 + get.tile) * kTile;
       float s0 = 0.f, s1 = 0.f;
       given(get.r, 8 * get.rt, tok0, s, c, e, s0, s1);
