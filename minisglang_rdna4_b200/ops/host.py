@@ -28,6 +28,9 @@ def host_lib() -> Optional[ctypes.CDLL]:
         lib = ctypes.CDLL(_LIB_PATH)
         lib.msgl_common_prefix_i32.restype = ctypes.c_int64
         lib.msgl_common_prefix_i32.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
+        if hasattr(lib, "msgl_prompt_plan"):
+            lib.msgl_prompt_plan.restype = ctypes.c_int
+            lib.msgl_prompt_plan.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 3 + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
         _lib = lib
     return _lib
 
@@ -49,3 +52,21 @@ def common_prefix_len(a: np.ndarray, b: np.ndarray, limit: int) -> int:
     a = np.ascontiguousarray(a[:n])
     b = np.ascontiguousarray(b[:n])
     return int(lib.msgl_common_prefix_i32(a.ctypes.data, b.ctypes.data, n))
+
+
+def prompt_tables(cu_q: np.ndarray, seq_lens: np.ndarray, window: int, tile: int):
+    """``(tables, t_pad, items, rows, longest request)`` as ``ops.cuda.PrefillPlan`` builds them (``cu_q``, ``seq_lens``: contiguous
+    int64); ``None`` where the library was not built."""
+    lib = host_lib()
+    if lib is None or not hasattr(lib, "msgl_prompt_plan"):
+        return None
+    out, info = np.empty(2048, dtype=np.int32), np.empty(5, dtype=np.int64)
+    for _ in range(2):
+        rc = lib.msgl_prompt_plan(cu_q.ctypes.data, seq_lens.ctypes.data, seq_lens.size, window, tile, out.ctypes.data, out.size,
+                                  info.ctypes.data)
+        if rc < 0:
+            raise ValueError("a request has from 0 to as many rows as tokens")
+        t_pad, items, rows, longest, words = info.tolist()
+        if rc:
+            return out[:words], t_pad, items, rows, longest
+        out = np.empty(words, dtype=np.int32)

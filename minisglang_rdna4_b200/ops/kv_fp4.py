@@ -11,6 +11,7 @@ import torch
 from . import _lib
 from . import cuda as K
 from ._lib import c_f, c_i, c_ll, c_p, check, lib
+from .host import prompt_tables
 
 _lib.bind("msgl_store_fp4", c_i, [c_p, c_p, c_ll, c_ll] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
 _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll, c_i, c_p])
@@ -204,6 +205,17 @@ class PromptPlan(K.PrefillPlan):
 
     __slots__ = ("window", "group", "dim", "rows", "longest")
 
+    def __init__(self, cu_q, seq_lens, device, window, tile, tables) -> None:
+        """``tables``: ``host.prompt_tables``; ``None``: they are built here."""
+        if tables is None:
+            super().__init__(cu_q, seq_lens, device, window, tile=tile)
+            return
+        host, self.t_pad, self.n_items = tables[:3]
+        self.n_req, self.tile = seq_lens.size, tile
+        self.off_blk = 8 * self.n_items
+        self.off_req = self.off_blk + self.t_pad // 128
+        self.tables = K._upload_tables(host, device)
+
 
 def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
     """The tcgen05 form of prompts: heads of 64 or 128 channels."""
@@ -211,16 +223,25 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
     group = q.shape[1] // hk
     if dim == 256:
         return None
-    cu_q, seq_lens = (np.minimum(np.asarray(x, dtype=np.int64), 1 << 30) for x in (cu_q, seq_lens))
-    b = seq_lens.size
-    if b == 0 or (np.diff(cu_q) > seq_lens).any():            # rows in front of their text
+    cu_q, seq_lens = (np.ascontiguousarray(x, dtype=np.int64) for x in (cu_q, seq_lens))
+    b, tile = seq_lens.size, 256 if group % 2 else 128
+    if b == 0:
         return None
-    if not K.tc_prefill_pays(int(cu_q[b]), K.PrefillPlan.rows_in_reach(cu_q, seq_lens, window)):
+    try:
+        tables = prompt_tables(cu_q, seq_lens, window, tile)
+    except ValueError:                                        # rows in front of their text
+        return None
+    if tables is None:
+        cu_q, seq_lens = np.minimum(cu_q, 1 << 30), np.minimum(seq_lens, 1 << 30)
+        if (np.diff(cu_q) > seq_lens).any():
+            return None
+    rows, reach = (tables[3], tables[1]) if tables else (int(cu_q[b]), K.PrefillPlan.rows_in_reach(cu_q, seq_lens, window))
+    if not K.tc_prefill_pays(rows, reach):
         return None
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a prefill plan is made of lengths on the host, outside of a graph's capture")
-    plan = PromptPlan(cu_q, seq_lens, q.device, window, tile=256 if group % 2 else 128)
-    plan.window, plan.group, plan.dim, plan.rows, plan.longest = window, group, dim, int(cu_q[b]), int(seq_lens.max())
+    plan = PromptPlan(cu_q, seq_lens, q.device, window, tile, tables)
+    plan.window, plan.group, plan.dim, plan.rows, plan.longest = window, group, dim, rows, tables[4] if tables else int(seq_lens.max())
     return plan
 
 

@@ -261,3 +261,27 @@ def test_what_the_engine_refuses(why):
             Engine._refuse_fp4_pool(engine)
     else:
         Engine._refuse_fp4_pool(engine)
+
+
+@pytest.mark.parametrize("window,tile", [(0, 128), (0, 256), (1, 128), (100, 256), (128, 128), (5000, 128)])
+def test_prompt_tables(window, tile):
+    """The tables that the host library builds are those that NumPy does; a step of many requests has larger ones."""
+    import numpy as np
+
+    from minisglang_rdna4_b200.ops import host
+    from minisglang_rdna4_b200.ops.cuda import PrefillPlan
+
+    rng = np.random.default_rng(0)
+    for b in (1, 2, 7, 400):
+        rows = rng.integers(0, 700, b)
+        lens = rows + np.where(rng.random(b) < 0.3, 0, rng.integers(0, 3000 // min(b, 20), b))
+        cu = np.concatenate([[0], np.cumsum(rows)])
+        want = PrefillPlan(cu, lens, "cpu", window, tile=tile)
+        tables, t_pad, items, total, longest = host.prompt_tables(cu, lens, window, tile)
+        assert (t_pad, items, total, longest) == (want.t_pad, want.n_items, rows.sum(), lens.max())
+        assert (8 * items, 8 * items + t_pad // 128) == (want.off_blk, want.off_req)
+        assert np.array_equal(tables, want.tables.numpy())
+    with pytest.raises(ValueError):
+        host.prompt_tables(np.array([0, 5]), np.array([4]), window, tile)
+    with pytest.raises(ValueError):
+        host.prompt_tables(np.array([5, 0]), np.array([4]), window, tile)
