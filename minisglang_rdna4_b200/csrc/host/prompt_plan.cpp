@@ -18,10 +18,12 @@ extern "C" {
 // `out` (`room` words): per (request, block of `tile` rows) first row, rows, first position, scratch row of the first key in sight,
 // blocks of 128 keys, request, position of that key, 0, the most blocks first; the request of every 128-row block of the scratch; per
 // request scratch row, length, first key. `info`: rows of the scratch, items, rows, longest request, words of the tables. Returns 1; 0
-// where the tables are larger than `room` (`info` is complete); -1 where a request has more rows than tokens, or fewer than none.
+// where the tables are larger than `room` (`info` is complete); -1 where a request has more rows than tokens, or fewer than none, or a row in
+// front of the first.
 __attribute__((visibility("default"))) int msgl_prompt_plan(const int64_t* cu_q, const int64_t* lens, int64_t b, int64_t window,
                                                             int64_t tile, int32_t* out, int64_t room, int64_t* info) {
   int64_t t_pad = 0, n_items = 0, longest = 0;
+  if (b > 0 && cu_q[0] < 0) return -1;
   for (int64_t i = 0; i < b; ++i) {
     const int64_t rows = cu_q[i + 1] - cu_q[i], n = std::min(lens[i], kLongest);
     if (rows < 0 || rows > n || cu_q[i + 1] > kLongest) return -1;

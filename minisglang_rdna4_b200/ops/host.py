@@ -60,12 +60,14 @@ def prompt_tables(cu_q: np.ndarray, seq_lens: np.ndarray, window: int, tile: int
     lib = host_lib()
     if lib is None or not hasattr(lib, "msgl_prompt_plan"):
         return None
+    if seq_lens.ndim != 1 or cu_q.ndim != 1 or cu_q.size < seq_lens.size + 1:
+        raise ValueError(f"first rows {cu_q.shape} of requests {seq_lens.shape}")
     out, info = np.empty(2048, dtype=np.int32), np.empty(5, dtype=np.int64)
     for _ in range(2):
         rc = lib.msgl_prompt_plan(cu_q.ctypes.data, seq_lens.ctypes.data, seq_lens.size, window, tile, out.ctypes.data, out.size,
                                   info.ctypes.data)
         if rc < 0:
-            raise ValueError("a request has from 0 to as many rows as tokens")
+            raise ValueError("a request has from 0 to as many rows as tokens, the first at 0 or behind it")
         t_pad, items, rows, longest, words = info.tolist()
         if rc:
             return out[:words], t_pad, items, rows, longest

@@ -227,6 +227,8 @@ def prefill_plan_fp4(q, cache, cu_q, seq_lens, window):
     b, tile = seq_lens.size, 256 if group % 2 else 128
     if b == 0:
         return None
+    if seq_lens.ndim != 1 or cu_q.shape != (b + 1,):
+        raise ValueError(f"cu_q and seq_lens are the lengths of one step, not {cu_q.shape} and {seq_lens.shape}")
     try:
         tables = prompt_tables(cu_q, seq_lens, window, tile)
     except ValueError:                                        # rows in front of their text

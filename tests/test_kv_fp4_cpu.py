@@ -285,3 +285,7 @@ def test_prompt_tables(window, tile):
         host.prompt_tables(np.array([0, 5]), np.array([4]), window, tile)
     with pytest.raises(ValueError):
         host.prompt_tables(np.array([5, 0]), np.array([4]), window, tile)
+    with pytest.raises(ValueError):
+        host.prompt_tables(np.array([-1, 3]), np.array([4]), window, tile)
+    with pytest.raises(ValueError):
+        host.prompt_tables(np.array([0, 3]), np.array([4, 4]), window, tile)

@@ -258,6 +258,8 @@ def test_steps_that_take_no_prompt_form():
     assert ops.prefill_plan_fp4(q, cache, n(0, 200), n(100)) is None              # more rows than tokens
     assert ops.prefill_plan_fp4(q[:20], cache, n(0, 20), n(50000)) is None        # few rows for the keys
     assert ops.prefill_plan_fp4(q[:0], cache, n(0), n()) is None
+    with pytest.raises(ValueError):
+        ops.prefill_plan_fp4(q, cache, n(0, 200), n(200, 200))
     wide = torch.zeros(4, 2, 1, 18 * 256, dtype=torch.uint8, device="cuda")
     assert ops.prefill_plan_fp4(torch.zeros(200, 4, 256, device="cuda").half(), wide, n(0, 200), n(200)) is None
 
