@@ -99,7 +99,7 @@ template <typename T, int D, int U> __global__ void __launch_bounds__(256) store
     loc[u] = -1;
     if (row < a.rows) {
       loc[u] = a.loc[row];
-      (void)MSGL_OOB(loc[u], a.slots);
+      if (loc[u] >= 0) (void)MSGL_OOB(loc[u], a.slots);
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -146,7 +146,7 @@ template <typename T, int D, int U> __global__ void __launch_bounds__(256) load_
   for (int u = 0; u < U; ++u) {
     code[u][0] = code[u][1] = 0;
     sf[u][0] = sf[u][1] = 0;
-    (void)MSGL_OOB(loc[u], a.slots);
+    if (loc[u] >= 0) (void)MSGL_OOB(loc[u], a.slots);
     if (loc[u] < 0 || loc[u] >= a.slots) continue;
     int t;
     long long at;

@@ -79,6 +79,10 @@ def test_store_and_load(dim, hk, page, dtype):
     first = cache.clone()
     ops.store_kv_fp4(odd.contiguous().view(rows, hk, dim), odd.contiguous().view(rows, hk, dim), cache, loc, ks, vs)
     assert torch.equal(first, cache)
+    # a bounds-checking build names the slot behind the pool, nothing else (rows without a slot, -1, are ordinary)
+    from minisglang_rdna4_b200.ops import cuda as K
+
+    assert all(line.endswith(f"value {pages * page} limit {pages * page}") for line in K.bounds_report())
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16"])
