@@ -2,7 +2,7 @@
 backend in the global context (python/minisgl/layers/attention.py:19-141)."""
 from __future__ import annotations
 
-from typing import Dict, Optional
+from typing import Dict, List, Optional
 
 import torch
 
@@ -14,18 +14,21 @@ from .base import BaseOP
 from .rotary import get_rope_cache
 
 
-_COUNTING: Dict[torch.device, torch.Tensor] = {}
+_COUNTING: Dict[torch.device, List[torch.Tensor]] = {}      # by device, ascending sizes
 
 
 def _counting(n: int, device) -> torch.Tensor:
-    """``0 .. n - 1`` (int32), shared by all layers and steps."""
-    have = _COUNTING.get(device)
-    if have is None or have.numel() < n:
-        have = torch.arange(max(n, 16384), dtype=torch.int32, device=device)
-        if have.is_cuda and torch.cuda.is_current_stream_capturing():
-            return have[:n]                  # a graph's memory: not for the steps outside of it
-        _COUNTING[device] = have
-    return have[:n]
+    """``0 .. n - 1`` (int32), shared by all layers and steps. What was handed out stays where it is: captured graphs hold its
+    address, so a longer step gets a tensor of its own beside it (at least twice as long: a few in all) and a step of ``n`` rows
+    always the same one. They come by a copy that the host waits for, so any stream may read them."""
+    made = _COUNTING.setdefault(device, [])
+    for have in made:
+        if have.numel() >= n:
+            return have[:n]
+    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        return torch.arange(n, dtype=torch.int32, device=device)      # a graph's memory: not for the steps outside of it
+    made.append(torch.arange(max(n, 2 * made[-1].numel() if made else 16384), dtype=torch.int32).to(device))
+    return made[-1][:n]
 
 
 class AttentionLayer(BaseOP):

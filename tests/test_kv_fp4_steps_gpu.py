@@ -1,0 +1,56 @@
+"""The engine's steps over the 4-bit K/V pool on a GPU: what graphs, streams and layers share."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _config(heads=8, kv_heads=2, dim=128, positions=4096):
+    from minisglang_rdna4_b200.models.config import ModelConfig
+
+    d = dict(model_type="qwen3", hidden_size=512, num_hidden_layers=2, num_attention_heads=heads, num_key_value_heads=kv_heads,
+             head_dim=dim, intermediate_size=1024, vocab_size=2048, max_position_embeddings=positions, rms_norm_eps=1e-6,
+             rope_theta=10000.0, tie_word_embeddings=True, architectures=["Qwen3ForCausalLM"])
+    return ModelConfig.from_hf(d)
+
+
+def _prompts(lens, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 2048, (n,), generator=g).tolist() for n in lens]
+
+
+def test_a_captured_graph_after_a_longer_step(monkeypatch):
+    """The slots that a graph has captured hold their numbers after a step of more rows, whatever is allocated then."""
+    from minisglang_rdna4_b200.layers import attention
+
+    monkeypatch.setattr(attention, "_COUNTING", {})
+    device = torch.device("cuda", torch.cuda.current_device())
+    attention._counting(8, device)                                # as the warm-up ahead of a capture does
+    got = torch.zeros(1000, dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got.copy_(attention._counting(1000, device))
+    assert torch.equal(attention._counting(50000, device).cpu(), torch.arange(50000, dtype=torch.int32))
+    junk = [torch.full((16384,), -7, dtype=torch.int32, device=device) for _ in range(64)]
+    graph.replay()
+    assert torch.equal(got.cpu(), torch.arange(1000, dtype=torch.int32)) and len(junk) == 64
+
+
+def test_graphs_match_eager_steps_after_a_long_prompt():
+    """Decode graphs, then a prompt of more rows than any step before in one go, then decode graphs again: as without graphs. (Four
+    requests of one length: no padded rows.)"""
+    from minisglang_rdna4_b200 import SamplingParams
+    from minisglang_rdna4_b200.llm import LLM
+
+    def run(**kw):
+        llm = LLM(model_config=_config(positions=20480), use_dummy_weight=True, kv_cache_dtype="nvfp4", device="cuda", page_size=16,
+                  max_running_req=4, num_page_override=2048, max_extend_tokens=20000, seed=0, **kw)
+        out = []
+        for i, lens in enumerate([[200] * 4, [17001], [211] * 4]):
+            sp = SamplingParams(temperature=0.0, max_tokens=9 if len(lens) > 1 else 1, ignore_eos=True)
+            out.append([o.token_ids for o in llm.generate(_prompts(lens, i), sp)])
+        llm.shutdown()
+        return out
+
+    assert run() == run(cuda_graph_max_bs=-1)
