@@ -603,18 +603,34 @@ class PrefillPlan:
         self.tables = _upload_tables(host, device)
 
 
-_TC_SCRATCH: Dict[Tuple[torch.device, torch.dtype, int], Tuple[torch.Tensor, torch.Tensor, int]] = {}
+# by device, type, heads and stream, the latest used last
+_TC_SCRATCH: Dict[Tuple[torch.device, torch.dtype, int, int], Tuple[torch.Tensor, torch.Tensor, int]] = {}
+_TC_SCRATCH_LOCK = threading.Lock()
+TC_SCRATCH_SETS = 4
 
 
 def _tc_scratch(device, dtype, hk: int, rows: int):
     """Dense K / V^T scratch shared by all layers of a step (each layer's gather overwrites it in
-    stream order). Grows in steps of 8192 rows."""
-    key = (device, dtype, hk)
-    hit = _TC_SCRATCH.get(key)
-    if hit is None or hit[2] < rows:
-        cap = -(-rows // 8192) * 8192
-        _TC_SCRATCH[key] = hit = (workspace(f"prefill K scratch {hk}", hk * cap * 128, dtype, device, zero=True),
-                                   workspace(f"prefill V scratch {hk}", hk * cap * 128, dtype, device, zero=True), cap)
+    stream order). Grows in steps of 8192 rows. One for each stream, since prompts on two streams may run side by side; of a
+    device, type and number of heads the one of the stream that has gone longest without a prompt is dropped when there are more
+    than ``TC_SCRATCH_SETS`` (its memory is the allocator's for that stream, so what still runs there is done with it first). A
+    captured graph has memory of its own."""
+    cap, stream = -(-rows // 8192) * 8192, _stream()
+    numel = hk * cap * 128
+    if _capture_id(stream):
+        return torch.zeros(numel, dtype=dtype, device=device), torch.zeros(numel, dtype=dtype, device=device), cap
+    key = (device, dtype, hk, stream)
+    with _TC_SCRATCH_LOCK:
+        hit = _TC_SCRATCH.pop(key, None)
+        if hit is None or hit[2] < rows:
+            hit = (workspace(f"prefill K scratch {hk} {stream:#x}", numel, dtype, device, zero=True),
+                   workspace(f"prefill V scratch {hk} {stream:#x}", numel, dtype, device, zero=True), cap)
+        _TC_SCRATCH[key] = hit
+        like = [k for k in _TC_SCRATCH if k[:3] == key[:3]]
+        for old in like[:len(like) - TC_SCRATCH_SETS]:
+            del _TC_SCRATCH[old]
+            for name in "KV":
+                _GUARDED.pop(f"prefill {name} scratch {hk} {old[3]:#x}@{device}", None)
     return hit
 
 

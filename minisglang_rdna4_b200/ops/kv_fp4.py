@@ -258,7 +258,7 @@ def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window, 
     if scale <= 0:
         raise ValueError("the form for prompts takes a scale above 0")
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the form for prompts, whose rows in 16 bits lie in memory of all layers and steps, is not captured in a graph")
+        raise RuntimeError("the form for prompts, whose rows in 16 bits lie in memory that a stream's layers and steps share, is not captured in a graph")
     kc, vt, cap = K._tc_scratch(q.device, q.dtype, hk, plan.t_pad)
     base = plan.tables.data_ptr()
     blk, req = base + 4 * plan.off_blk, base + 4 * plan.off_req

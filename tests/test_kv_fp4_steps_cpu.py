@@ -15,3 +15,37 @@ def test_slots_of_a_step_stay_where_a_captured_graph_has_them(monkeypatch):
     middle = attention._counting(17000, device).data_ptr()
     attention._counting(300000, device)
     assert attention._counting(17000, device).data_ptr() == middle != first
+
+
+def test_prompts_on_two_streams_share_no_scratch(monkeypatch):
+    """The rows that a prompt gathers lie in memory of its stream: another stream's prompt neither overwrites nor frees them, and a
+    graph's are its own."""
+    from minisglang_rdna4_b200.ops import cuda as K
+
+    at = [11, 0]                     # stream, capture
+    monkeypatch.setattr(K, "_TC_SCRATCH", {})
+    monkeypatch.setattr(K, "_stream", lambda: at[0])
+    monkeypatch.setattr(K, "_capture_id", lambda stream: at[1])
+    get = lambda rows: K._tc_scratch(torch.device("cpu"), torch.float16, 1, rows)  # noqa: E731
+    spans = lambda hit: [(x.data_ptr(), x.data_ptr() + 2 * x.numel()) for x in hit[:2]]  # noqa: E731
+    first = get(100)
+    assert get(8192)[0] is first[0] and first[2] == 8192 and first[0].numel() == 8192 * 128
+    at[0] = 12
+    second, grown = get(100), get(9000)
+    assert second[0] is not first[0] and grown[2] == 16384
+    for x in spans(first):
+        for y in spans(second) + spans(grown):
+            assert x[1] <= y[0] or y[1] <= x[0]
+    at[0] = 11
+    assert get(1)[0] is first[0]
+    at[1] = 5
+    captured = get(1)
+    assert captured[0] is not first[0] and not captured[0].any()
+    at[1] = 0
+    assert get(1)[0] is first[0]
+    for at[0] in range(20, 40):      # a stream in use keeps its own, the others do not pile up
+        get(1)
+        at[0], keep = 11, at[0]
+        assert get(1)[0] is first[0]
+        at[0] = keep
+    assert len(K._TC_SCRATCH) == K.TC_SCRATCH_SETS

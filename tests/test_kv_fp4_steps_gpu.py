@@ -54,3 +54,40 @@ def test_graphs_match_eager_steps_after_a_long_prompt():
         return out
 
     assert run() == run(cuda_graph_max_bs=-1)
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _step(pages, hk, dim, lens, news, seed):
+    """A prompt step over a pool of its own, as a call without arguments."""
+    from minisglang_rdna4_b200 import ops
+
+    g = torch.Generator("cuda").manual_seed(seed)
+    cache = torch.zeros(pages, hk, 1, 18 * dim, dtype=torch.uint8, device="cuda")
+    k, v = (torch.randn(pages * 16, hk, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    ops.store_kv_fp4(k, v, cache, torch.arange(pages * 16, dtype=torch.int32, device="cuda"))
+    width = -(-max(lens) // 16)
+    table = torch.randint(0, pages, (len(lens), width), generator=g, device="cuda", dtype=torch.int32)
+    cu = _ints([0] + torch.tensor(news).cumsum(0).tolist())
+    q = torch.randn(sum(news), 4 * hk, dim, generator=g, device="cuda").bfloat16()
+    plan = ops.prefill_plan_fp4(q, cache, cu.cpu().numpy(), _ints(lens).cpu().numpy())
+    assert plan is not None
+    n = _ints(lens)
+    return lambda: ops.paged_attention_fp4(q, cache, table, cu, n, 0.1, max_q=max(news), plan=plan)
+
+
+def test_prompts_on_two_streams_at_once():
+    """Steps of different lengths and contents, one of which needs the larger scratch, side by side: as one after the other."""
+    steps = [_step(300, 2, 128, [1500, 3000], [700, 900], 0), _step(300, 2, 128, [9000, 700, 2000], [1500, 700, 100], 1)]
+    want = [run() for run in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(12):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(steps[i]())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
