@@ -627,7 +627,7 @@ def _tc_scratch(device, dtype, hk: int, rows: int):
                    workspace(f"prefill V scratch {hk} {stream:#x}", numel, dtype, device, zero=True), cap)
         _TC_SCRATCH[key] = hit
         like = [k for k in _TC_SCRATCH if k[:3] == key[:3]]
-        for old in like[:len(like) - TC_SCRATCH_SETS]:
+        for old in like[:max(0, len(like) - TC_SCRATCH_SETS)]:
             del _TC_SCRATCH[old]
             for name in "KV":
                 _GUARDED.pop(f"prefill {name} scratch {hk} {old[3]:#x}@{device}", None)
