@@ -625,12 +625,12 @@ def _tc_scratch(device, dtype, hk: int, rows: int):
         if hit is None or hit[2] < rows:
             hit = (workspace(f"prefill K scratch {hk} {stream:#x}", numel, dtype, device, zero=True),
                    workspace(f"prefill V scratch {hk} {stream:#x}", numel, dtype, device, zero=True), cap)
+            others = [k for k in _TC_SCRATCH if k[:3] == key[:3]]
+            for old in others[:max(0, len(others) + 1 - TC_SCRATCH_SETS)]:
+                del _TC_SCRATCH[old]
+                for name in "KV":
+                    _GUARDED.pop(f"prefill {name} scratch {hk} {old[3]:#x}@{device}", None)
         _TC_SCRATCH[key] = hit
-        like = [k for k in _TC_SCRATCH if k[:3] == key[:3]]
-        for old in like[:max(0, len(like) - TC_SCRATCH_SETS)]:
-            del _TC_SCRATCH[old]
-            for name in "KV":
-                _GUARDED.pop(f"prefill {name} scratch {hk} {old[3]:#x}@{device}", None)
     return hit
 
 
