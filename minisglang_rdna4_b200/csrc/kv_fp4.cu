@@ -240,7 +240,8 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
     layer = blockIdx.x % per / a.hk;
   }
   const int unit = (layer * a.requests + b) * a.hk + h;
-  const int n = min(max(a.lens[b], 0), KEPT ? longest : a.width * a.page_size);
+  const int n = min(max(a.lens[b], 0), a.width * a.page_size);
+  const bool in_shared = KEPT && n <= longest;     // a request that is longer than the caller said reads its weights in every pass
   int32_t* kept = a.kept + (long long)unit * a.budget;
   if (layer == 0 && h == 0 && threadIdx.x == 0) a.new_lens[b] = min(n, a.budget);
   if (n <= a.budget) {
@@ -271,7 +272,7 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
     }
     return k;
   };
-  auto keys4 = [&](int i) { return KEPT ? *reinterpret_cast<const uint4*>(keys + i) : read4(i, column(i), table[column(i)]); };
+  auto keys4 = [&](int i) { return in_shared ? *reinterpret_cast<const uint4*>(keys + i) : read4(i, column(i), table[column(i)]); };
   for (int i = threadIdx.x; i < kCopies * kBins; i += kSelThreads) hist[0][i] = 0;
   __syncthreads();
   uint32_t bound = 0, mask = 0;
@@ -296,7 +297,7 @@ template <bool KEPT> __global__ void __launch_bounds__(kSelThreads, 1) evict_sel
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (i0 + 4 * u * kSelThreads >= hi) break;
-          if (KEPT) *reinterpret_cast<uint4*>(keys + i0 + 4 * u * kSelThreads) = key[u];
+          if (in_shared) *reinterpret_cast<uint4*>(keys + i0 + 4 * u * kSelThreads) = key[u];
           auto count = [&](uint32_t k) {
             if (k == kZeroKey) ++zeros;
             else if (k != 0) atomicAdd(&hist[lane % kCopies][k >> 21], 1);

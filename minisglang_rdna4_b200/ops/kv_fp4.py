@@ -143,7 +143,7 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
     check(lib().msgl_evict_fp4(
         cache.data_ptr(), cache.stride(0) if lead else 0, weights.data_ptr(), weights.stride(0) if lead else 0, layers,
         block_table.data_ptr(), block_table.shape[1], new_table.data_ptr(), new_table.shape[1], seq_lens.data_ptr(),
-        kept.data_ptr(), lens.data_ptr(), b, hk, dim, page, pages, budget, recent, sinks, max_kv,
+        kept.data_ptr(), lens.data_ptr(), b, hk, dim, page, pages, budget, recent, sinks, min(max_kv, block_table.shape[1] * page),
         K._stream()), "evict_kv_fp4")
     K._count("evict_kv_fp4", "evict_select_kernel + evict_move_kernel", 2)
     return kept, lens
