@@ -421,14 +421,16 @@ template <int D> __global__ void __launch_bounds__(256) evict_move_kernel(const 
   float* weights = a.weights + layer * a.layer_weights;
   // lane t: where row t comes from, as (tile of the pool) * 16 + row of the tile; rows that are not there come from row 0's place
   const int to_off = tile * kTile % a.page_size;
-  const long long to_page = page_of(a, a.new_table, a.new_width, b, tile * kTile);
+  const int to_page = a.new_table[(long long)b * a.new_width + tile * kTile / a.page_size];
+  (void)MSGL_OOB(to_page, a.pages);
+  if (to_page < 0 || to_page >= a.pages) return;   // nobody's page: as the store skips a slot outside the pool
   long long from;
   {
     const int i = a.kept[(long long)unit * a.budget + tile * kTile + min(lane, rows - 1)];
     const int off = i % a.page_size;
     const long long page = page_of(a, a.table, a.width, b, i);
     from = ((page * a.hk + h) * (a.page_size / kTile) + off / kTile) * kTile + off % kTile;
-    if (lane < rows) weights[(to_page * a.hk + h) * a.page_size + to_off + lane] = weights[(page * a.hk + h) * a.page_size + off];
+    if (lane < rows) weights[((long long)to_page * a.hk + h) * a.page_size + to_off + lane] = weights[(page * a.hk + h) * a.page_size + off];
   }
   uint8_t* to = pool + tile_at<D>(to_page, to_off, h, a.hk, a.page_size);
   auto source = [&](int t, int& ts) {

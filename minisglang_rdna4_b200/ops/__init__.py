@@ -259,7 +259,7 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     ``sinks``, its last ``recent``, and of the others those with the largest weights (of equal ones the earlier; a NaN is
     larger than any number); a shorter one keeps all. What stays is copied in its order, rows and weights, to the pages
     ``new_table [B, at least budget / page]``, which must not be among the pages of any request here; slots behind it and the old
-    pages stay as they are. ``max_kv``: what ``seq_lens`` are expected to stay below (0: what the table holds); a longer request
+    pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected to stay below (0: what the table holds); a longer request
     takes longer.
 
     Returns ``(kept [(layers,) B, Hk, budget] int32: token indices in order, -1 behind them, new lengths [B] int32)``. Later steps

@@ -138,7 +138,7 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
         m = min(n, budget)
         if m == 0:
             continue
-        old, new = block_table[b].long().clamp(0, cache.shape[0] - 1), new_table[b].long().clamp(0, cache.shape[0] - 1)
+        old, new = block_table[b].long().clamp(0, cache.shape[0] - 1), new_table[b, :-(-m // page)].long()
         i = torch.arange(n, device=cache.device)
         w = weights[old[i // page], :, i % page].T                                       # [hk, n]
         if n > budget:
@@ -150,11 +150,12 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget, recen
             stay = i.expand(hk, n)
         kept[b, :, :m] = stay.int()
         parts = [x.transpose(0, 1).flatten(1, 3) for x in unpack_tiles(cache[old])]     # [hk, tokens, bytes]
-        used = new[:-(-m // page)]
-        fresh = [x.transpose(0, 1).flatten(1, 3) for x in unpack_tiles(cache[used])]
+        fresh = [x.transpose(0, 1).flatten(1, 3) for x in unpack_tiles(cache[new.clamp(0, cache.shape[0] - 1)])]
         for x, y in zip(parts, fresh):
             y[:, :m] = x.gather(1, stay[..., None].expand(*stay.shape, x.shape[-1]))
-        cache[used] = pack_tiles(*(y.unflatten(1, (-1, page // 16, 16)).transpose(0, 1) for y in fresh))
+        there = (new >= 0) & (new < cache.shape[0])                                      # what would go to any other page is dropped
+        cache[new[there]] = pack_tiles(*(y.unflatten(1, (-1, page // 16, 16)).transpose(0, 1) for y in fresh))[there]
         j = torch.arange(m, device=cache.device)
-        weights[new[j // page], :, j % page] = w.gather(1, stay).T
+        j = j[there[j // page]]
+        weights[new[j // page], :, j % page] = w.gather(1, stay).T[j]
     return kept, torch.clamp(lens, max=budget).int()

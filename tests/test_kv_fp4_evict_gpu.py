@@ -36,3 +36,21 @@ def test_requests_longer_than_said_lose_nothing(lens, budget, recent, sinks, max
     kept, got_now = ops.evict_kv_fp4(cache, weights, table, n, new, budget, recent, sinks, max_kv=max_kv)
     assert torch.equal(got_now, now.to(got_now)) and torch.equal(kept, stay)
     assert torch.equal(cache, want) and torch.equal(weights, want_w)
+
+
+def test_new_pages_outside_the_pool_are_written_nowhere():
+    """Pages below 0 and behind the pool in the new table: the pool's first and last page stay as they are, the other new pages get
+    their rows, and what is kept is as ever."""
+    lens, budget = [300, 20, 77, 500], 40
+    cache, weights, table, n, new = _case(lens, budget)
+    pages = cache.shape[1]
+    whole, whole_w = cache.clone(), weights.clone()
+    stay, now = ref_fp4.evict_kv_fp4(whole, whole_w, table, n, new, budget, 6, 3)
+    bad = new.clone()
+    bad[0, 1], bad[1, 0], bad[2, 2], bad[3] = -1, pages, 1 << 30, -(1 << 31)
+    want, want_w = cache.clone(), weights.clone()
+    good = new[bad == new].long()
+    want[:, good], want_w[:, good] = whole[:, good], whole_w[:, good]
+    kept, got_now = ops.evict_kv_fp4(cache, weights, table, n, bad, budget, 6, 3)
+    assert torch.equal(got_now, now.to(got_now)) and torch.equal(kept, stay)
+    assert torch.equal(cache, want) and torch.equal(weights, want_w)

@@ -49,3 +49,20 @@ def test_prompts_on_two_streams_share_no_scratch(monkeypatch):
         assert get(1)[0] is first[0]
         at[0] = keep
     assert len(K._TC_SCRATCH) == K.TC_SCRATCH_SETS
+
+
+def test_new_pages_outside_the_pool_are_written_nowhere():
+    from minisglang_rdna4_b200 import ops
+
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    g = torch.Generator().manual_seed(0)
+    cache = torch.randint(0, 256, (9, 2, 1, 18 * 64), generator=g, dtype=torch.uint8)
+    weights = torch.rand(9, 2, 16, generator=g)
+    table, lens = ints([[1, 2, 3], [4, 4, 4]]), ints([48, 7])
+    good, good_w = cache.clone(), weights.clone()
+    stay, _ = ops.evict_kv_fp4(good, good_w, table, lens, ints([[5, 6], [7, 7]]), 20, 4)
+    want, want_w = cache.clone(), weights.clone()
+    want[6], want_w[6] = good[6], good_w[6]
+    kept, now = ops.evict_kv_fp4(cache, weights, table, lens, ints([[-1, 6], [9, 7]]), 20, 4)
+    assert torch.equal(kept, stay) and now.tolist() == [20, 7]
+    assert torch.equal(cache, want) and torch.equal(weights, want_w)
