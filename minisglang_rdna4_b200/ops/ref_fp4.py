@@ -95,7 +95,8 @@ def load_kv_fp4(cache, slots, k_scale, v_scale, dtype):
     pages, back = torch.unique(loc // page, return_inverse=True)
     parts = unpack_tiles(cache[pages])
     kc, vc, ks, vs = (x[back, :, loc % page // 16, loc % 16] for x in parts)
-    return tuple((dequantise(c, s, h) * inside[:, None, None]).to(dtype) for c, s, h in ((kc, ks, k_scale), (vc, vs, v_scale)))
+    outside = ~inside[:, None, None]                # (slot 0 is read for them, which may hold a NaN)
+    return tuple(dequantise(c, s, h).masked_fill(outside, 0.0).to(dtype) for c, s, h in ((kc, ks, k_scale), (vc, vs, v_scale)))
 
 
 def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale=None, v_scale=None, window=0, weights=None):

@@ -66,3 +66,24 @@ def test_new_pages_outside_the_pool_are_written_nowhere():
     kept, now = ops.evict_kv_fp4(cache, weights, table, lens, ints([[-1, 6], [9, 7]]), 20, 4)
     assert torch.equal(kept, stay) and now.tolist() == [20, 7]
     assert torch.equal(cache, want) and torch.equal(weights, want_w)
+
+
+def _nan_pool(dim=64, hk=2, pages=4):
+    from minisglang_rdna4_b200 import ops
+
+    g = torch.Generator().manual_seed(1)
+    cache = torch.zeros(pages, hk, 1, 18 * dim, dtype=torch.uint8)
+    k, v = (torch.randn(pages * 16, hk, dim, generator=g).bfloat16() for _ in range(2))
+    return cache, k, v, lambda: ops.store_kv_fp4(k, v, cache, torch.arange(pages * 16, dtype=torch.int32))
+
+
+def test_slots_outside_the_pool_are_zeros_beside_a_nan():
+    from minisglang_rdna4_b200 import ops
+
+    cache, k, v, store = _nan_pool()
+    k[0, 0, 3] = v[0, 1, 40] = float("nan")
+    store()
+    slots = torch.tensor([-1, 0, 64, -(1 << 31), 1 << 30], dtype=torch.int32)
+    for x in (ops.load_kv_fp4(cache, slots), [y[0] for y in ops.load_kv_fp4(torch.stack([cache, cache]), slots)]):
+        for y in x:
+            assert (y[[0, 2, 3, 4]] == 0).all() and int(y[1].isnan().sum()) == 16
