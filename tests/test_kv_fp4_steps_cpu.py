@@ -1,4 +1,5 @@
 """What the engine's steps over the 4-bit K/V pool keep and share, on the CPU."""
+import pytest
 import torch
 
 
@@ -87,3 +88,37 @@ def test_slots_outside_the_pool_are_zeros_beside_a_nan():
     for x in (ops.load_kv_fp4(cache, slots), [y[0] for y in ops.load_kv_fp4(torch.stack([cache, cache]), slots)]):
         for y in x:
             assert (y[[0, 2, 3, 4]] == 0).all() and int(y[1].isnan().sum()) == 16
+
+
+def _with_and_without_a_nan(where, window):
+    """A request of 50 tokens with 30 rows over a pool with and without a NaN in channels 16 .. 31 of key head 1 of token 35's key or
+    value: ``(outputs, weights, rows that see it)``."""
+    from minisglang_rdna4_b200 import ops
+
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    got = []
+    for value in (0.0, float("nan")):
+        cache, k, v, store = _nan_pool()
+        (k if where == "key" else v)[35, 1, 16:32] = value
+        store()
+        q = torch.randn(30, 4, 64, generator=torch.Generator().manual_seed(2)).half()
+        weights = torch.zeros(4, 2, 16)
+        out = ops.paged_attention_fp4(q, cache, ints([[0, 1, 2, 3]]), ints([0, 30]), ints([50]), 0.1, window=window, weights=weights)
+        got.append((out, weights.transpose(0, 1).flatten(1)))
+    pos = torch.arange(20, 50)
+    return got, (pos >= 35) & ((pos < 35 + window) if window else pos >= 0)
+
+
+@pytest.mark.parametrize("window", [0, 5])
+@pytest.mark.parametrize("where", ["key", "value"])
+def test_a_nan_reaches_the_rows_that_see_it_alone(where, window):
+    ((clean, clean_w), (out, weights)), sees = _with_and_without_a_nan(where, window)
+    bad = torch.zeros(30, 4, 64, dtype=torch.bool)
+    bad[sees, 2:, slice(16, 32) if where == "value" else slice(64)] = True
+    assert torch.equal(out.isnan(), bad) and torch.equal(out[~bad], clean[~bad])
+    given = torch.zeros(2, 64, dtype=torch.bool)
+    if where == "key":                   # the weights that its rows give are none either
+        first = 35 - window + 1 if window else 0
+        given[1, first:35 + window if window else 50] = True
+        given[1, 50:] = False
+    assert torch.equal(weights.isnan(), given) and torch.equal(weights[~given], clean_w[~given])
