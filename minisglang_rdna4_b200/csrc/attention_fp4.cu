@@ -1109,8 +1109,8 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
       for (int w = 0; w < 2; ++w) *reinterpret_cast<uint4*>(row + 64 + j * 16 + 8 * w) = make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e)                  // what lies behind the request may be anything
-    if (tok0 + 4 * j + e >= n) x.vs[0] &= ~(0xFFu << (8 * e));
+  for (int e = 0; e < 4; ++e)                  // what lies behind the request may be anything; fp4_prompt_nans_kernel puts NaNs back
+    if (tok0 + 4 * j + e >= n || (x.vs[0] >> (8 * e) & 0x7F) == 0x7F) x.vs[0] &= ~(0xFFu << (8 * e));
   const uint32_t s01 = widen_e4m3(x.vs[0]), s23 = widen_e4m3(x.vs[0] >> 16);
 #pragma unroll
   for (int w = 0; w < D / 64; ++w) {
@@ -1132,6 +1132,46 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
   if (D == 64)
 #pragma unroll
     for (int i = 0; i < 8; ++i) *reinterpret_cast<uint2*>(vt + ((long long)h * 128 + 64 + g * 8 + i) * t_cap + t0 + 4 * j) = make_uint2(0, 0);
+}
+
+// NaN values of a prompt step. The product of probabilities and values would give one that only later rows of a block see to the
+// earlier ones too (0 * NaN), so the gather leaves zeros in their place and this kernel writes the NaNs over the output of the rows
+// that see them: 16 channels of a value each. Without any, which is nearly always, it reads a tile's value scales and is done.
+template <typename T, int D> __global__ void __launch_bounds__(256)
+fp4_prompt_nans_kernel(const Fp4Args a, T* __restrict__ out, const int* __restrict__ items, int n_items, const int* __restrict__ blk_req,
+                       const int* __restrict__ req_info, int tiles) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, id = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (id >= tiles) return;
+  const int h = blockIdx.y, t0 = id * kTile, req = blk_req[t0 >> 7];
+  const int tok0 = t0 - req_info[3 * req] + req_info[3 * req + 2], n = req_info[3 * req + 1];
+  if (tok0 >= n) return;
+  const int page = min(max(a.table[(long long)req * a.table_stride + min(tok0 / a.page_size, a.width - 1)], 0), a.pages - 1);
+  const uint8_t* tile = a.pool + ((long long)(page * a.hk + h) * a.per + tok0 / kTile % a.per) * Tile<D>::bytes;
+  uint32_t bad = 0;                            // lanes 4 b .. 4 b + 3: tokens whose block b is NaN
+  if (lane < D / 4) {
+    const uint32_t sf = *reinterpret_cast<const uint32_t*>(tile + Tile<D>::v_sf + 4 * lane);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = 4 * (lane & 3) + e;
+      if ((sf >> (8 * e) & 0x7F) == 0x7F && tok0 + t < n) bad |= 1u << t;
+    }
+  }
+  if (!__any_sync(0xffffffffu, bad != 0)) return;
+  bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+  bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+  for (int i = 0; i < n_items; ++i) {          // blocks of rows: first row, rows, first position, ., ., request
+    const int* it = items + 8 * i;
+    if (it[5] != req) continue;
+    for (int row = 0; row < it[1]; ++row) {
+      const int hi = it[2] + row - tok0, lo = a.window > 0 ? hi - a.window : -1;        // tokens lo + 1 .. hi of the tile are seen
+      uint32_t seen = hi < 0 ? 0u : (2u << min(hi, 15)) - 1u;
+      if (lo >= 0) seen &= ~((2u << min(lo, 15)) - 1u);
+      if (lane < D / 4 && (bad & seen))
+        for (int g = 0; g < a.group; ++g)      // four channels a lane
+          *reinterpret_cast<uint2*>(out + ((long long)(it[0] + row) * a.hq + h * a.group + g) * D + 4 * lane) = make_uint2(0x7FFF7FFFu, 0x7FFF7FFFu);
+    }
+  }
 }
 
 template <typename T, int D, int NB> int launch(const Fp4Args& a, cudaStream_t stream) {
@@ -1239,18 +1279,28 @@ MSGL_API int msgl_attention_fp4(const void* q, void* out, const void* pool, cons
   return MSGL_OK;
 }
 
-MSGL_API int msgl_gather_fp4(const void* pool, const void* table, long long table_stride, int width, void* kc, void* vt, const void* blk_req,
-                             const void* req_info, long long t_cap, int t_pad, int hk, int d, int page_size, int pages, int dtype,
-                             cudaStream_t stream) {
-  if (t_pad <= 0) return MSGL_OK;
-  if (hk <= 0 || (d != 64 && d != 128) || page_size <= 0 || page_size % kTile || (uintptr_t)pool % 16 || t_pad % 128 || t_pad > t_cap ||
-      width <= 0 || (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
-    msgl_set_error_text("gather of a 4-bit pool: heads of 64 or 128 channels, blocks of 128 rows");
+MSGL_API int msgl_attn_prefill_tc(const void* q, long long q_row_stride, void* out, const void* k_pool, const void* v_pool, void* kc,
+                                  void* vt, long long t_cap, int t_pad, const void* items, int n_items, const void* blk_req,
+                                  const void* req_info, const void* block_table, int bt_stride, const void* k_scale, const void* v_scale,
+                                  int total_q, int hq, int hk, int d, int page_size, int kv_fp8, float scale, int window, int chunk,
+                                  float softcap, const void* gate, long long ldg, const void* bias, int entries, int zero,
+                                  const void* sink, int all_values, int pos_form, int dtype, cudaStream_t stream);
+
+// A prompt step: the rows in sight to 16 bits (`kc`, `vt`: 128 hk t_cap elements each), the tensor-core kernel, NaN values. `items`,
+// `blk_req`, `req_info`: the tables of the step, as there.
+MSGL_API int msgl_prompt_fp4(const void* q, void* out, const void* pool, const void* table, long long table_stride, int width, void* kc,
+                             void* vt, long long t_cap, int t_pad, const void* items, int n_items, const void* blk_req,
+                             const void* req_info, const void* k_head, const void* v_head, int total_q, int hq, int hk, int d,
+                             int page_size, int pages, int window, int pos_form, float scale, int dtype, cudaStream_t stream) {
+  if (t_pad <= 0 || n_items <= 0 || total_q <= 0) return MSGL_OK;
+  if (hk <= 0 || hq <= 0 || hq % hk || (d != 64 && d != 128) || page_size <= 0 || page_size % kTile || (uintptr_t)pool % 16 ||
+      (uintptr_t)out % 16 || t_pad % 128 || t_pad > t_cap || width <= 0 || (dtype != MSGL_BF16 && dtype != MSGL_F16)) {
+    msgl_set_error_text("prompts over a 4-bit pool: heads of 64 or 128 channels, blocks of 128 rows");
     return MSGL_BAD_ARG;
   }
   Fp4Args a{};
   a.pool = (const uint8_t*)pool; a.table = (const int32_t*)table; a.table_stride = table_stride; a.width = width;
-  a.hk = hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages;
+  a.hq = hq; a.hk = hk; a.group = hq / hk; a.page_size = page_size; a.per = page_size / kTile; a.pages = pages; a.window = window;
   const int tiles = t_pad / kTile;
   const dim3 grid((tiles + 7) / 8, hk);
 #define GATHER(T, D) msgl_launch(fp4_gather_kernel<T, D>, grid, dim3(256), 0, stream, a, (T*)kc, (T*)vt, (const int*)blk_req, (const int*)req_info, t_cap, tiles)
@@ -1258,6 +1308,15 @@ MSGL_API int msgl_gather_fp4(const void* pool, const void* table, long long tabl
   else { if (d == 64) GATHER(__half, 64); else GATHER(__half, 128); }
 #undef GATHER
   MSGL_CHECK_LAUNCH("gather of a 4-bit pool");
+  const int rc = msgl_attn_prefill_tc(q, (long long)hq * d, out, nullptr, nullptr, kc, vt, t_cap, t_pad, items, n_items, blk_req, req_info,
+                                      table, 0, k_head, v_head, total_q, hq, hk, d, page_size, 2, scale, window, 0, 0.f, nullptr, 0,
+                                      nullptr, 0, 0, nullptr, 0, pos_form, dtype, stream);
+  if (rc != MSGL_OK) return rc;
+#define NANS(T, D) msgl_launch(fp4_prompt_nans_kernel<T, D>, grid, dim3(256), 0, stream, a, (T*)out, (const int*)items, n_items, (const int*)blk_req, (const int*)req_info, tiles)
+  if (dtype == MSGL_BF16) { if (d == 64) NANS(__nv_bfloat16, 64); else NANS(__nv_bfloat16, 128); }
+  else { if (d == 64) NANS(__half, 64); else NANS(__half, 128); }
+#undef NANS
+  MSGL_CHECK_LAUNCH("NaN values of a prompt");
   return MSGL_OK;
 }
 

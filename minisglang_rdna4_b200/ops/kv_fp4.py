@@ -18,7 +18,7 @@ _lib.bind("msgl_load_fp4", c_i, [c_p, c_ll, c_i] + [c_p] * 5 + [c_i] * 4 + [c_ll
 _lib.bind("msgl_evict_fp4", c_i, [c_p, c_ll, c_p, c_ll, c_i, c_p, c_i, c_p, c_i, c_p, c_p, c_p] + [c_i] * 9 + [c_p])
 _lib.bind("msgl_attention_fp4", c_i, [c_p] * 4 + [c_ll, c_i] + [c_p] * 7 + [c_i] * 9 + [c_f, c_i, c_p])
 _lib.bind("msgl_attention_fp4_workspace", c_ll, [c_i] * 6 + [c_p])
-_lib.bind("msgl_gather_fp4", c_i, [c_p, c_p, c_ll, c_i] + [c_p] * 4 + [c_ll] + [c_i] * 6 + [c_p])
+_lib.bind("msgl_prompt_fp4", c_i, [c_p] * 4 + [c_ll, c_i, c_p, c_p, c_ll, c_i, c_p, c_i] + [c_p] * 4 + [c_i] * 8 + [c_f, c_i, c_p])
 _lib.bind("msgl_attention_fp4_status", c_i, [c_i])
 
 TILE = 16                       # tokens of a tile
@@ -261,13 +261,10 @@ def _prefill(q, cache, out, block_table, plan, scale, k_scale, v_scale, window, 
         raise RuntimeError("the form for prompts, whose rows in 16 bits lie in memory that a stream's layers and steps share, is not captured in a graph")
     kc, vt, cap = K._tc_scratch(q.device, q.dtype, hk, plan.t_pad)
     base = plan.tables.data_ptr()
-    blk, req = base + 4 * plan.off_blk, base + 4 * plan.off_req
-    check(lib().msgl_gather_fp4(cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], kc.data_ptr(),
-                                vt.data_ptr(), blk, req, cap, plan.t_pad, hk, dim, page, pages, K._dt(q), K._stream()), "gather_fp4")
-    check(lib().msgl_attn_prefill_tc(
-        q.data_ptr(), q.stride(0), out.data_ptr(), None, None, kc.data_ptr(), vt.data_ptr(), cap, plan.t_pad, base, plan.n_items, blk,
-        req, block_table.data_ptr(), block_table.stride(0), K._p(k_scale), K._p(v_scale), q.shape[0], q.shape[1], hk, dim, page, 2,
-        float(scale), int(window), 0, 0.0, None, 0, None, 0, 0, None, 0, int(plan.tile == 256), K._dt(q), K._stream()),
-        "attn_prefill_tc")
-    K._count("paged_attention_fp4 (prompts)", "fp4_gather_kernel + attn_prefill_tc_kernel", 2)
+    check(lib().msgl_prompt_fp4(
+        q.data_ptr(), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], kc.data_ptr(),
+        vt.data_ptr(), cap, plan.t_pad, base, plan.n_items, base + 4 * plan.off_blk, base + 4 * plan.off_req, K._p(k_scale), K._p(v_scale),
+        q.shape[0], q.shape[1], hk, dim, page, pages, int(window), int(plan.tile == 256), float(scale), K._dt(q), K._stream()),
+        "paged_attention_fp4 (prompts)")
+    K._count("paged_attention_fp4 (prompts)", "fp4_gather_kernel + attn_prefill_tc_kernel + fp4_prompt_nans_kernel", 3)
     return out
