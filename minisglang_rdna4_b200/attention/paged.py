@@ -38,7 +38,8 @@ class LayerPlans:
 
 
 class Fp4Plans:
-    """Tables of the form for prompts over a 4-bit pool, one set per window of the step's layers."""
+    """Tables of the form for prompts over a 4-bit pool, one set per window and number of query heads a key head of the step's
+    layers (layers may differ in both)."""
 
     def __init__(self, cu_q, seq_lens) -> None:
         self._lens, self._plans = (cu_q, seq_lens), {}
@@ -46,9 +47,10 @@ class Fp4Plans:
     def of(self, q, cache, window: int):
         from ..env import ENV
 
-        if window not in self._plans:
-            self._plans[window] = None if ENV.DISABLE_TC_PREFILL.value else ops.prefill_plan_fp4(q, cache, *self._lens, window)
-        return self._plans[window]
+        key = (window, q.shape[1] // cache.shape[1])
+        if key not in self._plans:
+            self._plans[key] = None if ENV.DISABLE_TC_PREFILL.value else ops.prefill_plan_fp4(q, cache, *self._lens, window)
+        return self._plans[key]
 
 
 class PagedAttentionBackend(BaseAttnBackend):

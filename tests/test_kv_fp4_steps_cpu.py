@@ -122,3 +122,16 @@ def test_a_nan_reaches_the_rows_that_see_it_alone(where, window):
         given[1, first:35 + window if window else 50] = True
         given[1, 50:] = False
     assert torch.equal(weights.isnan(), given) and torch.equal(weights[~given], clean_w[~given])
+
+
+def test_layers_that_differ_in_query_heads_have_plans_of_their_own(monkeypatch):
+    from minisglang_rdna4_b200.attention import paged
+
+    made = []
+    monkeypatch.setattr(paged.ops, "prefill_plan_fp4", lambda q, cache, cu, n, window: made.append((window, q.shape[1])) or made[-1])
+    cache = torch.zeros(1, 2, 1, 18 * 64, dtype=torch.uint8)
+    plans = paged.Fp4Plans(None, None)
+    for _ in range(2):                   # layers of a model with 8 and 12 query heads, with and without a window
+        for window, heads in ((0, 8), (0, 12), (64, 12), (64, 8)):
+            assert plans.of(torch.zeros(5, heads, 64), cache, window) == (window, heads)
+    assert len(made) == 4
