@@ -481,6 +481,8 @@ class Engine:
             why = "a pool of their own for sliding-window layers (MSGL_SWA_POOL)"
         elif mc.global_head_dim and len({mc.attn_geometry(i) for i in range(mc.num_kv_layers)}) > 1:
             why = "layers whose heads differ"
+        elif mc.global_head_dim and mc.attn_geometry(0) != (mc.num_kv_heads, mc.head_dim):
+            why = "layers of {} key heads of {} channels, all of them global,".format(*mc.attn_geometry(0))
         elif mc.head_dim not in (64, 128, 256):
             why = f"heads of {mc.head_dim} channels"
         elif cfg.page_size % 16:

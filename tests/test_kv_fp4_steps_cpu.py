@@ -135,3 +135,28 @@ def test_layers_that_differ_in_query_heads_have_plans_of_their_own(monkeypatch):
         for window, heads in ((0, 8), (0, 12), (64, 12), (64, 8)):
             assert plans.of(torch.zeros(5, heads, 64), cache, window) == (window, heads)
     assert len(made) == 4
+
+
+def _engine(**model):
+    """As much of an engine as its boot has when the pool is sized, on a GPU of 64 GiB."""
+    from types import SimpleNamespace as Some
+
+    mc = Some(**{**dict(latent_layers=[], layered=False, has_fp32_kernels=False, is_mla=False, canvas_length=0, vision=None,
+                        image_bidirectional=True, swa_layers=[], global_head_dim=0, num_kv_layers=3, num_kv_heads=2, head_dim=128,
+                        model_type="some", is_recurrent=False, intermediate_size=512, q_size=1024, kv_size=256, hidden_size=512,
+                        attn_geometry=lambda i: (2, 128)), **model})
+    config = Some(spec_algorithm="none", page_size=16, num_page_override=None, tp_size=1, memory_ratio=0.9, max_running_req=4,
+                  max_extend_tokens=1024)
+    return Some(config=config, model_config=mc, kv_fp8=False, kv_fp4=True, dtype=torch.bfloat16, kv_layers=3, kv_heads_local=2,
+                page_size=16, _main_geometry=None, mla_latent=False, _head_geometry=None, device=torch.device("cuda"), _swa_layers=0,
+                cpu_group=None)
+
+
+def test_a_pool_whose_layers_all_have_another_geometry_is_refused():
+    from minisglang_rdna4_b200.engine.engine import Engine
+
+    Engine._refuse_fp4_pool(_engine())
+    Engine._refuse_fp4_pool(_engine(global_head_dim=128))
+    for heads, width in ((2, 256), (1, 128)):
+        with pytest.raises(ValueError, match=f"nvfp4 does not go with layers of {heads} key heads of {width} channels"):
+            Engine._refuse_fp4_pool(_engine(global_head_dim=width, attn_geometry=lambda i: (heads, width)))
