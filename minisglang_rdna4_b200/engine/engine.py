@@ -607,9 +607,9 @@ class Engine:
         itemsize = 1 if self.kv_fp8 else torch.empty((), dtype=self.dtype).element_size()
         per_page = MHAKVCache.token_bytes(self.kv_layers, self.kv_heads_local, mc.head_dim,
                                           itemsize) * self.page_size
-        if self.kv_fp4:
+        if self.kv_fp4:                             # (one geometry, that of head_dim: _refuse_fp4_pool)
             per_page = FP4KVCache.token_bytes(self.kv_layers, self.kv_heads_local, mc.head_dim) * self.page_size
-        if self._main_geometry:
+        elif self._main_geometry:
             per_page = MHAKVCache.token_bytes(self.kv_layers, 1, max(h * d for h, d in self._main_geometry),
                                               itemsize) * self.page_size
         if self.mla_latent:

@@ -160,3 +160,14 @@ def test_a_pool_whose_layers_all_have_another_geometry_is_refused():
     for heads, width in ((2, 256), (1, 128)):
         with pytest.raises(ValueError, match=f"nvfp4 does not go with layers of {heads} key heads of {width} channels"):
             Engine._refuse_fp4_pool(_engine(global_head_dim=width, attn_geometry=lambda i: (heads, width)))
+
+
+def test_pages_are_counted_in_4_bits_whatever_names_the_geometry(monkeypatch):
+    from minisglang_rdna4_b200.engine.engine import Engine
+
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (60 << 30, 64 << 30))
+    plain, named, wide = _engine(), _engine(global_head_dim=128), _engine(global_head_dim=128)
+    named._main_geometry = wide._main_geometry = [(2, 128)] * 3
+    wide.kv_fp4 = False
+    pages = [Engine._determine_num_pages(e) for e in (plain, named, wide)]
+    assert pages[0] == pages[1] and 3.5 < pages[0] / pages[2] < 3.6          # 16 bits against 4.5
