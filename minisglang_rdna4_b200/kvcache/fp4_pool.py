@@ -78,7 +78,10 @@ class FP4KVCache(BaseKVCachePool):
     v_cache = k_cache
 
     def set_scales(self, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
-        """Install the factors per (layer, head): the largest magnitude over 2688 (6 times the largest scale)."""
+        """Install the factors per (layer, head), above 0: the largest magnitude over 2688 (6 times the largest scale)."""
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if not bool(((t > 0) & torch.isfinite(t.float())).all()):      # a head's zeros would come back as NaN
+                raise ValueError(f"factors of 4-bit K/V heads are positive numbers; {name} holds others")
         self.k_scale.copy_(k_scale.to(self.k_scale))
         self.v_scale.copy_(v_scale.to(self.v_scale))
 

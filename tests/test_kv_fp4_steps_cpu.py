@@ -171,3 +171,18 @@ def test_pages_are_counted_in_4_bits_whatever_names_the_geometry(monkeypatch):
     wide.kv_fp4 = False
     pages = [Engine._determine_num_pages(e) for e in (plain, named, wide)]
     assert pages[0] == pages[1] and 3.5 < pages[0] / pages[2] < 3.6          # 16 bits against 4.5
+
+
+def test_factors_that_are_no_positive_numbers_are_refused():
+    from minisglang_rdna4_b200.kvcache import FP4KVCache
+
+    pool = FP4KVCache(2, 4, 16, 2, 64, torch.bfloat16, "cpu")
+    good = torch.full((2, 2), 0.25)
+    for value in (0.0, -1.0, float("nan"), float("inf")):
+        bad = good.clone()
+        bad[1, 0] = value
+        for pair in ((bad, good), (good, bad)):
+            with pytest.raises(ValueError, match="positive"):
+                pool.set_scales(*pair)
+    pool.set_scales(good, 2 * good)
+    assert torch.equal(pool.k_scale, good) and torch.equal(pool.v_scale, 2 * good)
