@@ -1140,9 +1140,13 @@ def gemm_fp8_block_status(reset=True) -> int:
 
 
 def attn_status(reset=True) -> int:
-    a = int(lib().msgl_attn_status(int(reset)))
-    b = int(lib().msgl_attn_tc_status(int(reset)))
-    return a or b or int(lib().msgl_talk_status(int(reset)))
+    """Nonzero: a wait in one of the attention kernels ran out. Each of them is read, so that ``reset`` reaches them all."""
+    from ._lib import bind, c_i
+
+    bind("msgl_attention_fp4_status", c_i, [c_i])
+    got = [int(read(int(reset))) for read in (lib().msgl_attn_status, lib().msgl_attn_tc_status, lib().msgl_talk_status,
+                                              lib().msgl_attention_fp4_status)]
+    return next((status for status in got if status), 0)
 
 
 # ------------------------------------------------------------------------------------------ sampling

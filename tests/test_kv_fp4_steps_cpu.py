@@ -186,3 +186,27 @@ def test_factors_that_are_no_positive_numbers_are_refused():
                 pool.set_scales(*pair)
     pool.set_scales(good, 2 * good)
     assert torch.equal(pool.k_scale, good) and torch.equal(pool.v_scale, 2 * good)
+
+
+def test_a_wait_that_ran_out_over_the_4_bit_pool_is_a_status_of_attention(monkeypatch):
+    from types import SimpleNamespace
+
+    from minisglang_rdna4_b200.ops import _lib, cuda
+
+    state = dict.fromkeys(("msgl_attn_status", "msgl_attn_tc_status", "msgl_talk_status", "msgl_attention_fp4_status"), 0)
+
+    def reader(name):
+        def read(reset):
+            got = state[name]
+            state[name] = 0 if reset else got
+            return got
+        return read
+
+    monkeypatch.setattr(cuda, "lib", lambda: SimpleNamespace(**{name: reader(name) for name in state}))
+    monkeypatch.setattr(_lib, "bind", lambda *args: None)
+    assert cuda.attn_status() == 0
+    for name in state:
+        state[name] = 401
+        assert cuda.attn_status(reset=False) == 401 and cuda.attn_status() == 401 and cuda.attn_status() == 0, name
+    state.update(dict.fromkeys(state, 5))
+    assert cuda.attn_status() == 5 and cuda.attn_status() == 0      # all are reset by one call
