@@ -181,6 +181,7 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale, v
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("max_q of 0 is read from the device, outside of a graph's capture")
         max_q = int((cu_q[1:] - cu_q[:-1]).max())
+    max_q = min(max_q, t)                # however large a bound the caller has
     if max_q == 0:
         return out
     need, workers = attention_fp4_workspace(t, hq, hk, dim, max_q, weights is not None)

@@ -91,3 +91,18 @@ def test_prompts_on_two_streams_at_once():
                 got[i].append(steps[i]())
     torch.cuda.synchronize()
     assert all(torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
+
+
+@pytest.mark.parametrize("max_q", [1 << 31, 1 << 32, (1 << 32) + 1, 1 << 40])
+def test_bounds_beyond_32_bits(max_q):
+    """``max_q`` and ``max_kv`` may be larger than what the step has, by any amount."""
+    from minisglang_rdna4_b200 import ops
+
+    g = torch.Generator("cuda").manual_seed(0)
+    cache = torch.zeros(20, 2, 1, 18 * 128, dtype=torch.uint8, device="cuda")
+    k, v = (torch.randn(320, 2, 128, generator=g, device="cuda").bfloat16() for _ in range(2))
+    ops.store_kv_fp4(k, v, cache, torch.arange(320, dtype=torch.int32, device="cuda"))
+    table, cu, lens = torch.arange(20, dtype=torch.int32, device="cuda").view(2, 10), _ints([0, 5, 6]), _ints([150, 20])
+    q = torch.randn(6, 8, 128, generator=g, device="cuda").bfloat16()
+    got = [ops.paged_attention_fp4(q, cache, table, cu, lens, 0.1, max_q=n, max_kv=n) for n in (6, max_q)]
+    assert torch.equal(*got) and torch.isfinite(got[0]).all()
