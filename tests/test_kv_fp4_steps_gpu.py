@@ -106,3 +106,122 @@ def test_bounds_beyond_32_bits(max_q):
     q = torch.randn(6, 8, 128, generator=g, device="cuda").bfloat16()
     got = [ops.paged_attention_fp4(q, cache, table, cu, lens, 0.1, max_q=n, max_kv=n) for n in (6, max_q)]
     assert torch.equal(*got) and torch.isfinite(got[0]).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,quant", [(8, 2, 128, None), (7, 1, 128, None), (8, 4, 64, None), (4, 2, 256, None), (8, 2, 128, "mxfp4")])
+def test_served_steps_against_loops_in_64_bits(monkeypatch, heads, kv_heads, dim, quant):
+    """Every layer of every step that the engine runs eagerly (chunked prompts, cached prefixes, decode steps), checked where it calls the
+    operators: rows go to the slots of their positions, quantised with the layer's own factors; what attention reads is what was stored;
+    its output is that of a plain form over these values."""
+    import plain_kv_fp4 as plain
+    from minisglang_rdna4_b200 import SamplingParams, ops
+    from minisglang_rdna4_b200.kvcache import fp8_scales
+    from minisglang_rdna4_b200.llm import LLM
+
+    g = torch.Generator().manual_seed(4)
+    factors = [2.0 ** torch.randint(lo, lo + 3, (2, kv_heads), generator=g) for lo in (-8, -10)]
+    monkeypatch.setattr(fp8_scales, "resolve_kv_scales", lambda *a, **k: (6 * factors[0], 6 * factors[1], "test"))
+    llm = LLM(model_config=_config(heads, kv_heads, dim), use_dummy_weight=True, quantization=quant, kv_cache_dtype="nvfp4", device="cuda",
+              page_size=16, max_running_req=8, num_page_override=512, max_extend_tokens=256, cuda_graph_max_bs=-1, seed=0)
+    pool = llm.engine.kv_cache
+    layer_of = {pool.plane(i).data_ptr(): i for i in range(2)}
+    held = [torch.full((2, 513 * 16, kv_heads, dim), float("nan"), dtype=torch.float64) for _ in range(2)]     # keys, values
+    store, attend, slots, seen = ops.store_kv_fp4, ops.paged_attention_fp4, {}, dict(plan=0, none=0, decode=0, prefix=0)
+
+    def checked_store(k, v, cache, out_loc, *args):
+        store(k, v, cache, out_loc, *args)
+        layer = layer_of[cache.data_ptr()]
+        slots[layer] = out_loc.cpu().long()
+        for x, y, head in zip(held, (k, v), factors):
+            x[layer, slots[layer]] = plain.rounded(y, head[layer])
+
+    def checked_attend(q, cache, table, cu_q, lens, scale, **kw):
+        out = attend(q, cache, table, cu_q, lens, scale, **kw)
+        layer, cu, rows = layer_of[cache.data_ptr()], cu_q.tolist(), table.cpu().long()
+        for b, n in enumerate(lens.tolist()):
+            at = (rows[b, :-(-n // 16), None] * 16 + torch.arange(16)).flatten()[:n]
+            assert torch.equal(slots[layer][cu[b]:cu[b + 1]], at[n - (cu[b + 1] - cu[b]):])
+            assert not held[0][layer, at].isnan().any()
+        pages = [x[layer].view(513, 16, kv_heads, dim).transpose(1, 2) for x in held]
+        read = [x.cpu() for x in plain.values(cache, factors[0][layer], factors[1][layer])]
+        for x, y in zip(pages, read):
+            assert torch.equal(x[~x.isnan()], y[~x.isnan()])
+        assert window_free(kw)
+        want, tol, _, _ = plain.attention(q, *read, rows, cu_q, lens, scale)
+        if kw.get("plan") is not None:
+            # probabilities of 8 bits in place of 11: 2^-8 of the sum of weighted magnitudes more, the attention over the magnitudes
+            tol = tol + 2.0 ** -8 * plain.attention(q, read[0], read[1].abs(), rows, cu_q, lens, scale)[0]
+        off = (out.cpu().double() - want).abs()
+        assert (off <= tol).all(), float((off / tol).max())
+        kind = "decode" if kw["max_q"] == 1 else "plan" if kw.get("plan") is not None else "none"
+        seen[kind] += 1
+        seen["prefix"] += kw["max_q"] > 1 and int((lens - (cu_q[1:] - cu_q[:-1])).max()) > 0
+        return out
+
+    def window_free(kw):
+        return kw.get("window", 0) == 0 and kw.get("weights") is None
+
+    monkeypatch.setattr(ops, "store_kv_fp4", checked_store)
+    monkeypatch.setattr(ops, "paged_attention_fp4", checked_attend)
+    sp = SamplingParams(temperature=0.0, max_tokens=5, ignore_eos=True)
+    for _ in range(2):
+        assert all(len(o.token_ids) == 5 for o in llm.generate(_prompts([1, 16, 17, 300, 5, 700]), sp))
+    llm.shutdown()
+    assert seen["decode"] and seen["prefix"] and (seen["plan"] if dim < 256 else seen["none"])
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(8, 2, 128), (7, 1, 64)])
+def test_replays_with_padded_requests(hq, hk, dim):
+    """A captured step of eight requests (store, attention), replayed with 8, 5, 1 and 0 real ones: the others are padding (one token of a
+    spare page), as the engine pads. Real rows against the plain form; nothing but their slots and the spare page changes."""
+    import plain_kv_fp4 as plain
+    from minisglang_rdna4_b200 import ops
+
+    g = torch.Generator("cuda").manual_seed(dim)
+    pages, spare, width = 120, 119, 14
+    cache = torch.zeros(pages, hk, 1, 18 * dim, dtype=torch.uint8, device="cuda")
+    ks, vs = (2.0 ** torch.randint(-7, -4, (hk,), generator=g, device="cuda") for _ in range(2))
+    fill = [torch.randn(pages * 16, hk, dim, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    ops.store_kv_fp4(*fill, cache, torch.arange(pages * 16, dtype=torch.int32, device="cuda"), ks, vs)
+    k, v = (torch.zeros(8, hk, dim, device="cuda").bfloat16() for _ in range(2))
+    q = torch.zeros(8, hq, dim, device="cuda").bfloat16()
+    loc, lens, cu = torch.full((8,), spare * 16, dtype=torch.int32, device="cuda"), _ints([1] * 8), _ints(list(range(9)))
+    table = torch.full((8, width), spare, dtype=torch.int32, device="cuda")
+
+    def step():
+        ops.store_kv_fp4(k, v, cache, loc, ks, vs)
+        return ops.paged_attention_fp4(q, cache, table, cu, lens, 0.1, k_scale=ks, v_scale=vs, max_q=1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    order = torch.randperm(119, generator=g, device="cuda").int()
+    for real in (8, 5, 1, 0, 8):
+        n = torch.randint(1, 16 * width, (8,), generator=g, device="cuda").int()
+        n[real:] = 1
+        table.fill_(spare)
+        loc.fill_(spare * 16)
+        at = 0
+        for b in range(real):
+            need = -(-int(n[b]) // 16)
+            table[b, :need] = order[at:at + need]
+            at += need
+            loc[b] = int(table[b, need - 1]) * 16 + (int(n[b]) - 1) % 16
+        lens.copy_(n)
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        before = plain.values(cache, ks, vs)
+        graph.replay()
+        after = plain.values(cache, ks, vs)
+        slots = loc[:real].cpu().long()
+        for x, y, rows, head in zip(before, after, (k, v), (ks, vs)):
+            x, y = (z[:spare].transpose(1, 2).flatten(0, 1) for z in (x, y))
+            x[slots] = plain.rounded(rows[:real], head)
+            assert torch.equal(x, y)
+        want, tol, _, _ = plain.attention(q, *after, table, cu, lens, 0.1)
+        assert ((out.cpu().double() - want).abs() <= tol)[:real].all() and torch.isfinite(out).all()
