@@ -258,7 +258,7 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     ``budget`` tokens (``seq_lens [B]``, pages ``block_table [B, .]``) keeps, in every layer and key head on its own, its first
     ``sinks``, its last ``recent``, and of the others those with the largest weights (of equal ones the earlier; a NaN is
     larger than any number); a shorter one keeps all. What stays is copied in its order, rows and weights, to the pages
-    ``new_table [B, at least budget / page]``, which must not be among the pages of any request here; slots behind it and the old
+    ``new_table [B, at least budget / page]``, each of them there once and not among the pages of any request here; slots behind it and the old
     pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected to stay below (0: what the table holds); a longer request
     takes longer.
 
@@ -268,6 +268,8 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     shape = _, pages, hk, page, _ = F4.pool_shape(cache, True)
     F4.check_here(cache, weights, block_table, seq_lens, new_table)
     F4.check_weights(weights, cache, pages, hk, page)
+    F4.check_apart("the pool", cache, 4)
+    F4.check_apart("the attention weights", weights, 3)
     F4.check_ints("seq_lens", seq_lens)
     F4.check_ints("block_table", block_table, seq_lens.shape[0], 2)
     F4.check_ints("new_table", new_table, seq_lens.shape[0], 2)

@@ -89,6 +89,12 @@ def check_weights(weights: torch.Tensor, cache: torch.Tensor, pages: int, hk: in
         raise ValueError(f"attention weights are contiguous fp32 {want}, not {weights.dtype} {tuple(weights.shape)}")
 
 
+def check_apart(name: str, t: torch.Tensor, dims: int) -> None:
+    """Layers in front of ``dims`` dimensions lie in memory of their own."""
+    if t.dim() > dims and t.shape[0] > 1 and t.stride(0) < t[0].numel():
+        raise ValueError(f"the layers of {name} overlap")
+
+
 def check_rows(k: torch.Tensor, v: torch.Tensor, rows: int, hk: int, dim: int) -> None:
     if k.dtype is not v.dtype or (k.dtype not in _ROWS and (k.is_cuda or k.dtype is not torch.float32)):
         raise TypeError(f"rows of bf16 or fp16, keys and values alike, not {k.dtype} and {v.dtype}")

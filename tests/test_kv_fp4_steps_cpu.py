@@ -210,3 +210,17 @@ def test_a_wait_that_ran_out_over_the_4_bit_pool_is_a_status_of_attention(monkey
         assert cuda.attn_status(reset=False) == 401 and cuda.attn_status() == 401 and cuda.attn_status() == 0, name
     state.update(dict.fromkeys(state, 5))
     assert cuda.attn_status() == 5 and cuda.attn_status() == 0      # all are reset by one call
+
+
+def test_eviction_refuses_layers_that_overlap():
+    from minisglang_rdna4_b200 import ops
+
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    cache, weights = torch.zeros(2, 4, 1, 1, 18 * 64, dtype=torch.uint8), torch.zeros(2, 4, 1, 16)
+    half = torch.zeros(6, 1, 1, 18 * 64, dtype=torch.uint8).as_strided((2, 4, 1, 1, 18 * 64), (2 * 18 * 64, 18 * 64, 18 * 64, 18 * 64, 1))
+    args = (ints([[0, 1]]), ints([20]), ints([[2]]), 8, 2)
+    for c, w in ((cache[:1].expand(2, -1, -1, -1, -1), weights), (half, weights), (cache, weights[:1].expand(2, -1, -1, -1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.evict_kv_fp4(c, w, *args)
+    assert ops.evict_kv_fp4(cache, weights, *args)[1].tolist() == [8]
+    assert ops.evict_kv_fp4(cache[:1].expand(1, -1, -1, -1, -1), weights[:1], *args)[1].tolist() == [8]
