@@ -503,7 +503,8 @@ bool shape_ok(int hk, int d, int page_size, long long pages, const void* pool, c
 }
 
 uint32_t magic(int per) { return (uint32_t)(((1ull << 32) + per - 1) / per); }
-int rows_of_a_thread(long long rows, int hk, int d) { return rows * hk * (d / 8) > 148ll * 2048 * 2 ? 4 : 1; }
+// four where threads of one row each would fill the GPU (2048 threads an SM) more than twice over
+int rows_of_a_thread(long long rows, int hk, int d) { return rows * hk * (d / 8) > 2ll * 2048 * device_sms() ? 4 : 1; }
 
 }  // namespace
 
