@@ -91,7 +91,7 @@ def check_weights(weights: torch.Tensor, cache: torch.Tensor, pages: int, hk: in
 
 def check_apart(name: str, t: torch.Tensor, dims: int) -> None:
     """Layers in front of ``dims`` dimensions lie in memory of their own."""
-    if t.dim() > dims and t.shape[0] > 1 and t.stride(0) < t[0].numel():
+    if t.dim() > dims and t.shape[0] > 1 and t.stride(0) < t.numel() // t.shape[0]:
         raise ValueError(f"the layers of {name} overlap")
 
 
