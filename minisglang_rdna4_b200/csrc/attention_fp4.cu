@@ -14,11 +14,11 @@
 // so that they are normal numbers down to 2^-21 of the largest; the maximum moves only when a score passes it by 2^8, which
 // the factor leaves room for (2^15).
 //
-// Bound: instructions. A tile of 16 tokens of 128 channels takes a warp about 290, of which 209 widen and multiply: 64 conversions
-// and 64 products with scales for 4096 values are what 4 bits cost over 8. At 0.6 of them a cycle and scheduler (the ALU half
-// busy with conversions) an SM takes 15 bytes a clock of the 23 that DRAM has for it. B200: 4 requests of 70 to 120 thousand
-// tokens, 8 key heads of 128, 103 us, 4.4 TB/s; 256 of 500 to 2300 117 us, 3.6 TB/s; 64 of them 39 us, 2.7 TB/s (4 us until the
-// first tiles come, 5 for the joins). Tried on the first: 16 warps an SM with 128 registers in place of 12 with 168 (105 to 107),
+// Bound: a warp's own chain of instructions. A tile of 16 tokens of 128 channels takes a warp about 290, of which 209 widen and
+// multiply: 64 conversions and 64 products with scales for 4096 values are what 4 bits cost over 8. The 12 warps that fit on an SM
+// issue 0.56 of them a cycle and scheduler (issue slots 56 % busy, the ALU pipe 53 %, neither full), and an SM takes 15 bytes a clock of
+// the 23 that DRAM has for it. B200, in a graph: 4 requests of 70 to 120 thousand tokens, 8 key heads of 128, 103 us, 4.3 TB/s; 256 of
+// 500 to 2300 120 us, 3.4 TB/s; 64 of them 40 us, 2.7 TB/s (4 us until the first tiles come, 5 for the joins). Tried on the first: 16 warps an SM with 128 registers in place of 12 with 168 (105 to 107),
 // 20 with 96 (spills, 127), the next pair's scores between this pair's values (105), parts joined by a second kernel (105), by all
 // warps of the last CTA (101, but the 64 requests 43).
 #include "kv_fp4.cuh"
@@ -161,7 +161,8 @@ template <typename V> __device__ __forceinline__ V scan(V v, V* sums, V& all) {
 
 // `few` > 0: units may be cut into pieces of their own. The tiles of all units are dealt evenly then only if there are many: a
 // CTA with the end of one unit and the beginning of another has two units to wait for, which counts where they are short.
-// B200, us, dealt -> cut, 32 query and 8 key heads of 128: one request of 700 tokens 16.4 -> 12.4, 8 of 100 to 300 16.6 -> 12.5.
+// B200, us, dealt -> cut when the cut was added, 32 query and 8 key heads of 128: one request of 700 tokens 16.4 -> 12.4, 8 of 100 to 300
+// 16.6 -> 12.5 (in a graph, both 10.2 now).
 __device__ __forceinline__ void lay_line(const Fp4Args& a, Line& line, bool whole_rows, int few) {
   __shared__ long long sums[kWarps];
   __shared__ int sums32[2][kWarps];
@@ -1136,7 +1137,8 @@ fp4_gather_kernel(const Fp4Args a, T* __restrict__ kc, T* __restrict__ vt, const
 
 // NaN values of a prompt step. The product of probabilities and values would give one that only later rows of a block see to the
 // earlier ones too (0 * NaN), so the gather leaves zeros in their place and this kernel writes the NaNs over the output of the rows
-// that see them: 16 channels of a value each. Without any, which is nearly always, it reads a tile's value scales and is done.
+// that see them: 16 channels of a value each. Without any, which is nearly always, it reads a tile's value scales and is done: 553 us of two prompts
+// of some 2000 rows behind prefixes stay 553.
 template <typename T, int D> __global__ void __launch_bounds__(256)
 fp4_prompt_nans_kernel(const Fp4Args a, T* __restrict__ out, const int* __restrict__ items, int n_items, const int* __restrict__ blk_req,
                        const int* __restrict__ req_info, int tiles) {

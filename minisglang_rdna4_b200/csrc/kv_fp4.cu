@@ -24,7 +24,7 @@ struct RowArgs {
 // A thread has 8 channels of a key and of its value (16-byte accesses; D / 8 threads for a row and head) in U rows that follow
 // each other, so that their loads are under way at once: four where the rows fill the GPU all the same, else one. B200, us, store
 // and load with one row a thread and with four: 64 rows of 8 heads of 128 6.2, 13.8; 8192 rows 41.8, 35.7 (with a key or value a
-// thread; both in one thread 30.4).
+// thread; both in one thread now 27.8, of 64 rows 4.1).
 template <int D, int U> struct Place {
   int h, c, row0;           // c: channels 8 c .. 8 c + 7
   int code_at[2], sf_at[2]; // the channels' part of where they lie in a tile, of keys and of values
@@ -85,8 +85,9 @@ template <typename T> __device__ __forceinline__ uint32_t quantise8(const Vec8<T
   return w;
 }
 
-// Bound: the 32 bytes in and 9 out of a thread and row; the 9 lie in pieces of 4 bytes (a value's in 8 sectors of 32), which costs
-// more than their number: 8192 rows of 8 heads of 128 take 20 us, 2.2 TB/s.
+// Floor: the 32 bytes in and 9 out of a thread and row. Bound: the chain from a row's loads over its scale, quotients, rounding and
+// packing to writes of 4 bytes (a value's in 8 sectors of 32): issue slots 64 % busy, the ALU pipe 53 %, neither full. 8192 rows of 8
+// heads of 128 take 17.5 us, 2.5 TB/s.
 template <typename T, int D, int U> __global__ void __launch_bounds__(256) store_fp4_kernel(const RowArgs a) {
   const Place<D, U> p(a);
   pdl_enter();

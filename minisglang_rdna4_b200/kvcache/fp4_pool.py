@@ -17,7 +17,8 @@ import torch
 from .base import BaseKVCachePool
 
 #: Factor of a head that nothing is known of: values up to 168 (2688 / 16) keep their block's scale, and blocks down to 0.006 have
-#: a normal one (6 * 2^-6 / 16).
+#: a normal one (6 * 2^-6 / 16). Its cost: what is larger saturates, where an 8-bit pool holds 448 (a factor of 1 / 6, with
+#: which blocks below 0.016 would lose bits of their scale). Heads that pass 168 need a calibrated factor.
 DEFAULT_SCALE = 1.0 / 16
 
 

@@ -208,8 +208,9 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale: float, *, 
 
     ``q [T, Hq, D]`` (bf16 or fp16, on a CPU fp32 too); request b has the rows ``cu_q[b]:cu_q[b + 1]`` (int32), the last positions of its
     ``seq_lens[b]`` tokens, whose pages are ``block_table[b]`` (int32). ``window`` > 0: a row sees that many positions, its own
-    included. A row that sees nothing gives zeros. ``max_q`` (rows of the longest request; 0: read from the device) may be
-    larger than what the step has; ``max_kv`` likewise.
+    included. A row that sees nothing gives zeros; rows in front of the first request and behind the last one are not written. A NaN key
+    or value reaches the rows that see it. ``max_q`` (rows of the longest request; 0: read from the device) may be larger than what the
+    step has. ``max_kv`` is taken as ``paged_attention`` takes it; no form over this pool needs it.
 
     ``weights [pages, Hk, page]`` (fp32): the softmax weights that the rows give a token, summed over the rows and the query
     heads of its key head, are added to the token's. (A page that several requests of the step share has them added in any
@@ -258,9 +259,9 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     ``budget`` tokens (``seq_lens [B]``, pages ``block_table [B, .]``) keeps, in every layer and key head on its own, its first
     ``sinks``, its last ``recent``, and of the others those with the largest weights (of equal ones the earlier; a NaN is
     larger than any number); a shorter one keeps all. What stays is copied in its order, rows and weights, to the pages
-    ``new_table [B, at least budget / page]``, each of them there once and not among the pages of any request here; slots behind it and the old
-    pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected to stay below (0: what the table holds); a longer request
-    takes longer.
+    ``new_table [B, at least budget / page]``, each of them there once and not among the pages of any request here; slots behind it
+    and the old pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected
+    to stay within (0: what the table holds); a longer request takes longer.
 
     Returns ``(kept [(layers,) B, Hk, budget] int32: token indices in order, -1 behind them, new lengths [B] int32)``. Later steps
     go on behind the new lengths, at the positions that their tokens have in the text."""
