@@ -225,3 +225,42 @@ def test_replays_with_padded_requests(hq, hk, dim):
             assert torch.equal(x, y)
         want, tol, _, _ = plain.attention(q, *after, table, cu, lens, 0.1)
         assert ((out.cpu().double() - want).abs() <= tol)[:real].all() and torch.isfinite(out).all()
+
+
+def test_layers_that_differ_in_query_heads_serve_prompts(monkeypatch):
+    """Layers of one window with 4 and with 8 query heads a key head: each takes the form for prompts with a plan of its own, and the
+    output of every call is that of a plain form."""
+    import plain_kv_fp4 as plain
+    from minisglang_rdna4_b200 import SamplingParams, ops
+    from minisglang_rdna4_b200.llm import LLM
+    from minisglang_rdna4_b200.models.config import ModelConfig
+
+    rope = {kind: {"rope_type": "default", "rope_theta": 10000.0} for kind in ("full_attention", "sliding_attention")}
+    config = ModelConfig.from_hf(dict(
+        model_type="laguna", architectures=["LagunaForCausalLM"], hidden_size=512, num_attention_heads=8,
+        num_attention_heads_per_layer=[8, 16, 16, 8], num_key_value_heads=2, head_dim=64, intermediate_size=512,
+        moe_intermediate_size=256, shared_expert_intermediate_size=256, num_experts=8, num_experts_per_tok=2, norm_topk_prob=True,
+        routed_scaling_factor=1.0, first_k_dense_replace=1, vocab_size=2048, num_hidden_layers=4,
+        layer_types=["full_attention", "full_attention", "sliding_attention", "sliding_attention"], sliding_window=100,
+        rms_norm_eps=1e-6, rope_parameters=rope, max_position_embeddings=2048, tie_word_embeddings=False, hidden_act="silu"))
+    llm = LLM(model_config=config, use_dummy_weight=True, kv_cache_dtype="nvfp4", device="cuda", page_size=16, max_running_req=4,
+              num_page_override=256, max_extend_tokens=512, cuda_graph_max_bs=-1, seed=0)
+    attend, seen = ops.paged_attention_fp4, set()
+
+    def checked(q, cache, table, cu_q, lens, scale, **kw):
+        out = attend(q, cache, table, cu_q, lens, scale, **kw)
+        read = plain.values(cache, kw["k_scale"], kw["v_scale"])
+        rows = table.cpu().long()
+        want, tol, _, _ = plain.attention(q, *read, rows, cu_q, lens, scale, kw["window"])
+        if kw["plan"] is not None:
+            seen.add((q.shape[1], kw["window"]))
+            # probabilities of 8 bits in place of 11: 2^-8 of the sum of weighted magnitudes more, the attention over the magnitudes
+            tol = tol + 2.0 ** -8 * plain.attention(q, read[0], read[1].abs(), rows, cu_q, lens, scale, kw["window"])[0]
+        assert ((out.cpu().double() - want).abs() <= tol).all()
+        return out
+
+    monkeypatch.setattr(ops, "paged_attention_fp4", checked)
+    out = llm.generate(_prompts([300, 700, 40]), SamplingParams(temperature=0.0, max_tokens=4, ignore_eos=True))
+    llm.shutdown()
+    assert all(len(o.token_ids) == 4 for o in out)
+    assert seen == {(8, 0), (16, 0), (16, 100), (8, 100)}
