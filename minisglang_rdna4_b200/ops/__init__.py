@@ -259,8 +259,8 @@ def evict_kv_fp4(cache, weights, block_table, seq_lens, new_table, budget: int, 
     ``budget`` tokens (``seq_lens [B]``, pages ``block_table [B, .]``) keeps, in every layer and key head on its own, its first
     ``sinks``, its last ``recent``, and of the others those with the largest weights (of equal ones the earlier; a NaN is
     larger than any number); a shorter one keeps all. What stays is copied in its order, rows and weights, to the pages
-    ``new_table [B, at least budget / page]``, each of them there once and not among the pages of any request here; slots behind it
-    and the old pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected
+    ``new_table [B, at least budget / page]``; a page that rows go to is there once and not among the pages of any request here. Slots
+    behind them and the old pages stay as they are. What would go to a page outside the pool is dropped. ``max_kv``: what ``seq_lens`` are expected
     to stay within (0: what the table holds); a longer request takes longer.
 
     Returns ``(kept [(layers,) B, Hk, budget] int32: token indices in order, -1 behind them, new lengths [B] int32)``. Later steps

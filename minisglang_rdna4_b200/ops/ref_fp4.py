@@ -122,9 +122,10 @@ def paged_attention_fp4(q, cache, block_table, cu_q, seq_lens, scale, k_scale=No
             hidden = hidden | (i <= pos - window)
         s = s.masked_fill(hidden, float("-inf"))
         p = torch.softmax(s, -1).masked_fill(hidden, 0.0)
-        o = torch.einsum("hgqn,nhd->qhgd", p, vv.nan_to_num(0.0))
-        if vv.isnan().any():                                  # a NaN reaches the rows that see it, no others
-            o = o.masked_fill(torch.einsum("qn,nhd->qhd", (~hidden).float(), vv.isnan().float())[:, :, None] > 0, float("nan"))
+        none = vv.isnan()
+        o = torch.einsum("hgqn,nhd->qhgd", p, vv.masked_fill(none, 0.0))
+        if none.any():                                        # a NaN reaches the rows that see it, no others
+            o = o.masked_fill(torch.einsum("qn,nhd->qhd", (~hidden).float(), none.float())[:, :, None] > 0, float("nan"))
         out[cu[b]:cu[b + 1]] = o.reshape(q_len, hq, dim)
         if weights is not None:
             weights[pages[i // page], :, i % page] += p.sum((1, 2)).T
