@@ -264,3 +264,33 @@ def test_layers_that_differ_in_query_heads_serve_prompts(monkeypatch):
     llm.shutdown()
     assert all(len(o.token_ids) == 4 for o in out)
     assert seen == {(8, 0), (16, 0), (16, 100), (8, 100)}
+
+
+def test_a_captured_prompt_keeps_its_scratch():
+    """A prompt over the 16-bit pool in a graph gathers into memory of the graph: longer prompts behind the capture neither free nor
+    overwrite it."""
+    import numpy as np
+
+    from minisglang_rdna4_b200.ops import cuda as K
+
+    g = torch.Generator("cuda").manual_seed(0)
+    pool = [torch.randn(700, 2, 16, 128, generator=g, device="cuda").bfloat16() for _ in range(2)]
+
+    def prompt(n):
+        q = torch.randn(n, 8, 128, generator=torch.Generator("cuda").manual_seed(n), device="cuda").bfloat16()
+        table = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
+        plan = K.PrefillPlan(np.array([0, n]), np.array([n]), q.device)
+        return lambda: K.paged_attention(q, *pool, table, None, None, 0.1, max_q=n, max_kv=n, plan=plan)
+
+    short, long = prompt(900), prompt(11000)
+    want = short()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = short()
+    first = long().clone()
+    junk = [torch.full((1 << 22,), float("nan"), device="cuda") for _ in range(8)]
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(got, want) and torch.equal(long(), first)
+    assert len(junk) == 8
